@@ -57,6 +57,16 @@ _SIGNATURES = {
     "cubk_mean_pool_static_scratch": (_I, [_P, _I, _I, _I, _I, _P, _P]),
     "cubk_logits_probs_{t}": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _P]),
     "cubk_pooler_head_{t}": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P]),
+    "cubk_residual_rms_norm_{t}": (_I, [_P, _P, _P, _L, _I, _F, _P, _P, _P]),
+    "cubk_residual_rms_norm_e4m3_{t}": (_I, [_P, _P, _P, _L, _I, _F, _I, _P, _P, _P, _P]),
+    "cubk_w4_packed_bytes": (_Z, [_I, _I]),
+    "cubk_w4_quantize_{t}": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "cubk_w4_pack": (_I, [_P, _I, _I, _P, _P]),
+    "cubk_w4_matvec_{t}": (_I, [_P, _I, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "cubk_w4_matvec_e4m3_{t}": (_I, [_P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "cubk_window_attention_{t}": (_I, [_P, _P, _P, _L, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P]),
+    "cubk_window_attention_step_{t}": (_I, [_P, _P, _P, _L, _L, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _L, _P]),
+    "cubk_window_cache_fill_{t}": (_I, [_P, _P, _L, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
     "cubk_not_{t}": (_I, [_P, _P, _L, _P]),
     "cubk_half_to_float": (_I, [_P, _P, _L, _P]),
 }

@@ -276,6 +276,99 @@ int cubk_pooler_head_f16(const void *x, const void *pooler_bias, const void *wei
                          int batch, int hidden, int labels, void *pooled, void *logits, void *probs,
                          void *stream);
 
+/* ---- K6: residual + root-mean-square norm -----------------------------------------------------------
+ * t = x (+ residual);  y = t / sqrt(mean(t^2) + eps) * gamma
+ * The norm of encoders and decoders that centre nothing; no counterpart in the reference, whose layers use K2.
+ * x, residual [rows, channels], gamma [channels]; residual may be NULL. `sum` [rows, channels] receives t, rounded
+ * to the storage type (the residual of the next layer), and may be NULL; y is computed from the unrounded t.
+ * sum or out may be x or residual itself (the in-place forms); any other overlap is not allowed.
+ * The _e4m3 calls store y in 8 bits: codes [rows, channels] e4m3 (4 exponent, 3 mantissa bits, no infinities), round
+ * to nearest even, and float32 scales with y = code * scale, scale = max|y| / 448 over the whole row (group = 0,
+ * scales [rows]) or over blocks of 128 columns (group = 128, scales [rows, ceil(channels / 128)], the last block as
+ * short as the row leaves it). A group whose largest |y| is below 2^-100 is stored as zeros with scale 0. A NaN in a
+ * group makes its scale and codes NaN. The e4m3 codes are what cubk_w4_matvec_e4m3_* and 8-bit library products read.
+ * eps >= 0; a row of zeros under eps = 0 gives NaN. */
+int cubk_residual_rms_norm_f32(const float *x, const float *residual, const float *gamma, int64_t rows, int channels, float eps,
+                               float *sum, float *out, void *stream);
+int cubk_residual_rms_norm_f16(const void *x, const void *residual, const void *gamma, int64_t rows, int channels, float eps,
+                               void *sum, void *out, void *stream);
+int cubk_residual_rms_norm_e4m3_f32(const float *x, const float *residual, const float *gamma, int64_t rows, int channels, float eps,
+                                    int group, float *sum, void *codes, float *scales, void *stream);
+int cubk_residual_rms_norm_e4m3_f16(const void *x, const void *residual, const void *gamma, int64_t rows, int channels, float eps,
+                                    int group, void *sum, void *codes, float *scales, void *stream);
+
+/* ---- K7: products of a few rows with 4-bit weights --------------------------------------------------
+ * out[m,n] = sum_k x[m,k] * code[n,k] * scale[k / group, n] (+ bias[n]),  code in -8..7,  group 32, 64 or 128
+ * For requests of a few tokens, whose dense products do nothing but read weights. No counterpart in the reference,
+ * whose products are float32 or binary16 library calls (src/cuBERT/op/Dense.cpp:41-52). Any number of rows is
+ * computed; from about a hundred on, a library product on unpacked weights is the better call.
+ * x [rows, k], bias [n] (or NULL), out [rows, n] and the scales [ceil(k / group), n] in the storage type. Sums are
+ * float32; a code times its scale is never rounded.
+ * The _e4m3 calls take x as the 8-bit codes and scales K6 writes: code_scales [rows] (code_group = 0) or
+ * [rows, ceil(k / 128)] (code_group = 128).
+ * packed: cubk_w4_packed_bytes(n, k) bytes on a 16-byte boundary (CUBK_ERR_UNSUPPORTED otherwise), laid out once by
+ * one of the calls below, in tiles of 16 rows x 128 columns (1 KB), those of the same 16 rows next to each other. Row
+ * r of a tile is 16 little-endian 32-bit words from byte 64 r; word 4 t + j holds columns 32 j + 8 t .. + 7, column
+ * 2 i of them in bits 4 i .. 4 i + 3 and column 2 i + 1 in bits 16 + 4 i .. 16 + 4 i + 3, as code + 8. Rows and columns
+ * past the matrix hold code 0 (8).
+ *   cubk_w4_quantize_*  rounds weights [n, k] to codes: scale = max|w| / 7 over a group of a row, rounded to the
+ *                       storage type; code = w / scale to the nearest whole number (a tie to the even one)
+ *   cubk_w4_pack        takes codes [n, k], one int8 in -8..7 each, from elsewhere */
+size_t cubk_w4_packed_bytes(int n, int k);
+int cubk_w4_quantize_f32(const float *weights, int n, int k, int group, void *packed, float *scales, void *stream);
+int cubk_w4_quantize_f16(const void *weights, int n, int k, int group, void *packed, void *scales, void *stream);
+int cubk_w4_pack(const int8_t *codes, int n, int k, void *packed, void *stream);
+int cubk_w4_matvec_f32(const float *x, int rows, int k, const void *packed, const float *scales, int group, int n, const float *bias,
+                       float *out, void *stream);
+int cubk_w4_matvec_f16(const void *x, int rows, int k, const void *packed, const void *scales, int group, int n, const void *bias,
+                       void *out, void *stream);
+int cubk_w4_matvec_e4m3_f32(const void *codes, const float *code_scales, int code_group, int rows, int k, const void *packed,
+                            const float *scales, int group, int n, const float *bias, float *out, void *stream);
+int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int code_group, int rows, int k, const void *packed,
+                            const void *scales, int group, int n, const void *bias, void *out, void *stream);
+
+/* ---- K8: attention with a sliding window and sinks ----------------------------------------------------
+ * Query i of a sequence sees key j when mask[b, j] != 0 (or mask is NULL), j <= i + after, and j >= i - before or
+ * j < sinks: a window around the query plus the sequence's first tokens, which stay visible from any distance.
+ *   context[i] = sum_j softmax_j(scale * q_i . k_j) v_j over the keys i sees; zeros when it sees none
+ * after = 0 is the causal form of decoders; before = after = w the local attention of encoders for long documents
+ * (sinks = 1: every token also sees [CLS]); before >= seq lifts the window. Unlike K4, a masked key is left out rather
+ * than lowered by 10000, whatever its rows hold (infinities and NaN included). The reference attends to every key of
+ * at most 512 (src/cuBERT/op_att/AttentionSelf.cpp:96-111); cubk_attention_small_* ends at 128 positions.
+ * Token s of sequence b is row b * seq + s of q, k, v and context; rows are q_stride (q), kv_stride (k and v) and
+ * context_stride elements apart, so the three may be parts of one projection's output. Head h of a row is at column
+ * h * head_dim and reads key/value head h / (heads / kv_heads); heads must be a multiple of kv_heads. head_dim is 1
+ * to 256 (CUBK_ERR_UNSUPPORTED beyond). mask int8 [batch, seq]. context must not overlap the inputs. */
+int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
+                              int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,
+                              float *context, int64_t context_stride, void *stream);
+int cubk_window_attention_f16(const void *q, const void *k, const void *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
+                              int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,
+                              void *context, int64_t context_stride, void *stream);
+
+/* K8 for one new token of each of `batch` streams. The keys and values a stream can still see live in a ring of
+ * sinks + window slots, k_cache and v_cache [batch, kv_heads, sinks + window, head_dim]: position p sits in slot p
+ * below sinks and in slot sinks + (p - sinks) % window from there on. positions[b] (device int32) is the number of
+ * tokens stream b has seen before this one; the call stores row b of k and v in that position's slot and writes the
+ * attention of row b of q over the stream's first min(position + 1, sinks + window) slots to row b of context: the
+ * causal form above with before = window - 1. A stream with a negative position is idle: its cache and its row of
+ * context are left as they are. Slots that no position has reached may hold anything. Positions are read on the
+ * device, so a captured call can be replayed as they advance; calls that share a cache must be ordered. */
+int cubk_window_attention_step_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride,
+                                   const int32_t *positions, int batch, int heads, int kv_heads, int head_dim, int window, int sinks,
+                                   float scale, float *k_cache, float *v_cache, float *context, int64_t context_stride, void *stream);
+int cubk_window_attention_step_f16(const void *q, const void *k, const void *v, int64_t q_stride, int64_t kv_stride,
+                                   const int32_t *positions, int batch, int heads, int kv_heads, int head_dim, int window, int sinks,
+                                   float scale, void *k_cache, void *v_cache, void *context, int64_t context_stride, void *stream);
+
+/* The ring caches of `batch` streams after a prompt: of the first lengths[b] (device int32, clamped to 0..seq; NULL:
+ * seq) tokens of sequence b, rows b * seq .. of k and v, the sinks and the last `window` ones go to their slots. The
+ * other slots are left as they are. The stream's next position is lengths[b]. */
+int cubk_window_cache_fill_f32(const float *k, const float *v, int64_t kv_stride, const int32_t *lengths, int batch, int seq, int kv_heads,
+                               int head_dim, int window, int sinks, float *k_cache, float *v_cache, void *stream);
+int cubk_window_cache_fill_f16(const void *k, const void *v, int64_t kv_stride, const int32_t *lengths, int batch, int seq, int kv_heads,
+                               int head_dim, int window, int sinks, void *k_cache, void *v_cache, void *stream);
+
 /* ---- helpers ------------------------------------------------------------------------------------
  * out[i] = !in[i] as 0/1 in the storage type. Replaces _not<T> (src/cuBERT/op_att/AttentionMask.h:9). */
 int cubk_not_f32(const int8_t *in, float *out, int64_t n, void *stream);
