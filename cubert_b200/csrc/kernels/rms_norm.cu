@@ -95,6 +95,197 @@ rms_norm_generic_kernel(const T *x, const T *residual, const T *gamma, int64_t r
     }
 }
 
+enum NormOut { NORM_SAME, NORM_E4M3_ROW, NORM_E4M3_128 };
+
+// Largest magnitude over WIDTH adjacent lanes, NaN if any is.
+template <int WIDTH>
+__device__ __forceinline__ float group_max_nan(float v) {
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) {
+        v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    }
+    return v;
+}
+
+// Rows of whole 16-byte vectors: a row stays in the registers of TPR threads (a warp, or a block), VPT vectors each, so x and
+// residual are read once and every output is written once: the kernel is bound by those bytes. Blocks are persistent: a thread's
+// columns do not change, and neither do its gamma registers.
+template <typename T, int TPR, int VPT, NormOut OUT>
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
+rms_norm_kernel(const T *x, const T *residual, const T *gamma, int64_t rows, int channels, int nvec, float eps, T *sum, T *out, uint8_t *codes,
+                float *scales) {
+    constexpr int BLOCK = TPR == 32 ? 128 : TPR, EPV = Vec<T>::EPV, PAIRS = Vec2<T>::PAIRS, WARPS = TPR / 32;
+    __shared__ float red[2][WARPS];
+    const int l = TPR == 32 ? threadIdx.x & 31 : threadIdx.x;
+    uint4 graw[VPT];
+#pragma unroll
+    for (int u = 0; u < VPT; ++u) {
+        graw[u] = l + u * TPR < nvec ? ld_param(gamma + (size_t) (l + u * TPR) * EPV) : make_uint4(0, 0, 0, 0);
+    }
+    const float inv_channels = 1.f / (float) channels;
+    const int64_t stride = (int64_t) gridDim.x * (BLOCK / TPR);
+    for (int64_t row = (int64_t) blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR; row < rows; row += stride) {
+        const int64_t base = row * channels;
+        uint4 xr[VPT], rr[VPT];
+#pragma unroll
+        for (int u = 0; u < VPT; ++u) {
+            xr[u] = l + u * TPR < nvec ? ld_stream(x + base + (size_t) (l + u * TPR) * EPV) : make_uint4(0, 0, 0, 0);
+        }
+        if (residual != nullptr) {
+#pragma unroll
+            for (int u = 0; u < VPT; ++u) {
+                rr[u] = l + u * TPR < nvec ? ld_stream(residual + base + (size_t) (l + u * TPR) * EPV) : make_uint4(0, 0, 0, 0);
+            }
+        }
+        float2 t[VPT][PAIRS];
+        float2 ss2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < VPT; ++u) {
+            Vec2<T>::unpack(xr[u], t[u]);
+            if (residual != nullptr) {
+                accumulate_vec<T, false>(rr[u], t[u]);
+            }
+#pragma unroll
+            for (int e = 0; e < PAIRS; ++e) {
+                ss2 = fma2(t[u][e], t[u][e], ss2);
+            }
+        }
+        float ss = group_sum<32>(ss2.x + ss2.y);
+        if (WARPS > 1) {
+            __syncthreads();   // the row before is done with `red`
+            if ((threadIdx.x & 31) == 0) {
+                red[0][threadIdx.x >> 5] = ss;
+            }
+            __syncthreads();
+            ss = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                ss += red[0][w];
+            }
+        }
+        if (sum != nullptr) {
+#pragma unroll
+            for (int u = 0; u < VPT; ++u) {
+                if (l + u * TPR < nvec) {
+                    st_vec(sum + base + (size_t) (l + u * TPR) * EPV, Vec2<T>::pack(t[u]));
+                }
+            }
+        }
+        const float2 rstd2 = splat2(1.f / sqrtf(ss * inv_channels + eps));
+        float top[VPT];
+#pragma unroll
+        for (int u = 0; u < VPT; ++u) {
+            float2 gm[PAIRS];
+            Vec2<T>::unpack(graw[u], gm);
+            top[u] = 0.f;
+#pragma unroll
+            for (int e = 0; e < PAIRS; ++e) {
+                t[u][e] = mul2(mul2(t[u][e], rstd2), gm[e]);
+                if (OUT != NORM_SAME && l + u * TPR < nvec) {
+                    top[u] = max_nan(top[u], max_nan(fabsf(t[u][e].x), fabsf(t[u][e].y)));
+                }
+            }
+        }
+        float2 sc = make_float2(0.f, 0.f);
+        if (OUT == NORM_E4M3_ROW) {
+            float all = top[0];
+#pragma unroll
+            for (int u = 1; u < VPT; ++u) {
+                all = max_nan(all, top[u]);
+            }
+            all = group_max_nan<32>(all);
+            if (WARPS > 1) {
+                if ((threadIdx.x & 31) == 0) {
+                    red[1][threadIdx.x >> 5] = all;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    all = max_nan(all, red[1][w]);
+                }
+            }
+            sc = e4m3_scale(all);
+            if (l == 0) {
+                scales[row] = sc.x;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < VPT; ++u) {
+            const int idx = l + u * TPR;
+            if (OUT == NORM_SAME) {
+                if (idx < nvec) {
+                    st_vec(out + base + (size_t) idx * EPV, Vec2<T>::pack(t[u]));
+                }
+                continue;
+            }
+            if (OUT == NORM_E4M3_128) {   // 128 columns: 16 or 32 adjacent lanes
+                constexpr int LANES = 128 / EPV;
+                sc = e4m3_scale(group_max_nan<LANES>(top[u]));
+                if (idx < nvec && idx % LANES == 0) {
+                    scales[row * ((channels + 127) / 128) + idx / LANES] = sc.x;
+                }
+            }
+            if (idx < nvec) {
+                const float2 by = splat2(sc.y);
+                uint32_t w[PAIRS / 2];
+#pragma unroll
+                for (int e = 0; e < PAIRS; e += 2) {
+                    const float2 a = mul2(t[u][e], by), z = mul2(t[u][e + 1], by);
+                    w[e / 2] = (uint32_t) e4m3_pair(a.x, a.y) | (uint32_t) e4m3_pair(z.x, z.y) << 16;
+                }
+                if (PAIRS == 4) {
+                    *reinterpret_cast<uint2 *>(codes + base + (size_t) idx * EPV) = make_uint2(w[0], w[PAIRS / 2 - 1]);
+                } else {
+                    *reinterpret_cast<uint32_t *>(codes + base + (size_t) idx * EPV) = w[0];
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int TPR, int VPT, NormOut OUT>
+int rms_norm_launch(const T *x, const T *residual, const T *gamma, int64_t rows, int channels, float eps, T *sum, T *out, uint8_t *codes,
+                    float *scales, cudaStream_t stream) {
+    constexpr int BLOCK = TPR == 32 ? 128 : TPR, ROWS = BLOCK / TPR;
+    static OccupancyCache cache;
+    const int64_t resident = resident_blocks(rms_norm_kernel<T, TPR, VPT, OUT>, BLOCK, 0, &cache), want = (rows + ROWS - 1) / ROWS;
+    rms_norm_kernel<T, TPR, VPT, OUT><<<(unsigned) (want < resident ? want : resident), BLOCK, 0, stream>>>(
+        x, residual, gamma, rows, channels, channels / Vec<T>::EPV, eps, sum, out, codes, scales);
+    return check_launch();
+}
+
+// By the vectors of a row: a warp per row up to four vectors a lane (eight of float32), a block of 128 to 512 threads beyond.
+// False: longer rows, for the general kernel.
+template <typename T, NormOut OUT>
+bool rms_norm_vectors(const T *x, const T *residual, const T *gamma, int64_t rows, int channels, float eps, T *sum, T *out, uint8_t *codes,
+                      float *scales, cudaStream_t stream, int *rc) {
+    const int nvec = channels / Vec<T>::EPV;
+#define NORM(TPR, VPT) (*rc = rms_norm_launch<T, TPR, VPT, OUT>(x, residual, gamma, rows, channels, eps, sum, out, codes, scales, stream))
+    if (nvec <= 32) {
+        NORM(32, 1);
+    } else if (nvec <= 64) {
+        NORM(32, 2);
+    } else if (nvec <= 128) {
+        NORM(32, 4);
+    } else if (nvec <= 256) {
+        if constexpr (sizeof(T) == 4) {
+            NORM(32, 8);
+        } else {
+            NORM(128, 2);
+        }
+    } else if (nvec <= 512) {
+        NORM(128, 4);
+    } else if (nvec <= 1024) {
+        NORM(256, 4);
+    } else if (nvec <= 2048) {
+        NORM(512, 4);
+    } else {
+        return false;
+    }
+#undef NORM
+    return true;
+}
+
 template <typename T, bool E4M3>
 int residual_rms_norm(const T *x, const T *residual, const T *gamma, int64_t rows, int channels, float eps, int group, T *sum,
                       T *out, uint8_t *codes, float *scales, cudaStream_t stream) {
@@ -104,6 +295,20 @@ int residual_rms_norm(const T *x, const T *residual, const T *gamma, int64_t row
     }
     if (rows == 0) {
         return CUBK_OK;
+    }
+    constexpr int EPV = Vec<T>::EPV;
+    if (channels % EPV == 0 && aligned16(x) && aligned16(residual) && aligned16(gamma) && aligned16(sum) && aligned16(out) && aligned8(codes)) {
+        int rc = CUBK_OK;
+        bool taken;
+        if constexpr (E4M3) {
+            taken = group == 0 ? rms_norm_vectors<T, NORM_E4M3_ROW>(x, residual, gamma, rows, channels, eps, sum, out, codes, scales, stream, &rc)
+                               : rms_norm_vectors<T, NORM_E4M3_128>(x, residual, gamma, rows, channels, eps, sum, out, codes, scales, stream, &rc);
+        } else {
+            taken = rms_norm_vectors<T, NORM_SAME>(x, residual, gamma, rows, channels, eps, sum, out, codes, scales, stream, &rc);
+        }
+        if (taken) {
+            return rc;
+        }
     }
     const unsigned blocks = (unsigned) (rows < 148 * 8 ? rows : 148 * 8);
     rms_norm_generic_kernel<T, E4M3><<<blocks, kRmsGenericBlock, 0, stream>>>(x, residual, gamma, rows, channels, eps,
