@@ -6,6 +6,7 @@
 // min(p + 1, sinks + window) and every one of them is visible to p.
 // Softmax statistics and all sums are float32. A key that a query does not see contributes nothing at all, whatever
 // bits its rows hold; a query that sees no key gets zeros.
+#include <cooperative_groups.h>
 #include <cuda.h>
 
 #include <atomic>
@@ -787,6 +788,446 @@ window_step_rows_kernel(const T *q, const T *k, const T *v, const int32_t *posit
     }
 }
 
+// ---- single tokens, 16-byte rows: a cluster of blocks per (stream, kv head)
+// The keys of a stream are cut into blocks that the warps of the cluster take in turn, each with a softmax of its own over
+// what it took; at the end the blocks read one another's partial sums through distributed shared memory and every block
+// writes its share of the context. Nothing is staged in device memory, so calls need no workspace and no order among them,
+// and the sums are added in the same order every time. The kernel is bound by the cache's bytes.
+constexpr int kStepWarps = 4;
+
+template <int HEADS, int DP>
+struct StepPartial {
+    float o[kStepWarps][HEADS][DP + 2];   // two columns of padding spread the rows over the banks
+    float2 stat[kStepWarps][HEADS];       // maximum (log2 domain) and sum
+};
+
+template <typename T, int HEADS, int DP>
+__device__ __forceinline__ void step_join(StepPartial<HEADS, DP> *part, int heads_here, int dim, T *out) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int blocks = (int) cluster.num_blocks();
+    for (int e = (int) cluster.block_rank() * (32 * kStepWarps) + threadIdx.x; e < heads_here * dim; e += blocks * 32 * kStepWarps) {
+        const int h = e / dim, x = e - h * dim;
+        float top = -INFINITY;
+        for (int r = 0; r < blocks; ++r) {
+            const StepPartial<HEADS, DP> *from = cluster.map_shared_rank(part, r);
+#pragma unroll
+            for (int w = 0; w < kStepWarps; ++w) {
+                top = fmaxf(top, from->stat[w][h].x);
+            }
+        }
+        float sum = 0.f, total = 0.f;
+        for (int r = 0; r < blocks; ++r) {
+            const StepPartial<HEADS, DP> *from = cluster.map_shared_rank(part, r);
+#pragma unroll
+            for (int w = 0; w < kStepWarps; ++w) {
+                const float2 st = from->stat[w][h];
+                const float weight = st.x == -INFINITY ? 0.f : fast_exp2(st.x - top);
+                if (st.y != 0.f) {   // a warp without keys left nothing
+                    total = fmaf(weight, st.y, total);
+                    sum = fmaf(weight, from->o[w][h][x], sum);
+                }
+            }
+        }
+        out[e] = from_float<T>(total == 0.f ? 0.f : sum / total);
+    }
+    cluster.sync();   // nobody leaves while its sums are read
+}
+
+struct StepPlace {
+    int b, kh, first_head, heads_here, slot, n;
+    int worker, workers;   // this warp among the cluster's
+};
+
+template <int HEADS>
+__device__ __forceinline__ bool step_place(const int32_t *positions, const RingShape &s, int chunks, StepPlace &at) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
+    const int64_t unit = blockIdx.x / blocks;
+    const int share = s.heads / s.kv_heads;
+    const int chunk = (int) (unit % chunks);
+    const int64_t pair = unit / chunks;
+    at.b = (int) (pair / s.kv_heads);
+    at.kh = (int) (pair - (int64_t) at.b * s.kv_heads);
+    at.first_head = at.kh * share + chunk * HEADS;
+    at.heads_here = min(HEADS, share - chunk * HEADS);
+    const int p = positions[at.b];
+    if (p < 0) {
+        return false;
+    }
+    const int slots = s.window + s.sinks;
+    at.slot = ring_slot(p, s.window, s.sinks);
+    at.n = p < slots ? p + 1 : slots;
+    at.worker = rank * kStepWarps + (threadIdx.x >> 5);
+    at.workers = blocks * kStepWarps;
+    return true;
+}
+
+// The new token's row into its slot, by the first chunk's first block; the readers of the slot take the token's own row.
+template <typename T>
+__device__ __forceinline__ void step_store(const T *kn, const T *vn, T *kc, T *vc, const StepPlace &at, const RingShape &s) {
+    if (at.first_head == at.kh * (s.heads / s.kv_heads) && at.worker < kStepWarps) {
+        constexpr int E = 16 / (int) sizeof(T);
+        for (int c = threadIdx.x; c < s.dim / E; c += 32 * kStepWarps) {
+            reinterpret_cast<uint4 *>(kc + (int64_t) at.slot * s.dim)[c] = reinterpret_cast<const uint4 *>(kn)[c];
+            reinterpret_cast<uint4 *>(vc + (int64_t) at.slot * s.dim)[c] = reinterpret_cast<const uint4 *>(vn)[c];
+        }
+    }
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// Binary16: S^T = K.Q^T and O^T += V^T.P^T on warp-level matrix instructions, 16 keys x 8 NT heads a block of keys. Lane
+// (g, t) = (lane / 4, lane % 4) reads 16 bytes (chunk t, t + 4, ..) of the K rows g and g + 8: eight columns that are two steps
+// of the reduction, in an order that Q shares. Of V it reads chunk g (g + 8) of the rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and pairs
+// the halves of two rows: word i of a chunk is rows g and g + 8 of the i-th 16 output columns. So K and V go from memory to
+// operands with no stop in shared memory; P^T turns around in registers.
+template <int DP, int NT>
+__global__ void __launch_bounds__(32 * kStepWarps, DP == 64 ? 4 : (NT == 1 ? 3 : 2))
+window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const int32_t *positions, __half *k_cache, __half *v_cache,
+                       __half *context, const __grid_constant__ RingShape s, int chunks) {
+    constexpr int HEADS = 8 * NT, KC = DP / 32, VC = DP / 64;
+    __shared__ StepPartial<HEADS, DP> part;
+    StepPlace at;
+    if (!step_place<HEADS>(positions, s, chunks, at)) {
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t slots = s.window + s.sinks;
+    const __half *kn = k + at.b * s.kv_stride + (int64_t) at.kh * s.dim, *vn = v + at.b * s.kv_stride + (int64_t) at.kh * s.dim;
+    __half *kc = k_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim, *vc = v_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim;
+    step_store<__half>(kn, vn, kc, vc, at, s);
+
+    uint32_t qf[NT][KC][4];
+#pragma unroll
+    for (int m = 0; m < NT; ++m) {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int col = 8 * (t + 4 * c), head = 8 * m + g;
+            uint4 r = make_uint4(0, 0, 0, 0);
+            if (head < at.heads_here && col < s.dim) {
+                r = ld_param(q + at.b * s.q_stride + (int64_t) (at.first_head + head) * s.dim + col);
+            }
+            qf[m][c][0] = r.x, qf[m][c][1] = r.y, qf[m][c][2] = r.z, qf[m][c][3] = r.w;
+        }
+    }
+    float o[NT][VC][4][4];
+    float top[NT][2], total[NT][2];
+#pragma unroll
+    for (int m = 0; m < NT; ++m) {
+        top[m][0] = top[m][1] = -INFINITY;
+        total[m][0] = total[m][1] = 0.f;
+#pragma unroll
+        for (int x = 0; x < VC; ++x) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[m][x][i][0] = o[m][x][i][1] = o[m][x][i][2] = o[m][x][i][3] = 0.f;
+            }
+        }
+    }
+    const float c2 = s.scale * kLog2e;
+    const int key_blocks = (at.n + 15) / 16;
+    for (int kb = at.worker; kb < key_blocks; kb += at.workers) {
+        const int j0 = kb * 16;
+        uint4 kr[2][KC], vr[4][VC];
+        const bool whole = j0 + 16 <= at.n && (at.slot < j0 || at.slot >= j0 + 16);
+        if (whole) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const __half *row = kc + (int64_t) (j0 + g + 8 * r) * s.dim;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const int col = 8 * (t + 4 * c);
+                    kr[r][c] = col < s.dim ? ld_stream(row + col) : make_uint4(0, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const __half *row = vc + (int64_t) (j0 + 2 * t + (r & 1) + 8 * (r >> 1)) * s.dim;
+#pragma unroll
+                for (int x = 0; x < VC; ++x) {
+                    const int col = 8 * (g + 8 * x);
+                    vr[r][x] = col < s.dim ? ld_stream(row + col) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int j = j0 + g + 8 * r;
+                const __half *row = j == at.slot ? kn : kc + (int64_t) j * s.dim;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const int col = 8 * (t + 4 * c);
+                    kr[r][c] = j < at.n && col < s.dim ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = j0 + 2 * t + (r & 1) + 8 * (r >> 1);
+                const __half *row = j == at.slot ? vn : vc + (int64_t) j * s.dim;
+#pragma unroll
+                for (int x = 0; x < VC; ++x) {
+                    const int col = 8 * (g + 8 * x);
+                    vr[r][x] = j < at.n && col < s.dim ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        }
+        float sc[NT][4];
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+            sc[m][0] = sc[m][1] = sc[m][2] = sc[m][3] = 0.f;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                mma_f16(sc[m], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, qf[m][c][0], qf[m][c][1]);
+                mma_f16(sc[m], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, qf[m][c][2], qf[m][c][3]);
+            }
+        }
+        bool raise = false;
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {   // e: head 2 t + e % 2, key g + 8 (e / 2)
+                sc[m][e] = j0 + g + 8 * (e >> 1) < at.n ? sc[m][e] * c2 : -INFINITY;
+                raise = raise || sc[m][e] - top[m][e & 1] > kRaiseBy;
+            }
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int m = 0; m < NT; ++m) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float here = fmaxf(fmaxf(sc[m][e], sc[m][e + 2]), top[m][e]);
+                    here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 4));
+                    here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 8));
+                    here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 16));
+                    const float shrink = top[m][e] == here ? 1.f : fast_exp2(top[m][e] - here);
+                    top[m][e] = here;
+                    total[m][e] *= shrink;
+#pragma unroll
+                    for (int x = 0; x < VC; ++x) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[m][x][i][e] *= shrink;
+                            o[m][x][i][e + 2] *= shrink;
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = sc[m][e] == -INFINITY ? 0.f : fast_exp2(sc[m][e] - top[m][e & 1]);
+                total[m][e & 1] += p[e];
+            }
+            const __half2 lo = __floats2half2_rn(p[0], p[1]), hi = __floats2half2_rn(p[2], p[3]);
+            const uint32_t b0 = transpose_8x8(*reinterpret_cast<const uint32_t *>(&lo)), b1 = transpose_8x8(*reinterpret_cast<const uint32_t *>(&hi));
+#pragma unroll
+            for (int x = 0; x < VC; ++x) {
+                const uint32_t w0[4] = {vr[0][x].x, vr[0][x].y, vr[0][x].z, vr[0][x].w}, w1[4] = {vr[1][x].x, vr[1][x].y, vr[1][x].z, vr[1][x].w};
+                const uint32_t w2[4] = {vr[2][x].x, vr[2][x].y, vr[2][x].z, vr[2][x].w}, w3[4] = {vr[3][x].x, vr[3][x].y, vr[3][x].z, vr[3][x].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    mma_f16(o[m][x][i], __byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x5410),
+                            __byte_perm(w2[i], w3[i], 0x7632), b0, b1);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < NT; ++m) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float sum = total[m][e];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            const int head = 8 * m + 2 * t + e;
+            if (g == 0) {
+                part.stat[warp][head] = make_float2(top[m][e], sum);
+            }
+#pragma unroll
+            for (int x = 0; x < VC; ++x) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    *reinterpret_cast<float2 *>(&part.o[warp][head][8 * (g + 8 * x) + 2 * i]) = make_float2(o[m][x][i][e], o[m][x][i][e + 2]);
+                }
+            }
+        }
+    }
+    step_join<__half, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
+}
+
+// float32: LPK lanes share a key, four columns each, so that a warp reads 32 / LPK whole rows per instruction; every group of
+// lanes keeps a softmax of its own over its keys, HEADS heads at once.
+template <int LPK, int HEADS>
+__global__ void __launch_bounds__(32 * kStepWarps)
+window_step_f32_kernel(const float *q, const float *k, const float *v, const int32_t *positions, float *k_cache, float *v_cache, float *context,
+                       const __grid_constant__ RingShape s, int chunks) {
+    constexpr int DP = 4 * LPK, GROUPS = 32 / LPK, U = HEADS == 1 ? 8 : 4;   // U: rows per lane group in flight
+    __shared__ StepPartial<HEADS, DP> part;
+    StepPlace at;
+    if (!step_place<HEADS>(positions, s, chunks, at)) {
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LPK, col = 4 * (lane % LPK);
+    const int64_t slots = s.window + s.sinks;
+    const float *kn = k + at.b * s.kv_stride + (int64_t) at.kh * s.dim, *vn = v + at.b * s.kv_stride + (int64_t) at.kh * s.dim;
+    float *kc = k_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim, *vc = v_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim;
+    step_store<float>(kn, vn, kc, vc, at, s);
+    const bool mine = col < s.dim;
+    const float c2 = s.scale * kLog2e;
+    float4 qf[HEADS], o[HEADS];
+    float top[HEADS], total[HEADS];
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        qf[h] = mine && h < at.heads_here
+                    ? __ldg(reinterpret_cast<const float4 *>(q + at.b * s.q_stride + (int64_t) (at.first_head + h) * s.dim + col))
+                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        o[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+        top[h] = -INFINITY;
+        total[h] = 0.f;
+    }
+    const int per_block = GROUPS * U, key_blocks = (at.n + per_block - 1) / per_block;
+    for (int kb = at.worker; kb < key_blocks; kb += at.workers) {
+        float4 kr[U], vr[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = kb * per_block + u * GROUPS + group;
+            const float *krow = j == at.slot ? kn : kc + (int64_t) j * s.dim, *vrow = j == at.slot ? vn : vc + (int64_t) j * s.dim;
+            const bool in = mine && j < at.n;
+            kr[u] = in ? *reinterpret_cast<const float4 *>(krow + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+            vr[u] = in ? *reinterpret_cast<const float4 *>(vrow + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+            float sc[U];
+            float here = top[h];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float d = fmaf(qf[h].x, kr[u].x, qf[h].y * kr[u].y) + fmaf(qf[h].z, kr[u].z, qf[h].w * kr[u].w);
+#pragma unroll
+                for (int m = LPK / 2; m > 0; m >>= 1) {
+                    d += __shfl_xor_sync(0xffffffffu, d, m);
+                }
+                sc[u] = kb * per_block + u * GROUPS + group < at.n ? d * c2 : -INFINITY;
+                here = fmaxf(here, sc[u]);
+            }
+            const float shrink = top[h] == here ? 1.f : fast_exp2(top[h] - here);
+            top[h] = here;
+            total[h] *= shrink;
+            o[h].x *= shrink, o[h].y *= shrink, o[h].z *= shrink, o[h].w *= shrink;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float p = sc[u] == -INFINITY ? 0.f : fast_exp2(sc[u] - here);
+                total[h] += p;
+                o[h].x = fmaf(p, vr[u].x, o[h].x);
+                o[h].y = fmaf(p, vr[u].y, o[h].y);
+                o[h].z = fmaf(p, vr[u].z, o[h].z);
+                o[h].w = fmaf(p, vr[u].w, o[h].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+        float all = top[h];
+#pragma unroll
+        for (int m = LPK; m < 32; m <<= 1) {
+            all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, m));
+        }
+        const float shrink = top[h] == all ? 1.f : (top[h] == -INFINITY ? 0.f : fast_exp2(top[h] - all));
+        float r[5] = {total[h] * shrink, o[h].x * shrink, o[h].y * shrink, o[h].z * shrink, o[h].w * shrink};
+#pragma unroll
+        for (int m = LPK; m < 32; m <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 5; ++i) {
+                r[i] += __shfl_xor_sync(0xffffffffu, r[i], m);
+            }
+        }
+        if (group == 0) {
+            if (lane == 0) {
+                part.stat[warp][h] = make_float2(all, r[0]);
+            }
+            *reinterpret_cast<float2 *>(&part.o[warp][h][col]) = make_float2(r[1], r[2]);
+            *reinterpret_cast<float2 *>(&part.o[warp][h][col + 2]) = make_float2(r[3], r[4]);
+        }
+    }
+    step_join<float, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
+}
+
+// Blocks of a cluster: enough of them to fill the GPU twice, none with less than 64 slots for its four warps.
+inline int step_cluster(int64_t units, int64_t slots) {
+    int blocks = 1;
+    while (blocks < 8 && units * blocks < 2 * 148 && slots > 64 * blocks) {
+        blocks *= 2;
+    }
+    return blocks;
+}
+
+template <typename T, int HEADS, typename Kernel>
+int step_launch(Kernel kernel, const T *q, const T *k, const T *v, const int32_t *positions, T *k_cache, T *v_cache, T *context,
+                const RingShape &s, cudaStream_t stream) {
+    const int chunks = (s.heads / s.kv_heads + HEADS - 1) / HEADS;
+    const int64_t units = (int64_t) s.batch * s.kv_heads * chunks;
+    const int cluster = step_cluster(units, (int64_t) s.window + s.sinks);
+    if (units * cluster > 0x7fffffffLL) {
+        return CUBK_ERR_UNSUPPORTED;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned) (units * cluster));
+    config.blockDim = dim3(32 * kStepWarps);
+    config.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned) cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, q, k, v, positions, k_cache, v_cache, context, s, chunks);
+    if (err != cudaSuccess) {
+        (void) cudaGetLastError();
+        set_last_error(err);
+        return CUBK_ERR_LAUNCH;
+    }
+    return CUBK_OK;
+}
+
+// Rows and heads that start on 16-byte boundaries, head dimension up to 128.
+inline int step_vectors(const __half *q, const __half *k, const __half *v, const int32_t *positions, __half *k_cache, __half *v_cache,
+                        __half *context, const RingShape &s, cudaStream_t stream) {
+    const int share = s.heads / s.kv_heads;
+    if (s.dim <= 64) {
+        return share <= 8 ? step_launch<__half, 8>(window_step_f16_kernel<64, 1>, q, k, v, positions, k_cache, v_cache, context, s, stream)
+                          : step_launch<__half, 16>(window_step_f16_kernel<64, 2>, q, k, v, positions, k_cache, v_cache, context, s, stream);
+    }
+    return share <= 8 ? step_launch<__half, 8>(window_step_f16_kernel<128, 1>, q, k, v, positions, k_cache, v_cache, context, s, stream)
+                      : step_launch<__half, 16>(window_step_f16_kernel<128, 2>, q, k, v, positions, k_cache, v_cache, context, s, stream);
+}
+
+inline int step_vectors(const float *q, const float *k, const float *v, const int32_t *positions, float *k_cache, float *v_cache, float *context,
+                        const RingShape &s, cudaStream_t stream) {
+    const int share = s.heads / s.kv_heads;
+#define STEP_F32(LPK)                                                                                                                       \
+    (share == 1 ? step_launch<float, 1>(window_step_f32_kernel<LPK, 1>, q, k, v, positions, k_cache, v_cache, context, s, stream)            \
+                : step_launch<float, 4>(window_step_f32_kernel<LPK, 4>, q, k, v, positions, k_cache, v_cache, context, s, stream))
+    return s.dim <= 32 ? STEP_F32(8) : s.dim <= 64 ? STEP_F32(16) : STEP_F32(32);
+#undef STEP_F32
+}
+
 template <typename T>
 int window_attention_step(const T *q, const T *k, const T *v, int64_t q_stride, int64_t kv_stride, const int32_t *positions, int batch,
                           int heads, int kv_heads, int dim, int window, int sinks, float scale, T *k_cache, T *v_cache, T *context,
@@ -803,6 +1244,14 @@ int window_attention_step(const T *q, const T *k, const T *v, int64_t q_stride, 
         return CUBK_OK;
     }
     const RingShape s = {batch, heads, kv_heads, dim, window, sinks, scale, q_stride, kv_stride, context_stride};
+    constexpr int E = 16 / (int) sizeof(T);
+    if (dim <= 128 && dim % E == 0 && q_stride % E == 0 && kv_stride % E == 0 && aligned16(q) && aligned16(k) && aligned16(v) &&
+        aligned16(k_cache) && aligned16(v_cache)) {
+        const int rc = step_vectors(q, k, v, positions, k_cache, v_cache, context, s, stream);
+        if (rc != CUBK_ERR_UNSUPPORTED) {
+            return rc;
+        }
+    }
     const int64_t groups = ((int64_t) batch * heads + kWindowRowWarps - 1) / kWindowRowWarps;
     const unsigned blocks = (unsigned) (groups < 148 * 64 ? groups : 148 * 64);
     window_step_rows_kernel<T><<<blocks, 32 * kWindowRowWarps, 0, stream>>>(q, k, v, positions, k_cache, v_cache, context, s);
