@@ -128,6 +128,245 @@ window_rows_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *co
     }
 }
 
+// ---- whole sequences on the float32 pipes (float32 storage; binary16 rows that TMA cannot read)
+// 64 query rows of a head a block, 64 keys a step out of one list: the sinks below the window, then the window. A thread owns 8 rows
+// x 4 keys of the scores and 8 rows x DP / 16 columns of the context; Q and K are transposed on their way into shared memory, so that
+// each step of a reduction is two or three 16-byte reads for 32 or 64 multiply-adds, issued in pairs of rows. The 16 threads of a row
+// are half a warp: maxima and sums need shuffles only. Bound by the multiply-adds.
+constexpr int kPlainRows = 64, kPlainKeys = 64, kPlainThreads = 128;
+
+template <int DP>
+struct WindowPlain {
+    static constexpr int QK = kPlainRows + 4;       // floats between columns of the transposed tiles: 16-byte rows over all banks
+    static constexpr int FLOATS = 2 * DP * QK + kPlainKeys * DP + kPlainKeys * QK;
+    static constexpr int BYTES = FLOATS * 4;
+};
+
+// Columns c .. c + 3 of a row as float32, zeros past the dimension.
+template <typename T>
+__device__ __forceinline__ float4 four_columns(const T *row, int c, int dim, bool vec) {
+    if (sizeof(T) == 4 && vec) {
+        return c < dim ? __ldg(reinterpret_cast<const float4 *>(row + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    return make_float4(c < dim ? to_float<T>(row[c]) : 0.f, c + 1 < dim ? to_float<T>(row[c + 1]) : 0.f,
+                       c + 2 < dim ? to_float<T>(row[c + 2]) : 0.f, c + 3 < dim ? to_float<T>(row[c + 3]) : 0.f);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPlainThreads, DP == 64 ? 3 : 2)
+window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *context, const __grid_constant__ WindowShape s, int row_blocks, bool vec) {
+    typedef WindowPlain<DP> C;
+    constexpr int VC = DP / 64;   // 4-column groups of a thread's context
+    extern __shared__ __align__(16) float plain_smem[];
+    float *s_q = plain_smem, *s_k = s_q + DP * C::QK, *s_v = s_k + DP * C::QK, *s_p = s_v + kPlainKeys * DP;   // [column][row], .., [key][column], [key][row]
+    __shared__ int s_kept[kPlainKeys], s_bad[kPlainRows];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rg = threadIdx.x >> 4, cg = threadIdx.x & 15;   // rows 8 rg .., keys 4 cg .., columns 4 cg + 64 x ..
+    const int rb = row_blocks - 1 - (int) (blockIdx.x % row_blocks);
+    const int64_t bh = blockIdx.x / row_blocks;
+    const int b = (int) (bh / s.heads), h = (int) (bh - (int64_t) b * s.heads), kh = h / (s.heads / s.kv_heads);
+    const int row0 = rb * kPlainRows, last_row = min(row0 + kPlainRows, s.seq) - 1;
+    const int64_t first = (int64_t) b * s.seq;
+    const T *qb = q + first * s.q_stride + (int64_t) h * s.dim, *kb = k + first * s.kv_stride + (int64_t) kh * s.dim;
+    const T *vb = v + first * s.kv_stride + (int64_t) kh * s.dim;
+    const int8_t *kept = mask != nullptr ? mask + first : nullptr;
+    const int lo = row0 > s.before ? row0 - s.before : 0;
+    const int hi = s.after < s.seq - 1 - last_row ? last_row + s.after + 1 : s.seq;
+    const int sinks_end = min(s.sinks, lo), listed = sinks_end + hi - lo;
+
+    for (int i = threadIdx.x; i < kPlainRows * (DP / 4); i += kPlainThreads) {
+        const int r = i % kPlainRows, c = 4 * (i / kPlainRows);
+        const float4 x = row0 + r < s.seq ? four_columns<T>(qb + (int64_t) (row0 + r) * s.q_stride, c, s.dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+        s_q[c * C::QK + r] = x.x, s_q[(c + 1) * C::QK + r] = x.y, s_q[(c + 2) * C::QK + r] = x.z, s_q[(c + 3) * C::QK + r] = x.w;
+    }
+    const float c2 = s.scale * kLog2e;
+    float top[8], total[8];
+    float2 o[4][4 * VC];   // pairs of rows x columns
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        top[r] = -INFINITY;
+        total[r] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int c = 0; c < 4 * VC; ++c) {
+            o[r][c] = make_float2(0.f, 0.f);
+        }
+    }
+    for (int u0 = 0; u0 < listed; u0 += kPlainKeys) {
+        const int keys = min(kPlainKeys, listed - u0);
+        auto key_of = [&](int u) { return u < sinks_end ? u : lo + u - sinks_end; };
+        bool on = false;
+        if (threadIdx.x < kPlainKeys) {   // before the barrier: whoever still reads s_kept is past the one after the products
+            on = (int) threadIdx.x < keys && (kept == nullptr || kept[key_of(u0 + threadIdx.x)] != 0);
+        }
+        const int any = __syncthreads_count(on);   // and the step before is done with K, V and P
+        if (any == 0) {
+            continue;
+        }
+        if (threadIdx.x < kPlainKeys) {
+            s_kept[threadIdx.x] = on ? key_of(u0 + threadIdx.x) : -1;
+        }
+        for (int i = threadIdx.x; i < kPlainKeys * (DP / 4); i += kPlainThreads) {
+            const int r = i % kPlainKeys, c = 4 * (i / kPlainKeys);
+            const float4 x = r < keys ? four_columns<T>(kb + (int64_t) key_of(u0 + r) * s.kv_stride, c, s.dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+            s_k[c * C::QK + r] = x.x, s_k[(c + 1) * C::QK + r] = x.y, s_k[(c + 2) * C::QK + r] = x.z, s_k[(c + 3) * C::QK + r] = x.w;
+        }
+        for (int i = threadIdx.x; i < kPlainKeys * (DP / 4); i += kPlainThreads) {
+            const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
+            *reinterpret_cast<float4 *>(&s_v[r * DP + c]) =
+                r < keys ? four_columns<T>(vb + (int64_t) key_of(u0 + r) * s.kv_stride, c, s.dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        __syncthreads();
+        float2 sc[4][4];   // pairs of rows x keys
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            sc[r][0] = sc[r][1] = sc[r][2] = sc[r][3] = make_float2(0.f, 0.f);
+        }
+#pragma unroll 4
+        for (int c = 0; c < s.dim; ++c) {
+            const float4 q0 = *reinterpret_cast<const float4 *>(&s_q[c * C::QK + 8 * rg]), q1 = *reinterpret_cast<const float4 *>(&s_q[c * C::QK + 8 * rg + 4]);
+            const float4 kk = *reinterpret_cast<const float4 *>(&s_k[c * C::QK + 4 * cg]);
+            const float2 rows[4] = {make_float2(q0.x, q0.y), make_float2(q0.z, q0.w), make_float2(q1.x, q1.y), make_float2(q1.z, q1.w)};
+            const float2 ks[4] = {splat2(kk.x), splat2(kk.y), splat2(kk.z), splat2(kk.w)};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[r][e] = fma2(rows[r], ks[e], sc[r][e]);
+                }
+            }
+        }
+        // a key counts for row i when it is kept, at most i + after, and at least i - before or below the sinks
+        const int4 js = *reinterpret_cast<const int4 *>(&s_kept[4 * cg]);
+        const int j4[4] = {js.x, js.y, js.z, js.w};
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int i = row0 + 8 * rg + r;
+            const int i_lo = i > s.before ? i - s.before : 0, i_hi = s.after < s.seq ? i + s.after : s.seq;
+            float p[4], here = top[r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = (r & 1) ? sc[r / 2][e].y : sc[r / 2][e].x;
+                const bool see = j4[e] >= 0 && j4[e] <= i_hi && (j4[e] >= i_lo || j4[e] < s.sinks);
+                p[e] = see ? x * c2 : -INFINITY;
+                here = fmaxf(here, p[e]);
+            }
+            here = group_max<16>(here);
+            const float base = here == -INFINITY ? 0.f : here, shrink = top[r] == here ? 1.f : fast_exp2(top[r] - here);
+            top[r] = here;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                p[e] = fast_exp2(p[e] - base);
+                sum += p[e];
+                if (r & 1) {
+                    sc[r / 2][e].y = p[e];
+                } else {
+                    sc[r / 2][e].x = p[e];
+                }
+            }
+            total[r] = fmaf(total[r], shrink, sum);   // of this thread's keys
+#pragma unroll
+            for (int c = 0; c < 4 * VC; ++c) {
+                if (r & 1) {
+                    o[r / 2][c].y *= shrink;
+                } else {
+                    o[r / 2][c].x *= shrink;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float *to = &s_p[(4 * cg + e) * C::QK + 8 * rg];
+            *reinterpret_cast<float4 *>(to) = make_float4(sc[0][e].x, sc[0][e].y, sc[1][e].x, sc[1][e].y);
+            *reinterpret_cast<float4 *>(to + 4) = make_float4(sc[2][e].x, sc[2][e].y, sc[3][e].x, sc[3][e].y);
+        }
+        __syncwarp();   // a row's weights stay within its warp
+#pragma unroll 4
+        for (int j = 0; j < keys; ++j) {
+            const float4 p0 = *reinterpret_cast<const float4 *>(&s_p[j * C::QK + 8 * rg]), p1 = *reinterpret_cast<const float4 *>(&s_p[j * C::QK + 8 * rg + 4]);
+            const float2 rows[4] = {make_float2(p0.x, p0.y), make_float2(p0.z, p0.w), make_float2(p1.x, p1.y), make_float2(p1.z, p1.w)};
+#pragma unroll
+            for (int x = 0; x < VC; ++x) {
+                const float4 vv = *reinterpret_cast<const float4 *>(&s_v[j * DP + 64 * x + 4 * cg]);
+                const float2 vs[4] = {splat2(vv.x), splat2(vv.y), splat2(vv.z), splat2(vv.w)};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[r][4 * x + e] = fma2(rows[r], vs[e], o[r][4 * x + e]);
+                    }
+                }
+            }
+        }
+    }
+    const float most = sizeof(T) == 4 ? 3.402823466e38f : 65504.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const float all = group_sum<16>(total[r]);
+        const float inv = all == 0.f ? 0.f : 1.f / all;
+        const int i = row0 + 8 * rg + r;
+        bool finite = true;
+        T *out = context + (first + i) * s.context_stride + (int64_t) h * s.dim;
+#pragma unroll
+        for (int c = 0; c < 4 * VC; ++c) {
+            const int col = 64 * (c / 4) + 4 * cg + c % 4;
+            const float x = ((r & 1) ? o[r / 2][c].y : o[r / 2][c].x) * inv;
+            if (col < s.dim) {
+                finite = finite && fabsf(x) <= most;
+                if (i < s.seq) {
+                    out[col] = from_float<T>(x);
+                }
+            }
+        }
+        const unsigned bad = __ballot_sync(0xffffffffu, !finite);
+        if (cg == 0) {
+            s_bad[8 * rg + r] = (bad >> (lane & 16) & 0xffffu) != 0 && i < s.seq;
+        }
+    }
+    __syncthreads();   // Q is no longer read: its place serves the rows that are computed again
+    for (int r = warp; r < kPlainRows; r += kPlainThreads / 32) {
+        if (s_bad[r] != 0) {
+            window_prompt_row<T>(q, k, v, mask, context, s, s_q + warp * kWindowMaxDim, b, row0 + r, h);
+        }
+    }
+}
+
+template <typename T, int DP>
+int window_plain_launch(const T *q, const T *k, const T *v, const int8_t *mask, T *context, const WindowShape &s, cudaStream_t stream) {
+    static std::atomic<uint64_t> prepared{0};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err == cudaSuccess && (dev >= 64 || ((prepared.load(std::memory_order_acquire) >> dev) & 1ull) == 0)) {
+        err = cudaFuncSetAttribute(window_plain_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, WindowPlain<DP>::BYTES);
+        if (err == cudaSuccess && dev < 64) {
+            prepared.fetch_or(1ull << dev, std::memory_order_release);
+        }
+    }
+    if (err != cudaSuccess) {
+        set_last_error(err);
+        return CUBK_ERR_LAUNCH;
+    }
+    const int row_blocks = (s.seq + kPlainRows - 1) / kPlainRows;
+    const int64_t blocks = (int64_t) row_blocks * s.batch * s.heads;
+    if (blocks > 0x7fffffffLL) {
+        return CUBK_ERR_UNSUPPORTED;
+    }
+    const bool vec = sizeof(T) == 4 && s.dim % 4 == 0 && s.q_stride % 4 == 0 && s.kv_stride % 4 == 0 && aligned16(q) && aligned16(k) && aligned16(v);
+    window_plain_kernel<T, DP><<<(unsigned) blocks, kPlainThreads, WindowPlain<DP>::BYTES, stream>>>(q, k, v, mask, context, s, row_blocks, vec);
+    return check_launch();
+}
+
+// Head dimensions up to 128; CUBK_ERR_UNSUPPORTED beyond.
+template <typename T>
+int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *context, const WindowShape &s, cudaStream_t stream) {
+    return s.dim > 128 ? CUBK_ERR_UNSUPPORTED
+           : s.dim > 64 ? window_plain_launch<T, 128>(q, k, v, mask, context, s, stream)
+                        : window_plain_launch<T, 64>(q, k, v, mask, context, s, stream);
+}
+
 // ---------------------------------------------------------------- whole sequences on tcgen05 (binary16)
 // A block owns NQ tiles of 128 query rows: two heads that share their keys, or consecutive rows of one head. Per step of up
 // to 128 keys and per tile: S = Q.K^T (tcgen05.mma, float32 accumulators in tensor memory), softmax by 128 threads that own
@@ -736,6 +975,10 @@ int window_attention(const T *q, const T *k, const T *v, int64_t q_stride, int64
         if (rc != CUBK_ERR_UNSUPPORTED) {
             return rc;
         }
+    }
+    const int rc = window_plain(q, k, v, mask, context, s, stream);
+    if (rc != CUBK_ERR_UNSUPPORTED) {
+        return rc;
     }
     const int64_t groups = ((int64_t) batch * seq * heads + kWindowRowWarps - 1) / kWindowRowWarps;
     const unsigned blocks = (unsigned) (groups < 148 * 64 ? groups : 148 * 64);
