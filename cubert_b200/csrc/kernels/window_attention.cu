@@ -138,7 +138,7 @@ constexpr int kPlainRows = 64, kPlainKeys = 64, kPlainThreads = 128;
 template <int DP>
 struct WindowPlain {
     static constexpr int QK = kPlainRows + 4;       // floats between columns of the transposed tiles: 16-byte rows over all banks
-    static constexpr int FLOATS = 2 * DP * QK + kPlainKeys * DP + kPlainKeys * QK;
+    static constexpr int FLOATS = 2 * DP * QK + kPlainKeys * DP;   // the weights take the keys' place
     static constexpr int BYTES = FLOATS * 4;
 };
 
@@ -158,7 +158,7 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
     typedef WindowPlain<DP> C;
     constexpr int VC = DP / 64;   // 4-column groups of a thread's context
     extern __shared__ __align__(16) float plain_smem[];
-    float *s_q = plain_smem, *s_k = s_q + DP * C::QK, *s_v = s_k + DP * C::QK, *s_p = s_v + kPlainKeys * DP;   // [column][row], .., [key][column], [key][row]
+    float *s_q = plain_smem, *s_k = s_q + DP * C::QK, *s_v = s_k + DP * C::QK, *s_p = s_k;   // [column][row], .., [key][column], [key][row]
     __shared__ int s_kept[kPlainKeys], s_bad[kPlainRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rg = threadIdx.x >> 4, cg = threadIdx.x & 15;   // rows 8 rg .., keys 4 cg .., columns 4 cg + 64 x ..
@@ -208,15 +208,29 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
         if (threadIdx.x < kPlainKeys) {
             s_kept[threadIdx.x] = on ? key_of(u0 + threadIdx.x) : -1;
         }
-        for (int i = threadIdx.x; i < kPlainKeys * (DP / 4); i += kPlainThreads) {
-            const int r = i % kPlainKeys, c = 4 * (i / kPlainKeys);
-            const float4 x = r < keys ? four_columns<T>(kb + (int64_t) key_of(u0 + r) * s.kv_stride, c, s.dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-            s_k[c * C::QK + r] = x.x, s_k[(c + 1) * C::QK + r] = x.y, s_k[(c + 2) * C::QK + r] = x.z, s_k[(c + 3) * C::QK + r] = x.w;
-        }
-        for (int i = threadIdx.x; i < kPlainKeys * (DP / 4); i += kPlainThreads) {
-            const int r = i / (DP / 4), c = 4 * (i % (DP / 4));
-            *reinterpret_cast<float4 *>(&s_v[r * DP + c]) =
-                r < keys ? four_columns<T>(vb + (int64_t) key_of(u0 + r) * s.kv_stride, c, s.dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+        // eight loads of a thread in flight at a time
+#pragma unroll
+        for (int half = 0; half < 2 * VC; ++half) {
+            constexpr int LOADS = kPlainKeys * 16 / kPlainThreads;   // of 64 columns
+            const bool is_v = half >= VC;
+            float4 x[LOADS];
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) {
+                const int i = threadIdx.x + u * kPlainThreads;
+                const int r = is_v ? i / 16 : i % kPlainKeys, c = 64 * (half % VC) + 4 * (is_v ? i % 16 : i / kPlainKeys);
+                x[u] = r < keys ? four_columns<T>((is_v ? vb : kb) + (int64_t) key_of(u0 + r) * s.kv_stride, c, s.dim, vec)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < LOADS; ++u) {
+                const int i = threadIdx.x + u * kPlainThreads;
+                const int r = is_v ? i / 16 : i % kPlainKeys, c = 64 * (half % VC) + 4 * (is_v ? i % 16 : i / kPlainKeys);
+                if (is_v) {
+                    *reinterpret_cast<float4 *>(&s_v[r * DP + c]) = x[u];
+                } else {
+                    s_k[c * C::QK + r] = x[u].x, s_k[(c + 1) * C::QK + r] = x[u].y, s_k[(c + 2) * C::QK + r] = x[u].z, s_k[(c + 3) * C::QK + r] = x[u].w;
+                }
+            }
         }
         __syncthreads();
         float2 sc[4][4];   // pairs of rows x keys
@@ -277,6 +291,7 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
                 }
             }
         }
+        __syncthreads();   // the keys have been read
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             float *to = &s_p[(4 * cg + e) * C::QK + 8 * rg];
