@@ -443,6 +443,18 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// True on one lane of the warp, the same every time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t mine;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(mine));
+    return mine != 0;
+}
+
+// A wait of a whole warp: false on every lane when any gave up.
+__device__ __forceinline__ bool wait_together(uint64_t *bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity)) != 0;
+}
+
 __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -513,7 +525,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     __shared__ float s_row[C::SOFTMAX_WARPS][kWindowMaxDim];
     unsigned char *tiles = tc_raw + ((1024u - (smem_addr(tc_raw) & 1023u)) & 1023u);
     unsigned char *s_qt = tiles, *s_kt = tiles + NQ * C::TILE_BYTES, *s_vt = s_kt + C::STAGES * C::TILE_BYTES;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     // the block's tiles: last rows first (with a one-sided window that reaches far, they have the most keys)
     const int per_head = row_blocks;
@@ -553,7 +565,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
 
     if (warp == C::SOFTMAX_WARPS + 1) {
         // ---- steps and loads
@@ -657,69 +669,76 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         }
         __syncwarp();
     } else if (warp == C::SOFTMAX_WARPS) {
-        // ---- matrix products, issued by one thread
-        if (lane == 0) {
-            const uint32_t ksteps = (uint32_t) (s.dim + 15) / 16;
-            const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((2 * ksteps) << 17) | ((kTileRows >> 4) << 24);   // N: the dimension, in 16s
-            bool ok = mbar_wait_bounded(&s_qfull, 0);
-            bool first[NQ];
+        // ---- matrix products: the warp walks together (its addresses stay in uniform registers), one lane issues
+        const uint32_t ksteps = (uint32_t) (s.dim + 15) / 16;
+        const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((2 * ksteps) << 17) | ((kTileRows >> 4) << 24);   // N: the dimension, in 16s
+        const bool leader = elect_one();
+        const uint64_t q_desc = swizzled_desc(smem_addr(s_qt), 16), k_desc = swizzled_desc(smem_addr(s_kt), 16);
+        const uint64_t v_desc = swizzled_desc(smem_addr(s_vt), kHalfTileBytes);
+        bool ok = wait_together(&s_qfull, 0);
+        uint32_t started = 0;   // bit t: O of tile t holds something
+        int keys_before = 0;
+        uint32_t flags_before = 0;
+        for (int step = 0; ok; ++step) {
+            const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES;
+            ok = wait_together(&s_kfull[st], (step / C::STAGES) & 1);
+            if (!ok) {
+                break;
+            }
+            const int keys = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].keys, 0);
+            const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0);
+            const uint32_t keys16 = (uint32_t) (keys + 15) / 16;
+            const uint32_t idesc_s = (1u << 4) | ((2 * keys16) << 17) | ((kTileRows >> 4) << 24);
 #pragma unroll
             for (int t = 0; t < NQ; ++t) {
-                first[t] = true;
-            }
-            int keys_before = 0;
-            uint32_t flags_before = 0;
-            for (int step = 0; ok; ++step) {
-                const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES;
-                ok = mbar_wait_bounded(&s_kfull[st], (step / C::STAGES) & 1);
-                if (!ok) {
-                    break;
-                }
-                const int keys = s_steps[step % kStepSlots].keys;
-                const uint32_t flags = s_steps[step % kStepSlots].flags;
-                const uint32_t keys16 = (uint32_t) (keys + 15) / 16;
-                const uint32_t idesc_s = (1u << 4) | ((2 * keys16) << 17) | ((kTileRows >> 4) << 24);
+                if (step > 0) {
+                    ok = ok && wait_together(&s_pfull[t], (step - 1) & 1);
+                    if (t == 0) {
+                        ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1);
+                    }
+                    tmem_fence_after();
+                    if (ok && (flags_before >> t & 1u) != 0) {
+                        const uint64_t vd = v_desc + (uint64_t) (st_before * (C::TILE_BYTES / 16));
+                        if (leader) {
 #pragma unroll
-                for (int t = 0; t < NQ; ++t) {
-                    if (step > 0) {
-                        ok = ok && mbar_wait_bounded(&s_pfull[t], (step - 1) & 1) &&
-                             mbar_wait_bounded(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1);
-                        tmem_fence_after();
-                        if (ok && (flags_before >> t & 1u) != 0) {
-                            const uint32_t vs = smem_addr(s_vt + st_before * C::TILE_BYTES);
-                            for (int kk = 0; kk < (keys_before + 15) / 16; ++kk) {
-                                mma_ts(tmem + NQ * 128 + t * DP, tmem + t * 128 + 8 * kk, swizzled_desc(vs + 2048 * kk, kHalfTileBytes), idesc_o,
-                                       !(first[t] && kk == 0));
+                            for (int kk = 0; kk < kTileRows / 16; ++kk) {
+                                if (16 * kk < keys_before) {
+                                    mma_ts(tmem + NQ * 128 + t * DP, tmem + t * 128 + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || (started >> t & 1u) != 0);
+                                }
                             }
-                            first[t] = false;
                         }
-                        if (t == NQ - 1 && ok) {
-                            mma_commit(&s_vempty[st_before]);
-                        }
+                        started |= 1u << t;
                     }
-                    if (ok && (flags >> t & 1u) != 0) {
-                        const uint32_t qs = smem_addr(s_qt + t * C::TILE_BYTES), ks = smem_addr(s_kt + st * C::TILE_BYTES);
-                        for (uint32_t kk = 0; kk < ksteps; ++kk) {
-                            const uint32_t at = (kk >> 2) * kHalfTileBytes + (kk & 3) * 32;
-                            mma_ss(tmem + t * 128, swizzled_desc(qs + at, 16), swizzled_desc(ks + at, 16), idesc_s, kk > 0);
-                        }
-                    }
-                    if (ok) {
-                        mma_commit(&s_sfull[t]);
-                        mbar_arrive(&s_sfull[t]);
+                    if (t == NQ - 1 && ok && leader) {
+                        mma_commit(&s_vempty[st_before]);
                     }
                 }
-                if (keys == 0) {
-                    break;
+                if (ok && leader) {
+                    if ((flags >> t & 1u) != 0) {
+                        const uint64_t qd = q_desc + (uint64_t) (t * (C::TILE_BYTES / 16)), kd = k_desc + (uint64_t) (st * (C::TILE_BYTES / 16));
+#pragma unroll
+                        for (int kk = 0; kk < DP / 16; ++kk) {
+                            if (kk < (int) ksteps) {
+                                const uint32_t at = ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16;
+                                mma_ss(tmem + t * 128, qd + at, kd + at, idesc_s, kk > 0);
+                            }
+                        }
+                    }
+                    mma_commit(&s_sfull[t]);
+                    mbar_arrive(&s_sfull[t]);
                 }
-                if (ok) {
-                    mma_commit(&s_kempty[st]);
-                }
-                keys_before = keys;
-                flags_before = flags;
+                __syncwarp();
             }
+            if (keys == 0) {
+                break;
+            }
+            if (ok && leader) {
+                mma_commit(&s_kempty[st]);
+            }
+            __syncwarp();
+            keys_before = keys;
+            flags_before = flags;
         }
-        __syncwarp();
     } else {
         // ---- softmax: a row per thread
         const int t = NQ == 1 ? 0 : warp / 4;
