@@ -384,12 +384,15 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 
 // ---------------------------------------------------------------- whole sequences on tcgen05 (binary16)
 // A block owns NQ tiles of 128 query rows: two heads that share their keys, or consecutive rows of one head. Per step of up
-// to 128 keys and per tile: S = Q.K^T (tcgen05.mma, float32 accumulators in tensor memory), softmax by 128 threads that own
-// a row each (tensor-memory lane = query row, so no shuffles), P back into tensor memory over S as binary16, O += P.V with P
-// as the tensor-memory operand. Warps: 4 NQ for the softmax, one that issues the MMAs, one that chooses the steps and
-// loads K and V with TMA (128-byte swizzle; V is read as it lies, as an MN-major operand).
-//   * Steps: first the sinks below the window, then the window in 128s. A step whose keys are all masked is left out; one that
-//     every row of a tile sees whole skips the masking.
+// to KEYS keys and per tile: S = Q.K^T (tcgen05.mma, float32 accumulators in tensor memory), softmax by 128 threads that own
+// a row each (tensor-memory lane = query row, so no shuffles), P back into tensor memory as binary16, O += P.V with P as the
+// tensor-memory operand. Warps: 4 NQ for the softmax, NQ that issue the MMAs of a tile, one that chooses the steps and loads K
+// and V with TMA (128-byte swizzle; V is read as it lies, as an MN-major operand).
+//   * The scores' place is free as soon as a row is in registers, so the next step's scores are computed while this step's
+//     exponentials are; the weights have a place of their own, so their product runs under the next step's softmax. KEYS is what
+//     fits beside the contexts: 128 for heads of up to 64 (two blocks of one tile share an SM), 80 for 128 (one of two tiles).
+//   * Steps: first the sinks below the window, then the window. A step whose keys are all masked is left out; one that every row of
+//     a tile sees whole skips the masking.
 //   * The running maximum of a row is raised only when a step's maximum exceeds it by 2^8 (a weight is then at most 256, far
 //     inside binary16, and the sums are float32), so that O is read back and scaled in few steps.
 //   * Weights of unseen keys are exactly 0, but 0 times an infinity or NaN in an unseen V row is NaN: a row that comes out not
@@ -397,7 +400,7 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 // Every wait is bounded; a block that gives up writes NaN, frees its tensor memory and returns.
 constexpr int kTileRows = 128;
 constexpr int kHalfTileBytes = kTileRows * 128;    // 128 rows x 64 binary16
-constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 1
+constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 2
 constexpr float kRaiseBy = 8.f;                    // log2 of the largest weight
 
 struct WindowStep {
@@ -408,14 +411,19 @@ struct WindowStep {
 
 template <int DP, int NQ>
 struct WindowTc {
+    static constexpr int KEYS = DP == 64 ? 128 : 80;         // of a step
+    static constexpr int CHUNKS = KEYS / 16;                 // the softmax goes by 16 columns
     static constexpr int HALVES = DP / 64;
     static constexpr int TILE_BYTES = HALVES * kHalfTileBytes;
-    static constexpr int STAGES = 2;
+    static constexpr int HALF_KV = KEYS * 128, KV_BYTES = HALVES * HALF_KV;
+    static constexpr int STAGES = DP == 64 ? 2 : 3;
     static constexpr int SOFTMAX_WARPS = 4 * NQ;
-    static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 2);
+    static constexpr int THREADS = 32 * (SOFTMAX_WARPS + NQ + 1);
+    static constexpr int WEIGHTS = NQ * KEYS, CONTEXT = WEIGHTS + NQ * KEYS / 2;   // columns of tensor memory behind the scores
     static constexpr int TMEM_COLS = NQ == 1 ? 256 : 512;
-    static constexpr int SMEM_BYTES = 1024 + (NQ + 2 * STAGES) * TILE_BYTES;   // 1024: alignment of the swizzled tiles
-    static_assert(NQ * (128 + DP) <= TMEM_COLS, "scores and contexts of all tiles");
+    static constexpr int SMEM_BYTES = 1024 + NQ * TILE_BYTES + 2 * STAGES * KV_BYTES;   // 1024: alignment of the swizzled tiles
+    static_assert(CONTEXT + NQ * DP <= TMEM_COLS, "scores, weights and contexts of all tiles");
+    static_assert(STAGES + 2 < kStepSlots, "a descriptor outlives its step");
 };
 
 __device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lbo_bytes) {
@@ -467,6 +475,21 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
@@ -491,7 +514,7 @@ __device__ __forceinline__ void tmem_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 
-// 128 rows x 64 columns of one head into a swizzled tile; rows and columns outside the tensor arrive as zeros.
+// The map's box of rows x 64 columns of one head into a swizzled tile; rows and columns outside the tensor arrive as zeros.
 __device__ __forceinline__ void tma_tile(void *dst, const CUtensorMap *map, int column, int row, int head, int batch, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
                      smem_addr(dst)),
@@ -519,12 +542,13 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                  int row_blocks, int pair_heads) {
     typedef WindowTc<DP, NQ> C;
     extern __shared__ unsigned char tc_raw[];
-    __shared__ uint64_t s_qfull, s_kfull[C::STAGES], s_kempty[C::STAGES], s_vfull[C::STAGES], s_vempty[C::STAGES], s_sfull[NQ], s_pfull[NQ];
+    __shared__ uint64_t s_qfull, s_kfull[C::STAGES], s_kempty[C::STAGES], s_vfull[C::STAGES], s_vempty[C::STAGES];
+    __shared__ uint64_t s_sfull[NQ], s_sfree[NQ], s_pfull[NQ], s_ofull[NQ];   // scores written, scores read, weights written, O added to
     __shared__ uint32_t s_tmem;
     __shared__ WindowStep s_steps[kStepSlots];
     __shared__ float s_row[C::SOFTMAX_WARPS][kWindowMaxDim];
     unsigned char *tiles = tc_raw + ((1024u - (smem_addr(tc_raw) & 1023u)) & 1023u);
-    unsigned char *s_qt = tiles, *s_kt = tiles + NQ * C::TILE_BYTES, *s_vt = s_kt + C::STAGES * C::TILE_BYTES;
+    unsigned char *s_qt = tiles, *s_kt = tiles + NQ * C::TILE_BYTES, *s_vt = s_kt + C::STAGES * C::KV_BYTES;
     const int warp = __shfl_sync(0xffffffffu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     // the block's tiles: last rows first (with a one-sided window that reaches far, they have the most keys)
@@ -552,13 +576,15 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         mbar_init(&s_qfull, 1);
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&s_kfull[i], 1);
-            mbar_init(&s_kempty[i], 1);
+            mbar_init(&s_kempty[i], NQ);
             mbar_init(&s_vfull[i], 1);
-            mbar_init(&s_vempty[i], 1);
+            mbar_init(&s_vempty[i], NQ);
         }
         for (int t = 0; t < NQ; ++t) {
-            mbar_init(&s_sfull[t], 2);   // the MMAs' completion and the issuing thread, which read the step's descriptor
+            mbar_init(&s_sfull[t], 2);   // the MMAs' completion and the issuing warp, which has seen the step's descriptor
+            mbar_init(&s_sfree[t], 4);
             mbar_init(&s_pfull[t], 4);
+            mbar_init(&s_ofull[t], 1);
         }
         mbar_init_fence();
     }
@@ -567,7 +593,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
 
-    if (warp == C::SOFTMAX_WARPS + 1) {
+    if (warp == C::SOFTMAX_WARPS + NQ) {
         // ---- steps and loads
         const int last_row = min(row0 + (pair_heads ? 1 : NQ) * kTileRows, s.seq) - 1;
         const int lo = row0 > s.before ? row0 - s.before : 0;
@@ -591,23 +617,25 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 in_sinks = false;
                 j0 = lo;
             }
-            const int keys = min((in_sinks ? sinks_end : hi) - j0, kTileRows);   // none left: 0 or less (only past the window)
+            const int keys = min((in_sinks ? sinks_end : hi) - j0, C::KEYS);   // none left: 0 or less (only past the window)
             WindowStep d;
             d.j0 = j0;
             d.keys = max(keys, 0);
             d.flags = 0;
             bool all = true;
+            uint32_t some = 0;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const int j = j0 + 32 * w + lane;
                 const bool in = 32 * w + lane < keys;
                 const bool on = in && (kept == nullptr || kept[j] != 0);
                 d.kept[w] = __ballot_sync(0xffffffffu, on);
+                some |= d.kept[w];
                 all = all && __all_sync(0xffffffffu, on || !in);
             }
-            j0 += kTileRows;
+            j0 += C::KEYS;
             if (keys > 0) {
-                if ((d.kept[0] | d.kept[1] | d.kept[2] | d.kept[3]) == 0) {
+                if (some == 0) {
                     continue;
                 }
 #pragma unroll
@@ -618,7 +646,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     if (first < s.seq && d.j0 < t_hi && (d.j0 + keys > t_lo || d.j0 < s.sinks)) {
                         d.flags |= 1u << t;
                     }
-                    const bool whole = all && keys % 32 == 0 && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
+                    const bool whole = all && keys % 16 == 0 && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
                                        (last - s.before <= d.j0 || d.j0 + keys <= s.sinks);
                     if (!whole) {
                         d.flags |= 16u << t;
@@ -628,7 +656,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             const int st = step % C::STAGES;
             const uint32_t again = (step / C::STAGES) & 1;
             if (step >= C::STAGES) {
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_kempty[st], again ^ 1));
+                ok = wait_together(&s_kempty[st], again ^ 1);
                 if (!ok) {
                     break;
                 }
@@ -636,9 +664,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             if (lane == 0) {
                 s_steps[step % kStepSlots] = d;
                 if (d.keys > 0) {
-                    mbar_arrive_expect(&s_kfull[st], C::TILE_BYTES);
+                    mbar_arrive_expect(&s_kfull[st], C::KV_BYTES);
                     for (int x = 0; x < C::HALVES; ++x) {
-                        tma_tile(s_kt + st * C::TILE_BYTES + x * kHalfTileBytes, &k_map, 64 * x, d.j0, kh, b, &s_kfull[st]);
+                        tma_tile(s_kt + st * C::KV_BYTES + x * C::HALF_KV, &k_map, 64 * x, d.j0, kh, b, &s_kfull[st]);
                     }
                 } else {
                     mbar_arrive(&s_kfull[st]);
@@ -649,12 +677,12 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 break;
             }
             if (step >= C::STAGES) {
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_vempty[st], again ^ 1));
+                ok = wait_together(&s_vempty[st], again ^ 1);
             }
             if (ok && lane == 0) {
-                mbar_arrive_expect(&s_vfull[st], C::TILE_BYTES);
+                mbar_arrive_expect(&s_vfull[st], C::KV_BYTES);
                 for (int x = 0; x < C::HALVES; ++x) {
-                    tma_tile(s_vt + st * C::TILE_BYTES + x * kHalfTileBytes, &v_map, 64 * x, d.j0, kh, b, &s_vfull[st]);
+                    tma_tile(s_vt + st * C::KV_BYTES + x * C::HALF_KV, &v_map, 64 * x, d.j0, kh, b, &s_vfull[st]);
                 }
             }
             __syncwarp();
@@ -668,15 +696,17 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             }
         }
         __syncwarp();
-    } else if (warp == C::SOFTMAX_WARPS) {
-        // ---- matrix products: the warp walks together (its addresses stay in uniform registers), one lane issues
+    } else if (warp >= C::SOFTMAX_WARPS) {
+        // ---- matrix products of a tile: the warp walks together (its addresses stay in uniform registers), one lane issues
+        const int t = warp - C::SOFTMAX_WARPS;
         const uint32_t ksteps = (uint32_t) (s.dim + 15) / 16;
         const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((2 * ksteps) << 17) | ((kTileRows >> 4) << 24);   // N: the dimension, in 16s
         const bool leader = elect_one();
-        const uint64_t q_desc = swizzled_desc(smem_addr(s_qt), 16), k_desc = swizzled_desc(smem_addr(s_kt), 16);
-        const uint64_t v_desc = swizzled_desc(smem_addr(s_vt), kHalfTileBytes);
+        const uint64_t q_desc = swizzled_desc(smem_addr(s_qt + t * C::TILE_BYTES), 16), k_desc = swizzled_desc(smem_addr(s_kt), 16);
+        const uint64_t v_desc = swizzled_desc(smem_addr(s_vt), C::HALF_KV);
+        const uint32_t t_s = tmem + t * C::KEYS, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2), t_o = tmem + C::CONTEXT + t * DP;
         bool ok = wait_together(&s_qfull, 0);
-        uint32_t started = 0;   // bit t: O of tile t holds something
+        bool started = false;   // O holds something
         int keys_before = 0;
         uint32_t flags_before = 0;
         for (int step = 0; ok; ++step) {
@@ -686,56 +716,53 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 break;
             }
             const int keys = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].keys, 0);
-            const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0);
-            const uint32_t keys16 = (uint32_t) (keys + 15) / 16;
-            const uint32_t idesc_s = (1u << 4) | ((2 * keys16) << 17) | ((kTileRows >> 4) << 24);
+            const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0) >> t;
+            if (step > 0) {
+                ok = wait_together(&s_sfree[t], (step - 1) & 1);
+                tmem_fence_after();
+            }
+            if (ok && leader) {
+                if ((flags & 1u) != 0) {
+                    const uint64_t kd = k_desc + (uint64_t) (st * (C::KV_BYTES / 16));
+                    const uint32_t idesc_s = (1u << 4) | ((2 * ((uint32_t) (keys + 15) / 16)) << 17) | ((kTileRows >> 4) << 24);
 #pragma unroll
-            for (int t = 0; t < NQ; ++t) {
-                if (step > 0) {
-                    ok = ok && wait_together(&s_pfull[t], (step - 1) & 1);
-                    if (t == 0) {
-                        ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1);
-                    }
-                    tmem_fence_after();
-                    if (ok && (flags_before >> t & 1u) != 0) {
-                        const uint64_t vd = v_desc + (uint64_t) (st_before * (C::TILE_BYTES / 16));
-                        if (leader) {
-#pragma unroll
-                            for (int kk = 0; kk < kTileRows / 16; ++kk) {
-                                if (16 * kk < keys_before) {
-                                    mma_ts(tmem + NQ * 128 + t * DP, tmem + t * 128 + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || (started >> t & 1u) != 0);
-                                }
-                            }
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        if (kk < (int) ksteps) {
+                            mma_ss(t_s, q_desc + ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16, kd + ((kk >> 2) * C::HALF_KV + (kk & 3) * 32) / 16,
+                                   idesc_s, kk > 0);
                         }
-                        started |= 1u << t;
-                    }
-                    if (t == NQ - 1 && ok && leader) {
-                        mma_commit(&s_vempty[st_before]);
                     }
                 }
+                mma_commit(&s_sfull[t]);
+                mbar_arrive(&s_sfull[t]);
+                if (keys != 0) {
+                    mma_commit(&s_kempty[st]);
+                }
+            }
+            __syncwarp();
+            if (step > 0) {
+                ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
+                tmem_fence_after();
+                const bool takes_part = (flags_before & 1u) != 0;
                 if (ok && leader) {
-                    if ((flags >> t & 1u) != 0) {
-                        const uint64_t qd = q_desc + (uint64_t) (t * (C::TILE_BYTES / 16)), kd = k_desc + (uint64_t) (st * (C::TILE_BYTES / 16));
+                    if (takes_part) {
+                        const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
 #pragma unroll
-                        for (int kk = 0; kk < DP / 16; ++kk) {
-                            if (kk < (int) ksteps) {
-                                const uint32_t at = ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16;
-                                mma_ss(tmem + t * 128, qd + at, kd + at, idesc_s, kk > 0);
+                        for (int kk = 0; kk < C::KEYS / 16; ++kk) {
+                            if (16 * kk < keys_before) {
+                                mma_ts(t_o, t_p + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || started);
                             }
                         }
                     }
-                    mma_commit(&s_sfull[t]);
-                    mbar_arrive(&s_sfull[t]);
+                    mma_commit(&s_ofull[t]);
+                    mma_commit(&s_vempty[st_before]);
                 }
+                started = started || takes_part;
                 __syncwarp();
             }
             if (keys == 0) {
                 break;
             }
-            if (ok && leader) {
-                mma_commit(&s_kempty[st]);
-            }
-            __syncwarp();
             keys_before = keys;
             flags_before = flags;
         }
@@ -745,14 +772,15 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const int i = tile_row[t] + 32 * (warp & 3) + lane;
         const int h = tile_head[t];
         const uint32_t lanes = (uint32_t) (32 * (warp & 3)) << 16;
-        const uint32_t t_s = tmem + t * 128 + lanes, t_o = tmem + NQ * 128 + t * DP + lanes;
+        const uint32_t t_s = tmem + t * C::KEYS + lanes, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2) + lanes, t_o = tmem + C::CONTEXT + t * DP + lanes;
         const int lo = i > s.before ? i - s.before : 0;
         const int hi = s.after < s.seq - 1 - i ? i + s.after + 1 : s.seq;
         const float c = s.scale * kLog2e;
         float top = -INFINITY, total = 0.f;   // top: of q.k, unscaled
         bool first = true, ok = true;
-        for (int step = 0;; ++step) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_sfull[t], step & 1));
+        int step = 0;
+        for (;; ++step) {
+            ok = wait_together(&s_sfull[t], step & 1);
             if (!ok) {
                 break;
             }
@@ -763,23 +791,34 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 break;
             }
             const uint32_t flags = d->flags >> t;
-            if ((flags & 1u) != 0) {
-                uint32_t r[4][32];
+            const bool takes_part = (flags & 1u) != 0;
+            uint32_t r[C::CHUNKS][16];
+            float shrink = 1.f;
+            bool raise = false;
+            if (takes_part) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if (32 * w < keys) {
-                        tmem_load32(t_s + 32 * w, r[w]);
+                for (int w = 0; w < C::CHUNKS; ++w) {
+                    if (16 * w < keys) {
+                        tmem_load16(t_s + 16 * w, r[w]);
                     }
                 }
                 tmem_wait_loads();
+            }
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&s_sfree[t]);   // the next scores may come
+            }
+            if (takes_part) {
                 if ((flags & 16u) != 0) {
                     const int j0 = d->j0;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        if (32 * w < keys) {
-                            const uint32_t see = d->kept[w] & (range_bits(lo, hi, j0 + 32 * w) | range_bits(0, min(s.sinks, hi), j0 + 32 * w));
+                    for (int w = 0; w < C::CHUNKS; ++w) {
+                        if (16 * w < keys) {
+                            const uint32_t see = (d->kept[w / 2] >> (16 * (w & 1))) &
+                                                 (range_bits(lo, hi, j0 + 16 * w) | range_bits(0, min(s.sinks, hi), j0 + 16 * w));
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
+                            for (int e = 0; e < 16; ++e) {
                                 r[w][e] = (see >> e & 1u) != 0 ? r[w][e] : 0xff800000u;
                             }
                         }
@@ -787,10 +826,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 }
                 float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if (32 * w < keys) {
+                for (int w = 0; w < C::CHUNKS; ++w) {
+                    if (16 * w < keys) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
+                        for (int e = 0; e < 16; e += 4) {
                             m0 = fmaxf(m0, __uint_as_float(r[w][e]));
                             m1 = fmaxf(m1, __uint_as_float(r[w][e + 1]));
                             m2 = fmaxf(m2, __uint_as_float(r[w][e + 2]));
@@ -799,24 +838,47 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     }
                 }
                 const float here = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-                const bool raise = (here - top) * c > kRaiseBy;   // the first visible key: infinity > 8
-                float shrink = 1.f;
+                raise = (here - top) * c > kRaiseBy;   // the first visible key: infinity > 8
                 if (raise) {
                     shrink = fast_exp2((top - here) * c);
                     top = here;
                 }
+                const float2 c2 = splat2(c), nt2 = splat2(top == -INFINITY ? 0.f : -top * c);
+                float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < C::CHUNKS; ++w) {
+                    if (16 * w < keys) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            float2 a = fma2(make_float2(__uint_as_float(r[w][e]), __uint_as_float(r[w][e + 1])), c2, nt2);
+                            float2 z = fma2(make_float2(__uint_as_float(r[w][e + 2]), __uint_as_float(r[w][e + 3])), c2, nt2);
+                            a = make_float2(fast_exp2(a.x), fast_exp2(a.y));
+                            z = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+                            sum0 = add2(sum0, a);
+                            sum1 = add2(sum1, z);
+                            const __half2 pa = __float22half2_rn(a), pz = __float22half2_rn(z);
+                            r[w][e / 2] = *reinterpret_cast<const uint32_t *>(&pa);
+                            r[w][e / 2 + 1] = *reinterpret_cast<const uint32_t *>(&pz);
+                        }
+                    }
+                }
+                sum0 = add2(sum0, sum1);
+                total = fmaf(total, shrink, sum0.x + sum0.y);
+            }
+            if (step > 0) {   // the product of the step before has read its weights and added to O
+                ok = wait_together(&s_ofull[t], (step - 1) & 1);
+                if (!ok) {
+                    break;
+                }
+                tmem_fence_after();
+            }
+            if (takes_part) {
                 if (!first && __any_sync(0xffffffffu, raise)) {
-                    // the products into O are done: they were issued before this step's scores
                     const float2 sh2 = splat2(shrink);
                     for (int x = 0; x < s.dim; x += 16) {
                         uint32_t o[16];
-                        asm volatile(
-                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-                            "tcgen05.wait::ld.sync.aligned;"
-                            : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]), "=r"(o[8]),
-                              "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-                            : "r"(t_o + x)
-                            : "memory");
+                        tmem_load16(t_o + x, o);
+                        tmem_wait_loads();
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
                             const float2 v2 = mul2(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), sh2);
@@ -827,29 +889,12 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     }
                 }
                 first = false;
-                const float2 c2 = splat2(c), nt2 = splat2(top == -INFINITY ? 0.f : -top * c);
-                float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if (32 * w < keys) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            float2 a = fma2(make_float2(__uint_as_float(r[w][e]), __uint_as_float(r[w][e + 1])), c2, nt2);
-                            float2 z = fma2(make_float2(__uint_as_float(r[w][e + 2]), __uint_as_float(r[w][e + 3])), c2, nt2);
-                            a = make_float2(fast_exp2(a.x), fast_exp2(a.y));
-                            z = make_float2(fast_exp2(z.x), fast_exp2(z.y));
-                            sum0 = add2(sum0, a);
-                            sum1 = add2(sum1, z);
-                            const __half2 pa = __float22half2_rn(a), pz = __float22half2_rn(z);
-                            p[e / 2] = *reinterpret_cast<const uint32_t *>(&pa);
-                            p[e / 2 + 1] = *reinterpret_cast<const uint32_t *>(&pz);
-                        }
-                        tmem_store16(t_s + 16 * w, p);
+                for (int w = 0; w < C::CHUNKS; ++w) {
+                    if (16 * w < keys) {
+                        tmem_store8(t_p + 8 * w, r[w]);
                     }
                 }
-                sum0 = add2(sum0, sum1);
-                total = fmaf(total, shrink, sum0.x + sum0.y);
                 tmem_wait_stores();
             }
             tmem_fence_before();
@@ -858,7 +903,11 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 mbar_arrive(&s_pfull[t]);
             }
         }
-        // ---- context rows (the last completion covers every product into O)
+        if (ok && step > 0) {
+            ok = wait_together(&s_ofull[t], (step - 1) & 1);
+            tmem_fence_after();
+        }
+        // ---- context rows
         const float inv = !ok ? NAN : (total == 0.f ? 0.f : 1.f / total);
         bool finite = true;
         __half *out = context + ((int64_t) b * s.seq + i) * s.context_stride + (int64_t) h * s.dim;
@@ -933,12 +982,12 @@ inline EncodeTiled encode_tiled() {
     return fn;
 }
 
-// [batch, heads, seq, dim] view of rows `stride` elements apart, read in boxes of 128 rows x 64 columns.
-inline bool window_map(CUtensorMap *map, const __half *p, int dim, int seq, int heads, int batch, int64_t stride) {
+// [batch, heads, seq, dim] view of rows `stride` elements apart, read in boxes of `rows` rows x 64 columns.
+inline bool window_map(CUtensorMap *map, const __half *p, int dim, int seq, int heads, int batch, int64_t stride, int rows) {
     const EncodeTiled encode = encode_tiled();
     const cuuint64_t dims[4] = {(cuuint64_t) dim, (cuuint64_t) seq, (cuuint64_t) heads, (cuuint64_t) batch};
     const cuuint64_t strides[3] = {(cuuint64_t) stride * 2, (cuuint64_t) dim * 2, (cuuint64_t) seq * (cuuint64_t) stride * 2};
-    const cuuint32_t box[4] = {64, kTileRows, 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t) rows, 1, 1}, step[4] = {1, 1, 1, 1};
     if (encode == nullptr || !aligned16(p) || strides[0] % 16 != 0 || strides[1] % 16 != 0 || strides[0] >= (1ull << 40) || strides[2] >= (1ull << 40)) {
         return false;
     }
@@ -980,8 +1029,10 @@ int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
 inline int window_tc(const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context, const WindowShape &s,
                      cudaStream_t stream) {
     CUtensorMap qm, km, vm;
-    if (s.dim > 128 || !(s.scale > 0.f) || !window_map(&qm, q, s.dim, s.seq, s.heads, s.batch, s.q_stride) ||
-        !window_map(&km, k, s.dim, s.seq, s.kv_heads, s.batch, s.kv_stride) || !window_map(&vm, v, s.dim, s.seq, s.kv_heads, s.batch, s.kv_stride)) {
+    const int keys = s.dim <= 64 ? WindowTc<64, 1>::KEYS : WindowTc<128, 2>::KEYS;
+    if (s.dim > 128 || !(s.scale > 0.f) || !window_map(&qm, q, s.dim, s.seq, s.heads, s.batch, s.q_stride, kTileRows) ||
+        !window_map(&km, k, s.dim, s.seq, s.kv_heads, s.batch, s.kv_stride, keys) ||
+        !window_map(&vm, v, s.dim, s.seq, s.kv_heads, s.batch, s.kv_stride, keys)) {
         return CUBK_ERR_UNSUPPORTED;
     }
     return s.dim <= 64 ? window_tc_launch<64, 1>(qm, km, vm, q, k, v, mask, context, s, stream)
