@@ -10,6 +10,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -383,7 +384,8 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 }
 
 // ---------------------------------------------------------------- whole sequences on tcgen05 (binary16)
-// A block owns NQ tiles of 128 query rows: two heads that share their keys, or consecutive rows of one head. Per step of up
+// A work item is NQ tiles of 128 query rows: two heads that share their keys, or consecutive rows of one head; blocks are
+// persistent and walk over items, loading and multiplying ahead into the next while the last one's rows are written. Per step of up
 // to KEYS keys and per tile: S = Q.K^T (tcgen05.mma, float32 accumulators in tensor memory), softmax by 128 threads that own
 // a row each (tensor-memory lane = query row, so no shuffles), P back into tensor memory as binary16, O += P.V with P as the
 // tensor-memory operand. Warps: 4 NQ for the softmax, NQ that issue the MMAs of a tile, one that chooses the steps and loads K
@@ -391,7 +393,7 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 //   * The scores' place is free as soon as a row is in registers, so the next step's scores are computed while this step's
 //     exponentials are; the weights have a place of their own, so their product runs under the next step's softmax. KEYS is what
 //     fits beside the contexts: 128 for heads of up to 64 (two blocks of one tile share an SM), 80 for 128 (one of two tiles).
-//   * Steps: first the sinks below the window, then the window. A step whose keys are all masked is left out; one that every row of
+//   * Steps of an item: first the sinks below the window, then the window, then one without keys that ends it. A step whose keys are all masked is left out; one that every row of
 //     a tile sees whole skips the masking.
 //   * The running maximum of a row is raised only when a step's maximum exceeds it by 2^8 (a weight is then at most 256, far
 //     inside binary16, and the sums are float32), so that O is read back and scaled in few steps.
@@ -402,9 +404,10 @@ constexpr int kTileRows = 128;
 constexpr int kHalfTileBytes = kTileRows * 128;    // 128 rows x 64 binary16
 constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 2
 constexpr float kRaiseBy = 8.f;                    // log2 of the largest weight
+constexpr int kMaskSteps = 48;                     // steps whose mask bits are gathered ahead
 
 struct WindowStep {
-    int j0, keys;            // keys = 0: no more steps
+    int j0, columns;         // columns: KEYS, 16 where no more keys are left, 0 at the end of an item
     uint32_t kept[4];
     uint32_t flags;          // bit t: tile t takes part; bit 4 + t: some row of tile t does not see some key
 };
@@ -416,12 +419,16 @@ struct WindowTc {
     static constexpr int HALVES = DP / 64;
     static constexpr int TILE_BYTES = HALVES * kHalfTileBytes;
     static constexpr int HALF_KV = KEYS * 128, KV_BYTES = HALVES * HALF_KV;
-    static constexpr int STAGES = DP == 64 ? 2 : 3;
+    static constexpr int STAGES = 2, QUERIES = 2;            // tiles of K and V, and of Q, on their way or in use
     static constexpr int SOFTMAX_WARPS = 4 * NQ;
-    static constexpr int THREADS = 32 * (SOFTMAX_WARPS + NQ + 1);
+    // Softmax warps in whole groups of four, and one more group for the others (the last of it idle), which hands most of its
+    // registers to them. Launched with 65536 / (THREADS x blocks per SM) each: 128 x 256 >= 192 x 128 + 56 x 128, 168 x 384 >= 224 x 256 + 56 x 128.
+    static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
+    static constexpr int LAUNCH_REGS = NQ == 1 ? 128 : 168, SOFTMAX_REGS = NQ == 1 ? 192 : 224, OTHER_REGS = 56;
+    static_assert(LAUNCH_REGS * THREADS >= SOFTMAX_REGS * 32 * SOFTMAX_WARPS + OTHER_REGS * 128, "a group that asks for more would wait forever");
     static constexpr int WEIGHTS = NQ * KEYS, CONTEXT = WEIGHTS + NQ * KEYS / 2;   // columns of tensor memory behind the scores
     static constexpr int TMEM_COLS = NQ == 1 ? 256 : 512;
-    static constexpr int SMEM_BYTES = 1024 + NQ * TILE_BYTES + 2 * STAGES * KV_BYTES;   // 1024: alignment of the swizzled tiles
+    static constexpr int SMEM_BYTES = 1024 + QUERIES * NQ * TILE_BYTES + 2 * STAGES * KV_BYTES;   // 1024: alignment of the swizzled tiles
     static_assert(CONTEXT + NQ * DP <= TMEM_COLS, "scores, weights and contexts of all tiles");
     static_assert(STAGES + 2 < kStepSlots, "a descriptor outlives its step");
 };
@@ -522,6 +529,13 @@ __device__ __forceinline__ void tma_tile(void *dst, const CUtensorMap *map, int 
                  : "memory");
 }
 
+// The largest of three, NaN if any is: one instruction.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Bits lo .. hi - 1 of a word that stands for positions base .. base + 31.
 __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int base) {
     const int a = min(max(lo - base, 0), 32), b = min(max(hi - base, 0), 32);
@@ -535,45 +549,60 @@ __device__ __noinline__ void window_row_again(const __half *q, const __half *k, 
     window_prompt_row<__half>(q, k, v, mask, context, *s, s_q, b, i, h);
 }
 
+// The rows and heads of a work item.
+template <int NQ>
+struct WindowItem {
+    int b, kh, row0, last_row, tile_row[NQ], tile_head[NQ];
+
+    __device__ __forceinline__ WindowItem(int item, const WindowShape &s, int row_blocks, int pair_heads) {
+        const int rb = row_blocks - 1 - item % row_blocks;   // last rows first: with a one-sided window they have the most keys
+        const int bh = item / row_blocks, head_groups = pair_heads ? s.heads / 2 : s.heads;
+        b = bh / head_groups;
+        const int h0 = (bh - b * head_groups) * (pair_heads ? 2 : 1);
+        const int tiles = pair_heads ? 1 : NQ;
+        row0 = rb * tiles * kTileRows;
+        last_row = min(row0 + tiles * kTileRows, s.seq) - 1;
+        kh = h0 / (s.heads / s.kv_heads);
+#pragma unroll
+        for (int t = 0; t < NQ; ++t) {
+            tile_row[t] = pair_heads ? row0 : row0 + t * kTileRows;
+            tile_head[t] = pair_heads ? h0 + t : h0;
+        }
+    }
+};
+
 template <int DP, int NQ>
 __global__ void __launch_bounds__(WindowTc<DP, NQ>::THREADS, NQ == 1 ? 2 : 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                  const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context, const __grid_constant__ WindowShape s,
-                 int row_blocks, int pair_heads) {
+                 int items, int row_blocks, int pair_heads) {
     typedef WindowTc<DP, NQ> C;
     extern __shared__ unsigned char tc_raw[];
-    __shared__ uint64_t s_qfull, s_kfull[C::STAGES], s_kempty[C::STAGES], s_vfull[C::STAGES], s_vempty[C::STAGES];
+    __shared__ uint64_t s_qfull[C::QUERIES], s_qempty[C::QUERIES], s_kfull[C::STAGES], s_kempty[C::STAGES], s_vfull[C::STAGES], s_vempty[C::STAGES];
     __shared__ uint64_t s_sfull[NQ], s_sfree[NQ], s_pfull[NQ], s_ofull[NQ];   // scores written, scores read, weights written, O added to
     __shared__ uint32_t s_tmem;
     __shared__ WindowStep s_steps[kStepSlots];
     __shared__ float s_row[C::SOFTMAX_WARPS][kWindowMaxDim];
+    __shared__ uint32_t s_bits[kMaskSteps][4];
     unsigned char *tiles = tc_raw + ((1024u - (smem_addr(tc_raw) & 1023u)) & 1023u);
-    unsigned char *s_qt = tiles, *s_kt = tiles + NQ * C::TILE_BYTES, *s_vt = s_kt + C::STAGES * C::KV_BYTES;
+    unsigned char *s_qt = tiles, *s_kt = tiles + C::QUERIES * NQ * C::TILE_BYTES, *s_vt = s_kt + C::STAGES * C::KV_BYTES;
     const int warp = __shfl_sync(0xffffffffu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-    // the block's tiles: last rows first (with a one-sided window that reaches far, they have the most keys)
-    const int per_head = row_blocks;
-    const int rb = per_head - 1 - (int) (blockIdx.x % per_head);
-    const int bh = (int) (blockIdx.x / per_head);
-    const int head_groups = pair_heads ? s.heads / 2 : s.heads;
-    const int b = bh / head_groups;
-    const int h0 = (bh - b * head_groups) * (pair_heads ? 2 : 1);
-    const int row0 = rb * (pair_heads ? kTileRows : NQ * kTileRows);
-    const int kh = h0 / (s.heads / s.kv_heads);
-    int tile_row[NQ], tile_head[NQ];
-#pragma unroll
-    for (int t = 0; t < NQ; ++t) {
-        tile_row[t] = pair_heads ? row0 : row0 + t * kTileRows;
-        tile_head[t] = pair_heads ? h0 + t : h0;
+    if (threadIdx.x == 64) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     }
-
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"((uint32_t) C::TMEM_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (threadIdx.x == 32) {
-        mbar_init(&s_qfull, 1);
+        for (int i = 0; i < C::QUERIES; ++i) {
+            mbar_init(&s_qfull[i], 1);
+            mbar_init(&s_qempty[i], NQ);
+        }
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&s_kfull[i], 1);
             mbar_init(&s_kempty[i], NQ);
@@ -593,110 +622,136 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     tmem_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
 
+    // Every barrier below completes one phase per step (or item), whatever the step is, so `step` and `turn`, which count through
+    // all items, give their parities.
+    if (warp >= C::SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
     if (warp == C::SOFTMAX_WARPS + NQ) {
         // ---- steps and loads
-        const int last_row = min(row0 + (pair_heads ? 1 : NQ) * kTileRows, s.seq) - 1;
-        const int lo = row0 > s.before ? row0 - s.before : 0;
-        const int hi = s.after < s.seq - 1 - last_row ? last_row + s.after + 1 : s.seq;
-        const int sinks_end = min(s.sinks, lo);
-        const int8_t *kept = mask != nullptr ? mask + (int64_t) b * s.seq : nullptr;
-        if (lane == 0) {
-            mbar_arrive_expect(&s_qfull, NQ * C::TILE_BYTES);
-            for (int t = 0; t < NQ; ++t) {
-                for (int x = 0; x < C::HALVES; ++x) {
-                    tma_tile(s_qt + t * C::TILE_BYTES + x * kHalfTileBytes, &q_map, 64 * x, tile_row[t], tile_head[t], b, &s_qfull);
-                }
-            }
-        }
         bool ok = true;
-        int step = 0;
-        int j0 = sinks_end > 0 ? 0 : lo;
-        bool in_sinks = sinks_end > 0;
-        while (ok) {
-            if (in_sinks && j0 >= sinks_end) {
-                in_sinks = false;
-                j0 = lo;
-            }
-            const int keys = min((in_sinks ? sinks_end : hi) - j0, C::KEYS);   // none left: 0 or less (only past the window)
-            WindowStep d;
-            d.j0 = j0;
-            d.keys = max(keys, 0);
-            d.flags = 0;
-            bool all = true;
-            uint32_t some = 0;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int j = j0 + 32 * w + lane;
-                const bool in = 32 * w + lane < keys;
-                const bool on = in && (kept == nullptr || kept[j] != 0);
-                d.kept[w] = __ballot_sync(0xffffffffu, on);
-                some |= d.kept[w];
-                all = all && __all_sync(0xffffffffu, on || !in);
-            }
-            j0 += C::KEYS;
-            if (keys > 0) {
-                if (some == 0) {
-                    continue;
-                }
-#pragma unroll
-                for (int t = 0; t < NQ; ++t) {
-                    const int first = tile_row[t], last = min(first + kTileRows, s.seq) - 1;
-                    const int t_lo = first > s.before ? first - s.before : 0;
-                    const int t_hi = s.after < s.seq - 1 - last ? last + s.after + 1 : s.seq;
-                    if (first < s.seq && d.j0 < t_hi && (d.j0 + keys > t_lo || d.j0 < s.sinks)) {
-                        d.flags |= 1u << t;
-                    }
-                    const bool whole = all && keys % 16 == 0 && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
-                                       (last - s.before <= d.j0 || d.j0 + keys <= s.sinks);
-                    if (!whole) {
-                        d.flags |= 16u << t;
-                    }
-                }
-            }
-            const int st = step % C::STAGES;
-            const uint32_t again = (step / C::STAGES) & 1;
-            if (step >= C::STAGES) {
-                ok = wait_together(&s_kempty[st], again ^ 1);
-                if (!ok) {
-                    break;
-                }
-            }
-            if (lane == 0) {
-                s_steps[step % kStepSlots] = d;
-                if (d.keys > 0) {
-                    mbar_arrive_expect(&s_kfull[st], C::KV_BYTES);
-                    for (int x = 0; x < C::HALVES; ++x) {
-                        tma_tile(s_kt + st * C::KV_BYTES + x * C::HALF_KV, &k_map, 64 * x, d.j0, kh, b, &s_kfull[st]);
-                    }
-                } else {
-                    mbar_arrive(&s_kfull[st]);
-                }
-            }
-            __syncwarp();
-            if (d.keys == 0) {
-                break;
-            }
-            if (step >= C::STAGES) {
-                ok = wait_together(&s_vempty[st], again ^ 1);
+        int step = 0, turn = 0;
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++turn) {
+            const WindowItem<NQ> w(item, s, row_blocks, pair_heads);
+            const int lo = w.row0 > s.before ? w.row0 - s.before : 0;
+            const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
+            const int sinks_end = min(s.sinks, lo), sink_steps = (sinks_end + C::KEYS - 1) / C::KEYS;
+            const int steps = sink_steps + (hi - lo + C::KEYS - 1) / C::KEYS;
+            const int8_t *kept = mask != nullptr ? mask + (int64_t) w.b * s.seq : nullptr;
+            const int qb = turn % C::QUERIES;
+            if (turn >= C::QUERIES) {
+                ok = wait_together(&s_qempty[qb], (turn / C::QUERIES - 1) & 1);
             }
             if (ok && lane == 0) {
-                mbar_arrive_expect(&s_vfull[st], C::KV_BYTES);
-                for (int x = 0; x < C::HALVES; ++x) {
-                    tma_tile(s_vt + st * C::KV_BYTES + x * C::HALF_KV, &v_map, 64 * x, d.j0, kh, b, &s_vfull[st]);
+                mbar_arrive_expect(&s_qfull[qb], NQ * C::TILE_BYTES);
+                for (int t = 0; t < NQ; ++t) {
+                    for (int x = 0; x < C::HALVES; ++x) {
+                        tma_tile(s_qt + (qb * NQ + t) * C::TILE_BYTES + x * kHalfTileBytes, &q_map, 64 * x, w.tile_row[t], w.tile_head[t], w.b,
+                                 &s_qfull[qb]);
+                    }
                 }
             }
-            __syncwarp();
-            ++step;
-        }
-        if (!ok) {   // the copies in flight land before the block's shared memory goes
-            (void) mbar_wait_bounded(&s_qfull, 0);
-            for (int i = max(step - C::STAGES, 0); i <= step; ++i) {
-                (void) mbar_wait_bounded(&s_kfull[i % C::STAGES], (i / C::STAGES) & 1);
-                (void) mbar_wait_bounded(&s_vfull[i % C::STAGES], (i / C::STAGES) & 1);
+            const bool gathered = kept != nullptr && steps <= kMaskSteps;
+            if (gathered) {   // the item's mask bits, eight loads in flight
+                for (int w0 = 0; w0 < steps * 4; w0 += 8) {
+                    int8_t byte[8];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const int at = (w0 + u) / 4, in_step = 32 * ((w0 + u) & 3) + lane;
+                        const int j = (at < sink_steps ? 0 : lo - sink_steps * C::KEYS) + at * C::KEYS + in_step;
+                        byte[u] = at < steps && in_step < C::KEYS && j < (at < sink_steps ? sinks_end : hi) ? kept[j] : (int8_t) 0;
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const uint32_t bits = __ballot_sync(0xffffffffu, byte[u] != 0);
+                        if (lane == 0 && w0 + u < steps * 4) {
+                            (&s_bits[0][0])[w0 + u] = bits;
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            for (int at = 0; at <= steps && ok; ++at) {
+                const bool in_sinks = at < sink_steps;
+                WindowStep d;
+                d.j0 = in_sinks ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS;
+                const int keys = at < steps ? min((in_sinks ? sinks_end : hi) - d.j0, C::KEYS) : 0;
+                d.columns = keys == 0 ? 0 : keys <= 16 ? 16 : C::KEYS;
+                d.flags = 0;
+                int count = 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (gathered) {
+                        d.kept[u] = at < steps ? s_bits[at][u] : 0;
+                    } else {
+                        const bool in = 32 * u + lane < keys;
+                        d.kept[u] = __ballot_sync(0xffffffffu, in && (kept == nullptr || kept[d.j0 + 32 * u + lane] != 0));
+                    }
+                    count += __popc(d.kept[u]);
+                }
+                if (keys > 0) {
+                    if (count == 0) {
+                        continue;
+                    }
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t) {
+                        const int first = w.tile_row[t], last = min(first + kTileRows, s.seq) - 1;
+                        const int t_lo = first > s.before ? first - s.before : 0;
+                        const int t_hi = s.after < s.seq - 1 - last ? last + s.after + 1 : s.seq;
+                        if (first < s.seq && d.j0 < t_hi && (d.j0 + keys > t_lo || d.j0 < s.sinks)) {
+                            d.flags |= 1u << t;
+                        }
+                        const bool whole = count == d.columns && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
+                                           (last - s.before <= d.j0 || d.j0 + keys <= s.sinks);
+                        if (!whole) {
+                            d.flags |= 16u << t;
+                        }
+                    }
+                }
+                const int st = step % C::STAGES;
+                const uint32_t before = (step / C::STAGES - 1) & 1;
+                if (step >= C::STAGES) {
+                    ok = wait_together(&s_kempty[st], before);
+                }
+                if (ok && lane == 0) {
+                    s_steps[step % kStepSlots] = d;
+                    if (keys > 0) {
+                        mbar_arrive_expect(&s_kfull[st], C::KV_BYTES);
+                        for (int x = 0; x < C::HALVES; ++x) {
+                            tma_tile(s_kt + st * C::KV_BYTES + x * C::HALF_KV, &k_map, 64 * x, d.j0, w.kh, w.b, &s_kfull[st]);
+                        }
+                    } else {
+                        mbar_arrive(&s_kfull[st]);
+                    }
+                }
+                __syncwarp();
+                if (ok && step >= C::STAGES) {
+                    ok = wait_together(&s_vempty[st], before);
+                }
+                if (ok && lane == 0) {
+                    if (keys > 0) {
+                        mbar_arrive_expect(&s_vfull[st], C::KV_BYTES);
+                        for (int x = 0; x < C::HALVES; ++x) {
+                            tma_tile(s_vt + st * C::KV_BYTES + x * C::HALF_KV, &v_map, 64 * x, d.j0, w.kh, w.b, &s_vfull[st]);
+                        }
+                    } else {
+                        mbar_arrive(&s_vfull[st]);
+                    }
+                }
+                __syncwarp();
+                step += ok ? 1 : 0;
             }
         }
-        __syncwarp();
-    } else if (warp >= C::SOFTMAX_WARPS) {
+        if (!ok) {   // the copies in flight land before the block's shared memory goes
+            for (int i = max(turn - C::QUERIES, 0); i <= turn; ++i) {
+                (void) wait_together(&s_qfull[i % C::QUERIES], (i / C::QUERIES) & 1);
+            }
+            for (int i = max(step - C::STAGES, 0); i <= step; ++i) {
+                (void) wait_together(&s_kfull[i % C::STAGES], (i / C::STAGES) & 1);
+                (void) wait_together(&s_vfull[i % C::STAGES], (i / C::STAGES) & 1);
+            }
+        }
+    } else if (warp < C::SOFTMAX_WARPS + NQ) {
         // ---- matrix products of a tile: the warp walks together (its addresses stay in uniform registers), one lane issues
         const int t = warp - C::SOFTMAX_WARPS;
         const uint32_t ksteps = (uint32_t) (s.dim + 15) / 16;
@@ -705,140 +760,129 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const uint64_t q_desc = swizzled_desc(smem_addr(s_qt + t * C::TILE_BYTES), 16), k_desc = swizzled_desc(smem_addr(s_kt), 16);
         const uint64_t v_desc = swizzled_desc(smem_addr(s_vt), C::HALF_KV);
         const uint32_t t_s = tmem + t * C::KEYS, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2), t_o = tmem + C::CONTEXT + t * DP;
-        bool ok = wait_together(&s_qfull, 0);
-        bool started = false;   // O holds something
-        int keys_before = 0;
+        bool ok = true, started = false;   // started: O holds something of this item
+        int columns_before = 0, step = 0, turn = 0;
         uint32_t flags_before = 0;
-        for (int step = 0; ok; ++step) {
-            const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES;
-            ok = wait_together(&s_kfull[st], (step / C::STAGES) & 1);
-            if (!ok) {
-                break;
-            }
-            const int keys = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].keys, 0);
-            const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0) >> t;
-            if (step > 0) {
-                ok = wait_together(&s_sfree[t], (step - 1) & 1);
-                tmem_fence_after();
-            }
-            if (ok && leader) {
-                if ((flags & 1u) != 0) {
-                    const uint64_t kd = k_desc + (uint64_t) (st * (C::KV_BYTES / 16));
-                    const uint32_t idesc_s = (1u << 4) | ((2 * ((uint32_t) (keys + 15) / 16)) << 17) | ((kTileRows >> 4) << 24);
-#pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk) {
-                        if (kk < (int) ksteps) {
-                            mma_ss(t_s, q_desc + ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16, kd + ((kk >> 2) * C::HALF_KV + (kk & 3) * 32) / 16,
-                                   idesc_s, kk > 0);
-                        }
-                    }
+        for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++turn) {
+            const int qb = turn % C::QUERIES;
+            ok = wait_together(&s_qfull[qb], (turn / C::QUERIES) & 1);
+            const uint64_t qd = q_desc + (uint64_t) (qb * NQ * (C::TILE_BYTES / 16));
+            for (int columns = 1; ok && columns != 0; ++step) {
+                const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES;
+                ok = wait_together(&s_kfull[st], (step / C::STAGES) & 1);
+                columns = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].columns, 0);
+                const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0) >> t;
+                if (step > 0) {
+                    ok = ok && wait_together(&s_sfree[t], (step - 1) & 1);
+                    tmem_fence_after();
                 }
-                mma_commit(&s_sfull[t]);
-                mbar_arrive(&s_sfull[t]);
-                if (keys != 0) {
-                    mma_commit(&s_kempty[st]);
-                }
-            }
-            __syncwarp();
-            if (step > 0) {
-                ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
-                tmem_fence_after();
-                const bool takes_part = (flags_before & 1u) != 0;
                 if (ok && leader) {
-                    if (takes_part) {
-                        const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
+                    if ((flags & 1u) != 0) {
+                        const uint64_t kd = k_desc + (uint64_t) (st * (C::KV_BYTES / 16));
+                        const uint32_t idesc_s = (1u << 4) | ((uint32_t) (columns / 8) << 17) | ((kTileRows >> 4) << 24);
 #pragma unroll
-                        for (int kk = 0; kk < C::KEYS / 16; ++kk) {
-                            if (16 * kk < keys_before) {
-                                mma_ts(t_o, t_p + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || started);
+                        for (int kk = 0; kk < DP / 16; ++kk) {
+                            if (kk < (int) ksteps) {
+                                mma_ss(t_s, qd + ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16, kd + ((kk >> 2) * C::HALF_KV + (kk & 3) * 32) / 16,
+                                       idesc_s, kk > 0);
                             }
                         }
                     }
-                    mma_commit(&s_ofull[t]);
-                    mma_commit(&s_vempty[st_before]);
-                }
-                started = started || takes_part;
-                __syncwarp();
-            }
-            if (keys == 0) {
-                break;
-            }
-            keys_before = keys;
-            flags_before = flags;
-        }
-    } else {
-        // ---- softmax: a row per thread
-        const int t = NQ == 1 ? 0 : warp / 4;
-        const int i = tile_row[t] + 32 * (warp & 3) + lane;
-        const int h = tile_head[t];
-        const uint32_t lanes = (uint32_t) (32 * (warp & 3)) << 16;
-        const uint32_t t_s = tmem + t * C::KEYS + lanes, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2) + lanes, t_o = tmem + C::CONTEXT + t * DP + lanes;
-        const int lo = i > s.before ? i - s.before : 0;
-        const int hi = s.after < s.seq - 1 - i ? i + s.after + 1 : s.seq;
-        const float c = s.scale * kLog2e;
-        float top = -INFINITY, total = 0.f;   // top: of q.k, unscaled
-        bool first = true, ok = true;
-        int step = 0;
-        for (;; ++step) {
-            ok = wait_together(&s_sfull[t], step & 1);
-            if (!ok) {
-                break;
-            }
-            tmem_fence_after();
-            const WindowStep *d = &s_steps[step % kStepSlots];
-            const int keys = d->keys;
-            if (keys == 0) {
-                break;
-            }
-            const uint32_t flags = d->flags >> t;
-            const bool takes_part = (flags & 1u) != 0;
-            uint32_t r[C::CHUNKS][16];
-            float shrink = 1.f;
-            bool raise = false;
-            if (takes_part) {
-#pragma unroll
-                for (int w = 0; w < C::CHUNKS; ++w) {
-                    if (16 * w < keys) {
-                        tmem_load16(t_s + 16 * w, r[w]);
+                    mma_commit(&s_sfull[t]);
+                    mbar_arrive(&s_sfull[t]);
+                    mma_commit(&s_kempty[st]);
+                    if (columns == 0) {
+                        mma_commit(&s_qempty[qb]);
                     }
                 }
+                __syncwarp();
+                if (step > 0) {   // O += P.V of the step before; of one that ended an item, only the wait until O has been read
+                    ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
+                    tmem_fence_after();
+                    const bool takes_part = (flags_before & 1u) != 0;
+                    if (ok && leader) {
+                        if (takes_part) {
+                            const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
+#pragma unroll
+                            for (int kk = 0; kk < C::KEYS / 16; ++kk) {
+                                if (16 * kk < columns_before) {
+                                    mma_ts(t_o, t_p + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || started);
+                                }
+                            }
+                        }
+                        mma_commit(&s_ofull[t]);
+                        mma_commit(&s_vempty[st_before]);
+                    }
+                    started = columns_before != 0 && (started || takes_part);
+                    __syncwarp();
+                }
+                columns_before = columns;
+                flags_before = flags;
+            }
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
+        // ---- softmax: a row per thread
+        const int t = NQ == 1 ? 0 : warp / 4;
+        const uint32_t lanes = (uint32_t) (32 * (warp & 3)) << 16;
+        const uint32_t t_s = tmem + t * C::KEYS + lanes, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2) + lanes, t_o = tmem + C::CONTEXT + t * DP + lanes;
+        const float c = s.scale * kLog2e;
+        const bool vec = (reinterpret_cast<uintptr_t>(context) & 15) == 0 && s.context_stride % 8 == 0;
+        bool ok = true;
+        int step = 0;
+        for (int item = blockIdx.x; item < items; item += gridDim.x) {
+            const WindowItem<NQ> work(item, s, row_blocks, pair_heads);
+            const int h = work.tile_head[t], i = work.tile_row[t] + 32 * (warp & 3) + lane;
+            const int lo = i > s.before ? i - s.before : 0;
+            const int hi = s.after < s.seq - 1 - i ? i + s.after + 1 : s.seq;
+            float top = -INFINITY, total = 0.f;   // top: of q.k, unscaled
+            bool first = true;
+            // One step of this row. The number of its 16-column chunks is fixed, so that its loops have no branches and the exponentials of
+            // one chunk overlap the arithmetic of the next (a branch per chunk costs a third of the rate).
+            auto softmax_step = [&](auto chunks, const WindowStep *d, uint32_t flags) {
+                constexpr int CHUNKS = decltype(chunks)::value;
+                uint32_t r[CHUNKS][16];
+#pragma unroll
+                for (int w = 0; w < CHUNKS; ++w) {
+                    tmem_load16(t_s + 16 * w, r[w]);
+                }
+                if (step > 0) {   // while they arrive: the product of the step before has read its weights and added to O
+                    ok = wait_together(&s_ofull[t], (step - 1) & 1);
+                    tmem_fence_after();
+                }
                 tmem_wait_loads();
-            }
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&s_sfree[t]);   // the next scores may come
-            }
-            if (takes_part) {
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&s_sfree[t]);   // the next scores may come
+                }
                 if ((flags & 16u) != 0) {
                     const int j0 = d->j0;
 #pragma unroll
-                    for (int w = 0; w < C::CHUNKS; ++w) {
-                        if (16 * w < keys) {
-                            const uint32_t see = (d->kept[w / 2] >> (16 * (w & 1))) &
-                                                 (range_bits(lo, hi, j0 + 16 * w) | range_bits(0, min(s.sinks, hi), j0 + 16 * w));
+                    for (int w = 0; w < CHUNKS; ++w) {
+                        const uint32_t see = (d->kept[w / 2] >> (16 * (w & 1))) &
+                                             (range_bits(lo, hi, j0 + 16 * w) | range_bits(0, min(s.sinks, hi), j0 + 16 * w));
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                r[w][e] = (see >> e & 1u) != 0 ? r[w][e] : 0xff800000u;
-                            }
+                        for (int e = 0; e < 16; ++e) {
+                            r[w][e] = (see >> e & 1u) != 0 ? r[w][e] : 0xff800000u;
                         }
                     }
                 }
-                float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int w = 0; w < C::CHUNKS; ++w) {
-                    if (16 * w < keys) {
+                for (int w = 0; w < CHUNKS; ++w) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            m0 = fmaxf(m0, __uint_as_float(r[w][e]));
-                            m1 = fmaxf(m1, __uint_as_float(r[w][e + 1]));
-                            m2 = fmaxf(m2, __uint_as_float(r[w][e + 2]));
-                            m3 = fmaxf(m3, __uint_as_float(r[w][e + 3]));
-                        }
+                    for (int e = 0; e < 16; e += 2) {
+                        m[e / 2 % 4] = max3_nan(m[e / 2 % 4], __uint_as_float(r[w][e]), __uint_as_float(r[w][e + 1]));
                     }
                 }
-                const float here = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-                raise = (here - top) * c > kRaiseBy;   // the first visible key: infinity > 8
+                const float here = max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
+                if (!(here < INFINITY)) {
+                    total = NAN;   // an infinite score or a NaN: the row is computed again
+                }
+                const bool raise = (here - top) * c > kRaiseBy;   // the first visible key: infinity > 8
+                float shrink = 1.f;
                 if (raise) {
                     shrink = fast_exp2((top - here) * c);
                     top = here;
@@ -846,33 +890,24 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 const float2 c2 = splat2(c), nt2 = splat2(top == -INFINITY ? 0.f : -top * c);
                 float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < C::CHUNKS; ++w) {
-                    if (16 * w < keys) {
+                for (int w = 0; w < CHUNKS; ++w) {
+                    uint32_t p[8];
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            float2 a = fma2(make_float2(__uint_as_float(r[w][e]), __uint_as_float(r[w][e + 1])), c2, nt2);
-                            float2 z = fma2(make_float2(__uint_as_float(r[w][e + 2]), __uint_as_float(r[w][e + 3])), c2, nt2);
-                            a = make_float2(fast_exp2(a.x), fast_exp2(a.y));
-                            z = make_float2(fast_exp2(z.x), fast_exp2(z.y));
-                            sum0 = add2(sum0, a);
-                            sum1 = add2(sum1, z);
-                            const __half2 pa = __float22half2_rn(a), pz = __float22half2_rn(z);
-                            r[w][e / 2] = *reinterpret_cast<const uint32_t *>(&pa);
-                            r[w][e / 2 + 1] = *reinterpret_cast<const uint32_t *>(&pz);
-                        }
+                    for (int e = 0; e < 16; e += 4) {
+                        float2 a = fma2(make_float2(__uint_as_float(r[w][e]), __uint_as_float(r[w][e + 1])), c2, nt2);
+                        float2 z = fma2(make_float2(__uint_as_float(r[w][e + 2]), __uint_as_float(r[w][e + 3])), c2, nt2);
+                        a = make_float2(fast_exp2(a.x), fast_exp2(a.y));
+                        z = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+                        sum0 = add2(sum0, a);
+                        sum1 = add2(sum1, z);
+                        const __half2 pa = __float22half2_rn(a), pz = __float22half2_rn(z);
+                        p[e / 2] = *reinterpret_cast<const uint32_t *>(&pa);
+                        p[e / 2 + 1] = *reinterpret_cast<const uint32_t *>(&pz);
                     }
+                    tmem_store8(t_p + 8 * w, p);
                 }
                 sum0 = add2(sum0, sum1);
                 total = fmaf(total, shrink, sum0.x + sum0.y);
-            }
-            if (step > 0) {   // the product of the step before has read its weights and added to O
-                ok = wait_together(&s_ofull[t], (step - 1) & 1);
-                if (!ok) {
-                    break;
-                }
-                tmem_fence_after();
-            }
-            if (takes_part) {
                 if (!first && __any_sync(0xffffffffu, raise)) {
                     const float2 sh2 = splat2(shrink);
                     for (int x = 0; x < s.dim; x += 16) {
@@ -889,72 +924,98 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     }
                 }
                 first = false;
-#pragma unroll
-                for (int w = 0; w < C::CHUNKS; ++w) {
-                    if (16 * w < keys) {
-                        tmem_store8(t_p + 8 * w, r[w]);
+                tmem_wait_stores();
+            };
+            for (; ok; ++step) {
+                ok = wait_together(&s_sfull[t], step & 1);
+                tmem_fence_after();
+                const WindowStep *d = &s_steps[step % kStepSlots];
+                const int columns = d->columns;
+                const uint32_t flags = d->flags >> t;
+                if (ok && (flags & 1u) != 0) {
+                    if (columns == C::KEYS) {
+                        softmax_step(std::integral_constant<int, C::CHUNKS>(), d, flags);
+                    } else {
+                        softmax_step(std::integral_constant<int, 1>(), d, flags);
+                    }
+                } else {
+                    if (step > 0) {
+                        ok = ok && wait_together(&s_ofull[t], (step - 1) & 1);
+                        tmem_fence_after();
+                    }
+                    if (!ok || columns == 0) {
+                        break;
+                    }
+                    if (lane == 0) {
+                        mbar_arrive(&s_sfree[t]);
                     }
                 }
-                tmem_wait_stores();
-            }
-            tmem_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&s_pfull[t]);
-            }
-        }
-        if (ok && step > 0) {
-            ok = wait_together(&s_ofull[t], (step - 1) & 1);
-            tmem_fence_after();
-        }
-        // ---- context rows
-        const float inv = !ok ? NAN : (total == 0.f ? 0.f : 1.f / total);
-        bool finite = true;
-        __half *out = context + ((int64_t) b * s.seq + i) * s.context_stride + (int64_t) h * s.dim;
-        const bool vec = (reinterpret_cast<uintptr_t>(context) & 15) == 0 && s.context_stride % 8 == 0;
-        for (int x = 0; x < s.dim; x += 32) {
-            uint32_t o[32];
-            if (first) {   // no step took part
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    o[e] = 0;
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0 && ok) {
+                    mbar_arrive(&s_pfull[t]);
                 }
-            } else {
-                tmem_load32(t_o + x, o);
-                tmem_wait_loads();
             }
-            uint32_t w[16];
+            // ---- context rows (the last completion waited for covers every product into O)
+            const float inv = !ok ? NAN : (total == 0.f ? 0.f : 1.f / total);
+            float most = 0.f;
+            __half *out = context + ((int64_t) work.b * s.seq + i) * s.context_stride + (int64_t) h * s.dim;
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                const float a = __uint_as_float(o[e]) * inv, z = __uint_as_float(o[e + 1]) * inv;
-                if (x + e < s.dim) {   // columns past the dimension hold leftovers of another block
-                    finite = finite && fabsf(a) <= 65504.f && fabsf(z) <= 65504.f;
-                }
-                const __half2 hv = __floats2half2_rn(a, z);
-                w[e / 2] = *reinterpret_cast<const uint32_t *>(&hv);
-            }
-            if (i < s.seq) {
+            for (int x = 0; x < DP; x += 32) {
+                if (x < s.dim) {
+                    uint32_t o[32];
+                    if (first) {   // no step took part
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (x + 8 * e < s.dim) {
-                        if (vec) {
-                            *reinterpret_cast<uint4 *>(out + x + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-                        } else {
-                            const __half *hw = reinterpret_cast<const __half *>(&w[4 * e]);
+                        for (int e = 0; e < 32; ++e) {
+                            o[e] = 0;
+                        }
+                    } else {
+                        tmem_load32(t_o + x, o);
+                        tmem_wait_loads();
+                    }
+                    if (x + 32 >= s.dim && ok) {   // O and the scores' place are free for the next item
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&s_sfree[t]);
+                            mbar_arrive(&s_pfull[t]);
+                        }
+                    }
+                    uint32_t w[16];
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) {
-                                out[x + 8 * e + u] = hw[u];
+                    for (int e = 0; e < 32; e += 2) {
+                        const float a = __uint_as_float(o[e]) * inv, z = __uint_as_float(o[e + 1]) * inv;
+                        if (x + e < s.dim) {   // columns past the dimension hold leftovers of another block
+                            most = max3_nan(most, fabsf(a), fabsf(z));
+                        }
+                        const __half2 hv = __floats2half2_rn(a, z);
+                        w[e / 2] = *reinterpret_cast<const uint32_t *>(&hv);
+                    }
+                    if (i < s.seq) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (x + 8 * e < s.dim) {
+                                if (vec) {
+                                    *reinterpret_cast<uint4 *>(out + x + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+                                } else {
+                                    const __half *hw = reinterpret_cast<const __half *>(&w[4 * e]);
+#pragma unroll
+                                    for (int u = 0; u < 8; ++u) {
+                                        out[x + 8 * e + u] = hw[u];
+                                    }
+                                }
                             }
                         }
                     }
                 }
             }
-        }
-        unsigned bad = __ballot_sync(0xffffffffu, ok && i < s.seq && !finite);
-        while (bad != 0) {
-            const int from = __ffs(bad) - 1;
-            bad &= bad - 1;
-            window_row_again(q, k, v, mask, context, &s, s_row[warp], b, i - lane + from, h);
+            unsigned bad = __ballot_sync(0xffffffffu, ok && i < s.seq && !(most <= 65504.f));
+            while (bad != 0) {
+                const int from = __ffs(bad) - 1;
+                bad &= bad - 1;
+                window_row_again(q, k, v, mask, context, &s, s_row[warp], work.b, i - lane + from, h);
+            }
+            ++step;
         }
     }
     tmem_fence_before();
@@ -995,6 +1056,21 @@ inline bool window_map(CUtensorMap *map, const __half *p, int dim, int seq, int 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+inline int sm_count(int dev) {
+    static std::atomic<int> known[kMaxDevices];
+    int n = dev < kMaxDevices ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+            (void) cudaGetLastError();
+            n = 148;
+        }
+        if (dev < kMaxDevices) {
+            known[dev].store(n, std::memory_order_relaxed);
+        }
+    }
+    return n;
+}
+
 template <int DP, int NQ>
 int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, const __half *q, const __half *k, const __half *v,
                      const int8_t *mask, __half *context, const WindowShape &s, cudaStream_t stream) {
@@ -1015,11 +1091,13 @@ int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
     const int pair = NQ == 2 && (s.heads / s.kv_heads) % 2 == 0 ? 1 : 0;
     const int rows = pair ? kTileRows : NQ * kTileRows;
     const int row_blocks = (s.seq + rows - 1) / rows;
-    const int64_t blocks = (int64_t) row_blocks * s.batch * (pair ? s.heads / 2 : s.heads);
-    if (blocks > 0x7fffffffLL) {
+    const int64_t items = (int64_t) row_blocks * s.batch * (pair ? s.heads / 2 : s.heads);
+    if (items > 0x7fffffffLL - (1 << 20)) {
         return CUBK_ERR_UNSUPPORTED;
     }
-    window_tc_kernel<DP, NQ><<<(unsigned) blocks, C::THREADS, C::SMEM_BYTES, stream>>>(qm, km, vm, q, k, v, mask, context, s, row_blocks, pair);
+    const int resident = sm_count(dev) * (NQ == 1 ? 2 : 1);
+    window_tc_kernel<DP, NQ><<<(unsigned) (items < resident ? items : resident), C::THREADS, C::SMEM_BYTES, stream>>>(
+        qm, km, vm, q, k, v, mask, context, s, (int) items, row_blocks, pair);
     return check_launch();
 }
 
