@@ -404,7 +404,6 @@ constexpr int kTileRows = 128;
 constexpr int kHalfTileBytes = kTileRows * 128;    // 128 rows x 64 binary16
 constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 2
 constexpr float kRaiseBy = 8.f;                    // log2 of the largest weight
-constexpr int kMaskSteps = 48;                     // steps whose mask bits are gathered ahead
 
 struct WindowStep {
     int j0, columns;         // columns: KEYS, 16 where no more keys are left, 0 at the end of an item
@@ -583,7 +582,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     __shared__ uint32_t s_tmem;
     __shared__ WindowStep s_steps[kStepSlots];
     __shared__ float s_row[C::SOFTMAX_WARPS][kWindowMaxDim];
-    __shared__ uint32_t s_bits[kMaskSteps][4];
+    __shared__ uint32_t s_bits[32][4];   // kept keys of 32 candidate steps
     unsigned char *tiles = tc_raw + ((1024u - (smem_addr(tc_raw) & 1023u)) & 1023u);
     unsigned char *s_qt = tiles, *s_kt = tiles + C::QUERIES * NQ * C::TILE_BYTES, *s_vt = s_kt + C::STAGES * C::KV_BYTES;
     const int warp = __shfl_sync(0xffffffffu, (int) threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -650,96 +649,98 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     }
                 }
             }
-            const bool gathered = kept != nullptr && steps <= kMaskSteps;
-            if (gathered) {   // the item's mask bits, eight loads in flight
-                for (int w0 = 0; w0 < steps * 4; w0 += 8) {
-                    int8_t byte[8];
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const int at = (w0 + u) / 4, in_step = 32 * ((w0 + u) & 3) + lane;
-                        const int j = (at < sink_steps ? 0 : lo - sink_steps * C::KEYS) + at * C::KEYS + in_step;
-                        byte[u] = at < steps && in_step < C::KEYS && j < (at < sink_steps ? sinks_end : hi) ? kept[j] : (int8_t) 0;
-                    }
+            // 32 candidates at a time, one per lane; then those that hold a kept key, and the item's end, one after another.
+            for (int base = 0; base <= steps && ok; base += 32) {
+                if (kept != nullptr) {   // mask bits, 16 loads in flight
+                    const int words = 4 * min(32, steps - base);
                     __syncwarp();
+                    for (int w0 = 0; w0 < words; w0 += 16) {
+                        int8_t byte[16];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const uint32_t bits = __ballot_sync(0xffffffffu, byte[u] != 0);
-                        if (lane == 0 && w0 + u < steps * 4) {
-                            (&s_bits[0][0])[w0 + u] = bits;
+                        for (int u = 0; u < 16; ++u) {
+                            const int at = base + (w0 + u) / 4, in_step = 32 * (u & 3) + lane;
+                            const int j = (at < sink_steps ? 0 : lo - sink_steps * C::KEYS) + at * C::KEYS + in_step;
+                            byte[u] = at < steps && in_step < C::KEYS && j < (at < sink_steps ? sinks_end : hi) ? kept[j] : (int8_t) 0;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const uint32_t bits = __ballot_sync(0xffffffffu, byte[u] != 0);
+                            if (lane == u && w0 + u < words) {
+                                (&s_bits[0][0])[w0 + u] = bits;
+                            }
                         }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
-            }
-            for (int at = 0; at <= steps && ok; ++at) {
+                const int at = base + lane;
                 const bool in_sinks = at < sink_steps;
+                const int keys = at < steps ? min((in_sinks ? sinks_end : hi) - (in_sinks ? at : at - sink_steps) * C::KEYS - (in_sinks ? 0 : lo), C::KEYS) : 0;
                 WindowStep d;
                 d.j0 = in_sinks ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS;
-                const int keys = at < steps ? min((in_sinks ? sinks_end : hi) - d.j0, C::KEYS) : 0;
                 d.columns = keys == 0 ? 0 : keys <= 16 ? 16 : C::KEYS;
                 d.flags = 0;
                 int count = 0;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    if (gathered) {
-                        d.kept[u] = at < steps ? s_bits[at][u] : 0;
-                    } else {
-                        const bool in = 32 * u + lane < keys;
-                        d.kept[u] = __ballot_sync(0xffffffffu, in && (kept == nullptr || kept[d.j0 + 32 * u + lane] != 0));
-                    }
+                    d.kept[u] = keys == 0 ? 0 : kept != nullptr ? s_bits[lane][u] : range_bits(0, keys, 32 * u);
                     count += __popc(d.kept[u]);
                 }
-                if (keys > 0) {
-                    if (count == 0) {
-                        continue;
-                    }
 #pragma unroll
-                    for (int t = 0; t < NQ; ++t) {
-                        const int first = w.tile_row[t], last = min(first + kTileRows, s.seq) - 1;
-                        const int t_lo = first > s.before ? first - s.before : 0;
-                        const int t_hi = s.after < s.seq - 1 - last ? last + s.after + 1 : s.seq;
-                        if (first < s.seq && d.j0 < t_hi && (d.j0 + keys > t_lo || d.j0 < s.sinks)) {
-                            d.flags |= 1u << t;
-                        }
-                        const bool whole = count == d.columns && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
-                                           (last - s.before <= d.j0 || d.j0 + keys <= s.sinks);
-                        if (!whole) {
-                            d.flags |= 16u << t;
-                        }
+                for (int t = 0; t < NQ; ++t) {
+                    const int first = w.tile_row[t], last = min(first + kTileRows, s.seq) - 1;
+                    const int t_lo = first > s.before ? first - s.before : 0;
+                    const int t_hi = s.after < s.seq - 1 - last ? last + s.after + 1 : s.seq;
+                    if (count > 0 && first < s.seq && d.j0 < t_hi && (d.j0 + keys > t_lo || d.j0 < s.sinks)) {
+                        d.flags |= 1u << t;
+                    }
+                    const bool whole = count == d.columns && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
+                                       (last - s.before <= d.j0 || d.j0 + keys <= s.sinks);
+                    if (!whole) {
+                        d.flags |= 16u << t;
                     }
                 }
-                const int st = step % C::STAGES;
-                const uint32_t before = (step / C::STAGES - 1) & 1;
-                if (step >= C::STAGES) {
-                    ok = wait_together(&s_kempty[st], before);
-                }
-                if (ok && lane == 0) {
-                    s_steps[step % kStepSlots] = d;
-                    if (keys > 0) {
-                        mbar_arrive_expect(&s_kfull[st], C::KV_BYTES);
-                        for (int x = 0; x < C::HALVES; ++x) {
-                            tma_tile(s_kt + st * C::KV_BYTES + x * C::HALF_KV, &k_map, 64 * x, d.j0, w.kh, w.b, &s_kfull[st]);
-                        }
-                    } else {
-                        mbar_arrive(&s_kfull[st]);
+                unsigned todo = __ballot_sync(0xffffffffu, (d.flags & 15u) != 0 || at == steps);
+                while (todo != 0 && ok) {
+                    const int from = __ffs(todo) - 1;
+                    todo &= todo - 1;
+                    const int j0 = __shfl_sync(0xffffffffu, d.j0, from);
+                    const bool end = base + from == steps;
+                    const int st = step % C::STAGES;
+                    const uint32_t before = (step / C::STAGES - 1) & 1;
+                    if (step >= C::STAGES) {
+                        ok = wait_together(&s_kempty[st], before);
                     }
-                }
-                __syncwarp();
-                if (ok && step >= C::STAGES) {
-                    ok = wait_together(&s_vempty[st], before);
-                }
-                if (ok && lane == 0) {
-                    if (keys > 0) {
-                        mbar_arrive_expect(&s_vfull[st], C::KV_BYTES);
-                        for (int x = 0; x < C::HALVES; ++x) {
-                            tma_tile(s_vt + st * C::KV_BYTES + x * C::HALF_KV, &v_map, 64 * x, d.j0, w.kh, w.b, &s_vfull[st]);
-                        }
-                    } else {
-                        mbar_arrive(&s_vfull[st]);
+                    if (lane == from) {
+                        s_steps[step % kStepSlots] = d;
                     }
+                    __syncwarp();
+                    if (ok && lane == 0) {
+                        if (!end) {
+                            mbar_arrive_expect(&s_kfull[st], C::KV_BYTES);
+                            for (int x = 0; x < C::HALVES; ++x) {
+                                tma_tile(s_kt + st * C::KV_BYTES + x * C::HALF_KV, &k_map, 64 * x, j0, w.kh, w.b, &s_kfull[st]);
+                            }
+                        } else {
+                            mbar_arrive(&s_kfull[st]);
+                        }
+                    }
+                    __syncwarp();
+                    if (ok && step >= C::STAGES) {
+                        ok = wait_together(&s_vempty[st], before);
+                    }
+                    if (ok && lane == 0) {
+                        if (!end) {
+                            mbar_arrive_expect(&s_vfull[st], C::KV_BYTES);
+                            for (int x = 0; x < C::HALVES; ++x) {
+                                tma_tile(s_vt + st * C::KV_BYTES + x * C::HALF_KV, &v_map, 64 * x, j0, w.kh, w.b, &s_vfull[st]);
+                            }
+                        } else {
+                            mbar_arrive(&s_vfull[st]);
+                        }
+                    }
+                    __syncwarp();
+                    step += ok ? 1 : 0;
                 }
-                __syncwarp();
-                step += ok ? 1 : 0;
             }
         }
         if (!ok) {   // the copies in flight land before the block's shared memory goes
@@ -836,6 +837,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             const int h = work.tile_head[t], i = work.tile_row[t] + 32 * (warp & 3) + lane;
             const int lo = i > s.before ? i - s.before : 0;
             const int hi = s.after < s.seq - 1 - i ? i + s.after + 1 : s.seq;
+            const int sinks_hi = min(s.sinks, hi);
             float top = -INFINITY, total = 0.f;   // top: of q.k, unscaled
             bool first = true;
             // One step of this row. The number of its 16-column chunks is fixed, so that its loops have no branches and the exponentials of
@@ -860,12 +862,11 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 if ((flags & 16u) != 0) {
                     const int j0 = d->j0;
 #pragma unroll
-                    for (int w = 0; w < CHUNKS; ++w) {
-                        const uint32_t see = (d->kept[w / 2] >> (16 * (w & 1))) &
-                                             (range_bits(lo, hi, j0 + 16 * w) | range_bits(0, min(s.sinks, hi), j0 + 16 * w));
+                    for (int w = 0; w < CHUNKS; w += 2) {   // 32 columns
+                        const uint32_t see = d->kept[w / 2] & (range_bits(lo, hi, j0 + 16 * w) | range_bits(0, sinks_hi, j0 + 16 * w));
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            r[w][e] = (see >> e & 1u) != 0 ? r[w][e] : 0xff800000u;
+                        for (int e = 0; e < (w + 1 < CHUNKS ? 32 : 16); ++e) {
+                            r[w + e / 16][e % 16] = (see >> e & 1u) != 0 ? r[w + e / 16][e % 16] : 0xff800000u;
                         }
                     }
                 }
