@@ -9,6 +9,8 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 
+#include <limits.h>
+
 #include <atomic>
 #include <type_traits>
 
@@ -384,8 +386,10 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 }
 
 // ---------------------------------------------------------------- whole sequences on tcgen05 (binary16)
-// A work item is NQ tiles of 128 query rows: two heads that share their keys, or consecutive rows of one head; blocks are
-// persistent and walk over items, loading and multiplying ahead into the next while the last one's rows are written. Per step of up
+// A work item is NQ tiles of 128 query rows: two heads that share their keys, or consecutive rows of one head. The grid has a block
+// per item; a block that runs takes over items of blocks that have not started yet (cluster launch control), loading and multiplying
+// ahead into the next while the last one's rows are written: no block waits for its first loads but the first on each SM, and masks
+// that make items unequal cost nothing. Per step of up
 // to KEYS keys and per tile: S = Q.K^T (tcgen05.mma, float32 accumulators in tensor memory), softmax by 128 threads that own
 // a row each (tensor-memory lane = query row, so no shuffles), P back into tensor memory as binary16, O += P.V with P as the
 // tensor-memory operand. Warps: 4 NQ for the softmax, NQ that issue the MMAs of a tile, one that chooses the steps and loads K
@@ -399,14 +403,16 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 //     inside binary16, and the sums are float32), so that O is read back and scaled in few steps.
 //   * Weights of unseen keys are exactly 0, but 0 times an infinity or NaN in an unseen V row is NaN: a row that comes out not
 //     finite is computed again by one warp over its visible keys alone.
-// Every wait is bounded; a block that gives up writes NaN, frees its tensor memory and returns.
+// Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, frees its tensor memory and
+// returns.
 constexpr int kTileRows = 128;
 constexpr int kHalfTileBytes = kTileRows * 128;    // 128 rows x 64 binary16
 constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 2
 constexpr float kRaiseBy = 8.f;                    // log2 of the largest weight
 
 struct WindowStep {
-    int j0, columns;         // columns: KEYS, 16 where no more keys are left, 0 at the end of an item
+    int item, j0;
+    int columns;             // KEYS, 16 where no more keys are left, 0 at the end of an item, -1 at the end of all
     uint32_t kept[4];
     uint32_t flags;          // bit t: tile t takes part; bit 4 + t: some row of tile t does not see some key
 };
@@ -535,6 +541,29 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
+// Asks for a block that has not started yet; 16 bytes of answer arrive on the barrier. Not to be asked again after a refusal.
+__device__ __forceinline__ void take_block(void *answer, uint64_t *bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_addr(answer)),
+                 "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// The block that was taken over, or -1.
+__device__ __forceinline__ int taken_block(const void *answer) {
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+        "ld.shared.b128 a, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+        : "=r"(got), "=r"(x)
+        : "r"(smem_addr(answer))
+        : "memory");
+    return got != 0 ? (int) x : -1;
+}
+
 // Bits lo .. hi - 1 of a word that stands for positions base .. base + 31.
 __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int base) {
     const int a = min(max(lo - base, 0), 32), b = min(max(hi - base, 0), 32);
@@ -574,11 +603,14 @@ template <int DP, int NQ>
 __global__ void __launch_bounds__(WindowTc<DP, NQ>::THREADS, NQ == 1 ? 2 : 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                  const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context, const __grid_constant__ WindowShape s,
-                 int items, int row_blocks, int pair_heads) {
+                 int row_blocks, int pair_heads) {
     typedef WindowTc<DP, NQ> C;
     extern __shared__ unsigned char tc_raw[];
     __shared__ uint64_t s_qfull[C::QUERIES], s_qempty[C::QUERIES], s_kfull[C::STAGES], s_kempty[C::STAGES], s_vfull[C::STAGES], s_vempty[C::STAGES];
     __shared__ uint64_t s_sfull[NQ], s_sfree[NQ], s_pfull[NQ], s_ofull[NQ];   // scores written, scores read, weights written, O added to
+    __shared__ __align__(16) uint4 s_taken[2];
+    __shared__ uint64_t s_takes;
+    __shared__ int s_items[4], s_turns, s_first_bad;   // items begun, the latest four; the first that a give-up left without rows
     __shared__ uint32_t s_tmem;
     __shared__ WindowStep s_steps[kStepSlots];
     __shared__ float s_row[C::SOFTMAX_WARPS][kWindowMaxDim];
@@ -598,6 +630,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (threadIdx.x == 32) {
+        s_turns = 0;
+        s_first_bad = INT_MAX;
+        mbar_init(&s_takes, 1);
         for (int i = 0; i < C::QUERIES; ++i) {
             mbar_init(&s_qfull[i], 1);
             mbar_init(&s_qempty[i], NQ);
@@ -629,8 +664,14 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         // ---- steps and loads
         bool ok = true;
         int step = 0, turn = 0;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++turn) {
+        for (int item = blockIdx.x; item >= 0 && ok; ++turn) {
             const WindowItem<NQ> w(item, s, row_blocks, pair_heads);
+            if (lane == 0) {   // the next item, asked for long before it is needed
+                s_items[turn & 3] = item;
+                s_turns = turn + 1;
+                mbar_arrive_expect(&s_takes, 16);
+                take_block(&s_taken[turn & 1], &s_takes);
+            }
             const int lo = w.row0 > s.before ? w.row0 - s.before : 0;
             const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
             const int sinks_end = min(s.sinks, lo), sink_steps = (sinks_end + C::KEYS - 1) / C::KEYS;
@@ -676,6 +717,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 const bool in_sinks = at < sink_steps;
                 const int keys = at < steps ? min((in_sinks ? sinks_end : hi) - (in_sinks ? at : at - sink_steps) * C::KEYS - (in_sinks ? 0 : lo), C::KEYS) : 0;
                 WindowStep d;
+                d.item = item;
                 d.j0 = in_sinks ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS;
                 d.columns = keys == 0 ? 0 : keys <= 16 ? 16 : C::KEYS;
                 d.flags = 0;
@@ -742,8 +784,27 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     step += ok ? 1 : 0;
                 }
             }
+            ok = ok && wait_together(&s_takes, turn & 1);
+            item = ok ? taken_block(&s_taken[turn & 1]) : -1;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the answer is read before its place is written again
+        }
+        if (ok) {   // the end of all
+            const int st = step % C::STAGES;
+            if (step >= C::STAGES) {
+                ok = wait_together(&s_kempty[st], (step / C::STAGES - 1) & 1);
+            }
+            if (ok && lane == 0) {
+                s_steps[step % kStepSlots].columns = -1;
+                s_steps[step % kStepSlots].flags = 0;
+                mbar_arrive(&s_kfull[st]);
+            }
+            __syncwarp();
         }
         if (!ok) {   // the copies in flight land before the block's shared memory goes
+            if (turn > 0 && wait_together(&s_takes, (turn - 1) & 1) && lane == 0 && taken_block(&s_taken[(turn - 1) & 1]) >= 0) {
+                s_items[turn & 3] = taken_block(&s_taken[(turn - 1) & 1]);   // taken over and not begun
+                s_turns = turn + 1;
+            }
             for (int i = max(turn - C::QUERIES, 0); i <= turn; ++i) {
                 (void) wait_together(&s_qfull[i % C::QUERIES], (i / C::QUERIES) & 1);
             }
@@ -764,61 +825,72 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         bool ok = true, started = false;   // started: O holds something of this item
         int columns_before = 0, step = 0, turn = 0;
         uint32_t flags_before = 0;
-        for (int item = blockIdx.x; item < items && ok; item += gridDim.x, ++turn) {
-            const int qb = turn % C::QUERIES;
-            ok = wait_together(&s_qfull[qb], (turn / C::QUERIES) & 1);
-            const uint64_t qd = q_desc + (uint64_t) (qb * NQ * (C::TILE_BYTES / 16));
-            for (int columns = 1; ok && columns != 0; ++step) {
-                const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES;
-                ok = wait_together(&s_kfull[st], (step / C::STAGES) & 1);
-                columns = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].columns, 0);
-                const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0) >> t;
-                if (step > 0) {
-                    ok = ok && wait_together(&s_sfree[t], (step - 1) & 1);
-                    tmem_fence_after();
-                }
-                if (ok && leader) {
-                    if ((flags & 1u) != 0) {
-                        const uint64_t kd = k_desc + (uint64_t) (st * (C::KV_BYTES / 16));
-                        const uint32_t idesc_s = (1u << 4) | ((uint32_t) (columns / 8) << 17) | ((kTileRows >> 4) << 24);
+        bool new_item = true;
+        uint64_t qd = 0;
+        for (; ok; ++step) {
+            const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES, qb = turn % C::QUERIES;
+            ok = wait_together(&s_kfull[st], (step / C::STAGES) & 1);
+            const int columns = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].columns, 0);
+            const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0) >> t;
+            if (new_item && columns >= 0) {
+                ok = ok && wait_together(&s_qfull[qb], (turn / C::QUERIES) & 1);
+                qd = q_desc + (uint64_t) (qb * NQ * (C::TILE_BYTES / 16));
+                new_item = false;
+            }
+            if (step > 0) {
+                ok = ok && wait_together(&s_sfree[t], (step - 1) & 1);
+                tmem_fence_after();
+            }
+            if (ok && leader) {
+                if ((flags & 1u) != 0) {
+                    const uint64_t kd = k_desc + (uint64_t) (st * (C::KV_BYTES / 16));
+                    const uint32_t idesc_s = (1u << 4) | ((uint32_t) (columns / 8) << 17) | ((kTileRows >> 4) << 24);
 #pragma unroll
-                        for (int kk = 0; kk < DP / 16; ++kk) {
-                            if (kk < (int) ksteps) {
-                                mma_ss(t_s, qd + ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16, kd + ((kk >> 2) * C::HALF_KV + (kk & 3) * 32) / 16,
-                                       idesc_s, kk > 0);
-                            }
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        if (kk < (int) ksteps) {
+                            mma_ss(t_s, qd + ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16, kd + ((kk >> 2) * C::HALF_KV + (kk & 3) * 32) / 16,
+                                   idesc_s, kk > 0);
                         }
                     }
-                    mma_commit(&s_sfull[t]);
-                    mbar_arrive(&s_sfull[t]);
+                }
+                mma_commit(&s_sfull[t]);
+                mbar_arrive(&s_sfull[t]);
+                if (columns >= 0) {
                     mma_commit(&s_kempty[st]);
-                    if (columns == 0) {
-                        mma_commit(&s_qempty[qb]);
-                    }
                 }
-                __syncwarp();
-                if (step > 0) {   // O += P.V of the step before; of one that ended an item, only the wait until O has been read
-                    ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
-                    tmem_fence_after();
-                    const bool takes_part = (flags_before & 1u) != 0;
-                    if (ok && leader) {
-                        if (takes_part) {
-                            const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
+                if (columns == 0) {
+                    mma_commit(&s_qempty[qb]);
+                }
+            }
+            __syncwarp();
+            if (columns < 0) {
+                break;
+            }
+            if (step > 0) {   // O += P.V of the step before; of one that ended an item, only the wait until O has been read
+                ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
+                tmem_fence_after();
+                const bool takes_part = (flags_before & 1u) != 0;
+                if (ok && leader) {
+                    if (takes_part) {
+                        const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
 #pragma unroll
-                            for (int kk = 0; kk < C::KEYS / 16; ++kk) {
-                                if (16 * kk < columns_before) {
-                                    mma_ts(t_o, t_p + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || started);
-                                }
+                        for (int kk = 0; kk < C::KEYS / 16; ++kk) {
+                            if (16 * kk < columns_before) {
+                                mma_ts(t_o, t_p + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || started);
                             }
                         }
-                        mma_commit(&s_ofull[t]);
-                        mma_commit(&s_vempty[st_before]);
                     }
-                    started = columns_before != 0 && (started || takes_part);
-                    __syncwarp();
+                    mma_commit(&s_ofull[t]);
+                    mma_commit(&s_vempty[st_before]);
                 }
-                columns_before = columns;
-                flags_before = flags;
+                started = columns_before != 0 && (started || takes_part);
+                __syncwarp();
+            }
+            columns_before = columns;
+            flags_before = flags;
+            if (columns == 0) {
+                new_item = true;
+                ++turn;
             }
         }
     }
@@ -832,8 +904,17 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const bool vec = (reinterpret_cast<uintptr_t>(context) & 15) == 0 && s.context_stride % 8 == 0;
         bool ok = true;
         int step = 0;
-        for (int item = blockIdx.x; item < items; item += gridDim.x) {
-            const WindowItem<NQ> work(item, s, row_blocks, pair_heads);
+        for (int turn = 0;; ++step, ++turn) {
+            ok = wait_together(&s_sfull[t], step & 1);   // an item's first step says which it is
+            if (!ok) {
+                atomicMin(&s_first_bad, turn);
+                break;
+            }
+            if (s_steps[step % kStepSlots].columns < 0) {
+                break;
+            }
+            const WindowItem<NQ> work(s_steps[step % kStepSlots].item, s, row_blocks, pair_heads);
+            bool waited = true;
             const int h = work.tile_head[t], i = work.tile_row[t] + 32 * (warp & 3) + lane;
             const int lo = i > s.before ? i - s.before : 0;
             const int hi = s.after < s.seq - 1 - i ? i + s.after + 1 : s.seq;
@@ -928,7 +1009,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 tmem_wait_stores();
             };
             for (; ok; ++step) {
-                ok = wait_together(&s_sfull[t], step & 1);
+                ok = waited || wait_together(&s_sfull[t], step & 1);
+                waited = false;
                 tmem_fence_after();
                 const WindowStep *d = &s_steps[step % kStepSlots];
                 const int columns = d->columns;
@@ -958,7 +1040,11 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 }
             }
             // ---- context rows (the last completion waited for covers every product into O)
-            const float inv = !ok ? NAN : (total == 0.f ? 0.f : 1.f / total);
+            if (!ok) {
+                atomicMin(&s_first_bad, turn);
+                break;
+            }
+            const float inv = total == 0.f ? 0.f : 1.f / total;
             float most = 0.f;
             __half *out = context + ((int64_t) work.b * s.seq + i) * s.context_stride + (int64_t) h * s.dim;
 #pragma unroll
@@ -974,7 +1060,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                         tmem_load32(t_o + x, o);
                         tmem_wait_loads();
                     }
-                    if (x + 32 >= s.dim && ok) {   // O and the scores' place are free for the next item
+                    if (x + 32 >= s.dim) {   // O and the scores' place are free for the next item
                         tmem_fence_before();
                         __syncwarp();
                         if (lane == 0) {
@@ -1010,17 +1096,25 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     }
                 }
             }
-            unsigned bad = __ballot_sync(0xffffffffu, ok && i < s.seq && !(most <= 65504.f));
+            unsigned bad = __ballot_sync(0xffffffffu, i < s.seq && !(most <= 65504.f));
             while (bad != 0) {
                 const int from = __ffs(bad) - 1;
                 bad &= bad - 1;
                 window_row_again(q, k, v, mask, context, &s, s_row[warp], work.b, i - lane + from, h);
             }
-            ++step;
         }
     }
     tmem_fence_before();
     __syncthreads();
+    for (int turn = s_first_bad; turn < s_turns; ++turn) {   // after a give-up only
+        const WindowItem<NQ> w(s_items[turn & 3], s, row_blocks, pair_heads);
+        for (int e = threadIdx.x; e < NQ * kTileRows * s.dim; e += C::THREADS) {
+            const int t = e / (kTileRows * s.dim), r = e / s.dim % kTileRows, i = w.tile_row[t] + r;
+            if (i < s.seq) {
+                context[((int64_t) w.b * s.seq + i) * s.context_stride + (int64_t) w.tile_head[t] * s.dim + e % s.dim] = __float2half_rn(NAN);
+            }
+        }
+    }
     if (warp == 0) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t) C::TMEM_COLS) : "memory");
     }
@@ -1057,21 +1151,6 @@ inline bool window_map(CUtensorMap *map, const __half *p, int dim, int seq, int 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-inline int sm_count(int dev) {
-    static std::atomic<int> known[kMaxDevices];
-    int n = dev < kMaxDevices ? known[dev].load(std::memory_order_relaxed) : 0;
-    if (n == 0) {
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
-            (void) cudaGetLastError();
-            n = 148;
-        }
-        if (dev < kMaxDevices) {
-            known[dev].store(n, std::memory_order_relaxed);
-        }
-    }
-    return n;
-}
-
 template <int DP, int NQ>
 int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, const __half *q, const __half *k, const __half *v,
                      const int8_t *mask, __half *context, const WindowShape &s, cudaStream_t stream) {
@@ -1093,12 +1172,10 @@ int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
     const int rows = pair ? kTileRows : NQ * kTileRows;
     const int row_blocks = (s.seq + rows - 1) / rows;
     const int64_t items = (int64_t) row_blocks * s.batch * (pair ? s.heads / 2 : s.heads);
-    if (items > 0x7fffffffLL - (1 << 20)) {
+    if (items > 0x7fffffffLL) {
         return CUBK_ERR_UNSUPPORTED;
     }
-    const int resident = sm_count(dev) * (NQ == 1 ? 2 : 1);
-    window_tc_kernel<DP, NQ><<<(unsigned) (items < resident ? items : resident), C::THREADS, C::SMEM_BYTES, stream>>>(
-        qm, km, vm, q, k, v, mask, context, s, (int) items, row_blocks, pair);
+    window_tc_kernel<DP, NQ><<<(unsigned) items, C::THREADS, C::SMEM_BYTES, stream>>>(qm, km, vm, q, k, v, mask, context, s, row_blocks, pair);
     return check_launch();
 }
 
