@@ -132,7 +132,8 @@ window_rows_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *co
 }
 
 // ---- whole sequences on the float32 pipes (float32 storage; binary16 rows that TMA cannot read)
-// 64 query rows of a head a block, 64 keys a step out of one list: the sinks below the window, then the window. A thread owns 8 rows
+// 64 query rows of a head a block, 64 keys a step out of one list: the kept ones of the sinks below the window, then of the window (so
+// that masked keys, wherever they are, cost neither loads nor multiply-adds). A thread owns 8 rows
 // x 4 keys of the scores and 8 rows x DP / 16 columns of the context; Q and K are transposed on their way into shared memory, so that
 // each step of a reduction is two or three 16-byte reads for 32 or 64 multiply-adds, issued in pairs of rows. The 16 threads of a row
 // are half a warp: maxima and sums need shuffles only. Bound by the multiply-adds.
@@ -162,7 +163,8 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
     constexpr int VC = DP / 64;   // 4-column groups of a thread's context
     extern __shared__ __align__(16) float plain_smem[];
     float *s_q = plain_smem, *s_k = s_q + DP * C::QK, *s_v = s_k + DP * C::QK, *s_p = s_k;   // [column][row], .., [key][column], [key][row]
-    __shared__ int s_kept[kPlainKeys], s_bad[kPlainRows];
+    __shared__ __align__(16) int s_list[kPlainKeys + kPlainThreads];   // kept keys not yet used
+    __shared__ int s_found[kPlainThreads / 32], s_bad[kPlainRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rg = threadIdx.x >> 4, cg = threadIdx.x & 15;   // rows 8 rg .., keys 4 cg .., columns 4 cg + 64 x ..
     const int rb = row_blocks - 1 - (int) (blockIdx.x % row_blocks);
@@ -197,20 +199,33 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
             o[r][c] = make_float2(0.f, 0.f);
         }
     }
-    for (int u0 = 0; u0 < listed; u0 += kPlainKeys) {
-        const int keys = min(kPlainKeys, listed - u0);
-        auto key_of = [&](int u) { return u < sinks_end ? u : lo + u - sinks_end; };
-        bool on = false;
-        if (threadIdx.x < kPlainKeys) {   // before the barrier: whoever still reads s_kept is past the one after the products
-            on = (int) threadIdx.x < keys && (kept == nullptr || kept[key_of(u0 + threadIdx.x)] != 0);
+    int cursor = 0, have = 0;   // candidates looked at, keys in the list
+    for (;;) {
+        while (have < kPlainKeys && cursor < listed) {
+            const int u = cursor + threadIdx.x, j = u < sinks_end ? u : lo + u - sinks_end;
+            const bool on = u < listed && (kept == nullptr || kept[j] != 0);
+            const unsigned found = __ballot_sync(0xffffffffu, on);
+            if (lane == 0) {
+                s_found[warp] = __popc(found);
+            }
+            __syncthreads();
+            int at = have;
+#pragma unroll
+            for (int w = 0; w < kPlainThreads / 32; ++w) {
+                at += w < warp ? s_found[w] : 0;
+                have += s_found[w];
+            }
+            if (on) {
+                s_list[at + __popc(found & ((1u << lane) - 1u))] = j;
+            }
+            cursor += kPlainThreads;
+            __syncthreads();
         }
-        const int any = __syncthreads_count(on);   // and the step before is done with K, V and P
-        if (any == 0) {
-            continue;
+        const int keys = min(have, kPlainKeys);
+        if (keys == 0) {
+            break;
         }
-        if (threadIdx.x < kPlainKeys) {
-            s_kept[threadIdx.x] = on ? key_of(u0 + threadIdx.x) : -1;
-        }
+        __syncthreads();   // the list, also where it needed nothing
         // eight loads of a thread in flight at a time
 #pragma unroll
         for (int half = 0; half < 2 * VC; ++half) {
@@ -221,7 +236,7 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
             for (int u = 0; u < LOADS; ++u) {
                 const int i = threadIdx.x + u * kPlainThreads;
                 const int r = is_v ? i / 16 : i % kPlainKeys, c = 64 * (half % VC) + 4 * (is_v ? i % 16 : i / kPlainKeys);
-                x[u] = r < keys ? four_columns<T>((is_v ? vb : kb) + (int64_t) key_of(u0 + r) * s.kv_stride, c, s.dim, vec)
+                x[u] = r < keys ? four_columns<T>((is_v ? vb : kb) + (int64_t) s_list[r] * s.kv_stride, c, s.dim, vec)
                                 : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
@@ -255,9 +270,9 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
                 }
             }
         }
-        // a key counts for row i when it is kept, at most i + after, and at least i - before or below the sinks
-        const int4 js = *reinterpret_cast<const int4 *>(&s_kept[4 * cg]);
-        const int j4[4] = {js.x, js.y, js.z, js.w};
+        // a key of the list counts for row i when it is at most i + after, and at least i - before or below the sinks
+        const int4 js = *reinterpret_cast<const int4 *>(&s_list[4 * cg]);
+        const int j4[4] = {4 * cg < keys ? js.x : -1, 4 * cg + 1 < keys ? js.y : -1, 4 * cg + 2 < keys ? js.z : -1, 4 * cg + 3 < keys ? js.w : -1};
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             const int i = row0 + 8 * rg + r;
@@ -319,6 +334,15 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
                 }
             }
         }
+        // what the list holds beyond this step moves to its front
+        const int left = have - keys;
+        __syncthreads();   // the list, keys, values and weights of this step have been read
+        const int moved = (int) threadIdx.x < left ? s_list[kPlainKeys + threadIdx.x] : 0;
+        __syncthreads();
+        if ((int) threadIdx.x < left) {
+            s_list[threadIdx.x] = moved;
+        }
+        have = left;
     }
     const float most = sizeof(T) == 4 ? 3.402823466e38f : 65504.f;
 #pragma unroll
@@ -666,11 +690,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         int step = 0, turn = 0;
         for (int item = blockIdx.x; item >= 0 && ok; ++turn) {
             const WindowItem<NQ> w(item, s, row_blocks, pair_heads);
-            if (lane == 0) {   // the next item, asked for long before it is needed
+            if (lane == 0) {
                 s_items[turn & 3] = item;
                 s_turns = turn + 1;
-                mbar_arrive_expect(&s_takes, 16);
-                take_block(&s_taken[turn & 1], &s_takes);
             }
             const int lo = w.row0 > s.before ? w.row0 - s.before : 0;
             const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
@@ -692,22 +714,39 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             }
             // 32 candidates at a time, one per lane; then those that hold a kept key, and the item's end, one after another.
             for (int base = 0; base <= steps && ok; base += 32) {
-                if (kept != nullptr) {   // mask bits, 16 loads in flight
-                    const int words = 4 * min(32, steps - base);
+                if (kept != nullptr) {   // four keys a lane, eight steps in flight
+                    const int candidates = min(32, steps - base);
                     __syncwarp();
-                    for (int w0 = 0; w0 < words; w0 += 16) {
-                        int8_t byte[16];
+                    for (int c0 = 0; c0 < candidates; c0 += 8) {
+                        uint32_t four[8];
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) {
-                            const int at = base + (w0 + u) / 4, in_step = 32 * (u & 3) + lane;
-                            const int j = (at < sink_steps ? 0 : lo - sink_steps * C::KEYS) + at * C::KEYS + in_step;
-                            byte[u] = at < steps && in_step < C::KEYS && j < (at < sink_steps ? sinks_end : hi) ? kept[j] : (int8_t) 0;
+                        for (int u = 0; u < 8; ++u) {
+                            const int at = base + c0 + u;
+                            const int j = (at < sink_steps ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS) + 4 * lane;
+                            const int left = c0 + u < candidates && 4 * lane < C::KEYS ? (at < sink_steps ? sinks_end : hi) - j : 0;
+                            const int8_t *from = kept + j;
+                            four[u] = 0;
+                            if (left >= 4 && (reinterpret_cast<uintptr_t>(from) & 3) == 0) {
+                                four[u] = *reinterpret_cast<const uint32_t *>(from);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    four[u] |= e < left ? (uint32_t) (uint8_t) from[e] << (8 * e) : 0u;
+                                }
+                            }
                         }
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) {
-                            const uint32_t bits = __ballot_sync(0xffffffffu, byte[u] != 0);
-                            if (lane == u && w0 + u < words) {
-                                (&s_bits[0][0])[w0 + u] = bits;
+                        for (int u = 0; u < 8; ++u) {
+                            // any bit of a byte -> its lowest; the four lowest bits side by side; eight lanes' to a word
+                            uint32_t v = four[u] | four[u] >> 4;
+                            v |= v >> 2;
+                            v |= v >> 1;
+                            v = ((v & 0x01010101u) * 0x01020408u >> 24 & 15u) << (4 * (lane & 7));
+                            v |= __shfl_xor_sync(0xffffffffu, v, 1);
+                            v |= __shfl_xor_sync(0xffffffffu, v, 2);
+                            v |= __shfl_xor_sync(0xffffffffu, v, 4);
+                            if ((lane & 7) == 0 && c0 + u < candidates) {
+                                s_bits[c0 + u][lane >> 3] = v;
                             }
                         }
                     }
@@ -747,6 +786,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     todo &= todo - 1;
                     const int j0 = __shfl_sync(0xffffffffu, d.j0, from);
                     const bool end = base + from == steps;
+                    if (end && lane == 0) {   // the next item: not earlier, so that blocks finish together
+                        mbar_arrive_expect(&s_takes, 16);
+                        take_block(&s_taken[turn & 1], &s_takes);
+                    }
                     const int st = step % C::STAGES;
                     const uint32_t before = (step / C::STAGES - 1) & 1;
                     if (step >= C::STAGES) {
@@ -1047,50 +1090,46 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             const float inv = total == 0.f ? 0.f : 1.f / total;
             float most = 0.f;
             __half *out = context + ((int64_t) work.b * s.seq + i) * s.context_stride + (int64_t) h * s.dim;
+            uint32_t o[DP / 16][16];
 #pragma unroll
-            for (int x = 0; x < DP; x += 32) {
-                if (x < s.dim) {
-                    uint32_t o[32];
-                    if (first) {   // no step took part
+            for (int x = 0; x < DP / 16; ++x) {
+                if (!first && 16 * x < s.dim) {
+                    tmem_load16(t_o + 16 * x, o[x]);
+                } else {   // no step took part
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            o[e] = 0;
-                        }
-                    } else {
-                        tmem_load32(t_o + x, o);
-                        tmem_wait_loads();
+                    for (int e = 0; e < 16; ++e) {
+                        o[x][e] = 0;
                     }
-                    if (x + 32 >= s.dim) {   // O and the scores' place are free for the next item
-                        tmem_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            mbar_arrive(&s_sfree[t]);
-                            mbar_arrive(&s_pfull[t]);
-                        }
-                    }
-                    uint32_t w[16];
+                }
+            }
+            tmem_wait_loads();
+            tmem_fence_before();
+            __syncwarp();
+            if (lane == 0) {   // O and the scores' place are free for the next item
+                mbar_arrive(&s_sfree[t]);
+                mbar_arrive(&s_pfull[t]);
+            }
+            const float2 inv2 = splat2(inv);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float a = __uint_as_float(o[e]) * inv, z = __uint_as_float(o[e + 1]) * inv;
-                        if (x + e < s.dim) {   // columns past the dimension hold leftovers of another block
-                            most = max3_nan(most, fabsf(a), fabsf(z));
-                        }
-                        const __half2 hv = __floats2half2_rn(a, z);
-                        w[e / 2] = *reinterpret_cast<const uint32_t *>(&hv);
+            for (int x = 0; x < DP / 8; ++x) {
+                if (8 * x < s.dim) {   // past the dimension V is zeros up to a whole 16 columns, and O too
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int at = 8 * (x & 1) + 2 * e;
+                        const float2 a = mul2(make_float2(__uint_as_float(o[x / 2][at]), __uint_as_float(o[x / 2][at + 1])), inv2);
+                        most = max3_nan(most, fabsf(a.x), fabsf(a.y));
+                        const __half2 hv = __float22half2_rn(a);
+                        w[e] = *reinterpret_cast<const uint32_t *>(&hv);
                     }
                     if (i < s.seq) {
+                        if (vec) {
+                            *reinterpret_cast<uint4 *>(out + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
+                        } else {
+                            const __half *hw = reinterpret_cast<const __half *>(w);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (x + 8 * e < s.dim) {
-                                if (vec) {
-                                    *reinterpret_cast<uint4 *>(out + x + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-                                } else {
-                                    const __half *hw = reinterpret_cast<const __half *>(&w[4 * e]);
-#pragma unroll
-                                    for (int u = 0; u < 8; ++u) {
-                                        out[x + 8 * e + u] = hw[u];
-                                    }
-                                }
+                            for (int u = 0; u < 8; ++u) {
+                                out[8 * x + u] = hw[u];
                             }
                         }
                     }
