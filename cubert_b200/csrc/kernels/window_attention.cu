@@ -179,10 +179,20 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
     const int hi = s.after < s.seq - 1 - last_row ? last_row + s.after + 1 : s.seq;
     const int sinks_end = min(s.sinks, lo), listed = sinks_end + hi - lo;
 
-    for (int i = threadIdx.x; i < kPlainRows * (DP / 4); i += kPlainThreads) {
-        const int r = i % kPlainRows, c = 4 * (i / kPlainRows);
-        const float4 x = row0 + r < s.seq ? four_columns<T>(qb + (int64_t) (row0 + r) * s.q_stride, c, s.dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-        s_q[c * C::QK + r] = x.x, s_q[(c + 1) * C::QK + r] = x.y, s_q[(c + 2) * C::QK + r] = x.z, s_q[(c + 3) * C::QK + r] = x.w;
+#pragma unroll
+    for (int part = 0; part < VC; ++part) {   // eight loads of a thread in flight
+        constexpr int LOADS = kPlainRows * 16 / kPlainThreads;
+        float4 x[LOADS];
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int i = threadIdx.x + u * kPlainThreads, r = i % kPlainRows, c = 64 * part + 4 * (i / kPlainRows);
+            x[u] = row0 + r < s.seq ? four_columns<T>(qb + (int64_t) (row0 + r) * s.q_stride, c, s.dim, vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int i = threadIdx.x + u * kPlainThreads, r = i % kPlainRows, c = 64 * part + 4 * (i / kPlainRows);
+            s_q[c * C::QK + r] = x[u].x, s_q[(c + 1) * C::QK + r] = x[u].y, s_q[(c + 2) * C::QK + r] = x[u].z, s_q[(c + 3) * C::QK + r] = x[u].w;
+        }
     }
     const float c2 = s.scale * kLog2e;
     float top[8], total[8];
@@ -1316,44 +1326,95 @@ window_step_rows_kernel(const T *q, const T *k, const T *v, const int32_t *posit
 // what it took; at the end the blocks read one another's partial sums through distributed shared memory and every block
 // writes its share of the context. Nothing is staged in device memory, so calls need no workspace and no order among them,
 // and the sums are added in the same order every time. The kernel is bound by the cache's bytes.
-constexpr int kStepWarps = 4;
-
-template <int HEADS, int DP>
+template <int WARPS, int HEADS, int DP>
 struct StepPartial {
-    float o[kStepWarps][HEADS][DP + 2];   // two columns of padding spread the rows over the banks
-    float2 stat[kStepWarps][HEADS];       // maximum (log2 domain) and sum
+    float o[WARPS][HEADS][DP + 2];   // two columns of padding spread the rows over the banks
+    float2 stat[WARPS][HEADS];       // maximum (log2 domain) and sum
 };
 
-template <typename T, int HEADS, int DP>
-__device__ __forceinline__ void step_join(StepPartial<HEADS, DP> *part, int heads_here, int dim, T *out) {
+constexpr int kStepBlocks = 8;   // of a cluster at most
+
+// Parts (maximum, sum, weighted sum of values) joined into one; a part without keys has the sum 0 and counts for nothing.
+template <int N>
+__device__ __forceinline__ float3 join_parts(const float2 (&stat)[N], const float (&o)[N]) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        top = fmaxf(top, stat[i].x);
+    }
+    float sum = 0.f, total = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float weight = stat[i].x == -INFINITY ? 0.f : fast_exp2(stat[i].x - top);
+        if (stat[i].y != 0.f) {
+            total = fmaf(weight, stat[i].y, total);
+            sum = fmaf(weight, o[i], sum);
+        }
+    }
+    return make_float3(top, total, sum);
+}
+
+// First the warps of a block, in its own shared memory, then the blocks: each output element's parts are loaded together.
+template <typename T, int WARPS, int HEADS, int DP>
+__device__ __forceinline__ void step_join(StepPartial<WARPS, HEADS, DP> *part, int heads_here, int dim, T *out) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
+    constexpr int PER_THREAD = (HEADS * DP + 32 * WARPS - 1) / (32 * WARPS);
+    float3 joined[PER_THREAD];
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < PER_THREAD; ++u) {
+        const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
+        if (h < heads_here) {
+            float2 stat[WARPS];
+            float o[WARPS];
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                stat[w] = part->stat[w][h];
+                o[w] = part->o[w][h][x];
+            }
+            joined[u] = join_parts<WARPS>(stat, o);
+        }
+    }
+    if (blocks == 1) {
+#pragma unroll
+        for (int u = 0; u < PER_THREAD; ++u) {
+            const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
+            if (h < heads_here && x < dim) {
+                out[h * dim + x] = from_float<T>(joined[u].y == 0.f ? 0.f : joined[u].z / joined[u].y);
+            }
+        }
+        return;
+    }
+    __syncthreads();   // every warp's part has been read: the first one's place takes the block's
+#pragma unroll
+    for (int u = 0; u < PER_THREAD; ++u) {
+        const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
+        if (h < heads_here) {
+            part->o[0][h][x] = joined[u].z;
+            if (x == 0) {
+                part->stat[0][h] = make_float2(joined[u].x, joined[u].y);
+            }
+        }
+    }
     cluster.sync();
-    const int blocks = (int) cluster.num_blocks();
-    for (int e = (int) cluster.block_rank() * (32 * kStepWarps) + threadIdx.x; e < heads_here * dim; e += blocks * 32 * kStepWarps) {
+    for (int e = rank * (32 * WARPS) + threadIdx.x; e < heads_here * dim; e += blocks * 32 * WARPS) {
         const int h = e / dim, x = e - h * dim;
-        float top = -INFINITY;
-        for (int r = 0; r < blocks; ++r) {
-            const StepPartial<HEADS, DP> *from = cluster.map_shared_rank(part, r);
+        float2 stat[kStepBlocks];
+        float o[kStepBlocks];
 #pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) {
-                top = fmaxf(top, from->stat[w][h].x);
+        for (int r = 0; r < kStepBlocks; ++r) {
+            stat[r] = make_float2(-INFINITY, 0.f);
+            o[r] = 0.f;
+            if (r < blocks) {
+                const StepPartial<WARPS, HEADS, DP> *from = cluster.map_shared_rank(part, r);
+                stat[r] = from->stat[0][h];
+                o[r] = from->o[0][h][x];
             }
         }
-        float sum = 0.f, total = 0.f;
-        for (int r = 0; r < blocks; ++r) {
-            const StepPartial<HEADS, DP> *from = cluster.map_shared_rank(part, r);
-#pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) {
-                const float2 st = from->stat[w][h];
-                const float weight = st.x == -INFINITY ? 0.f : fast_exp2(st.x - top);
-                if (st.y != 0.f) {   // a warp without keys left nothing
-                    total = fmaf(weight, st.y, total);
-                    sum = fmaf(weight, from->o[w][h][x], sum);
-                }
-            }
-        }
-        out[e] = from_float<T>(total == 0.f ? 0.f : sum / total);
+        const float3 all = join_parts<kStepBlocks>(stat, o);
+        out[e] = from_float<T>(all.y == 0.f ? 0.f : all.z / all.y);
     }
     cluster.sync();   // nobody leaves while its sums are read
 }
@@ -1363,7 +1424,7 @@ struct StepPlace {
     int worker, workers;   // this warp among the cluster's
 };
 
-template <int HEADS>
+template <int WARPS, int HEADS>
 __device__ __forceinline__ bool step_place(const int32_t *positions, const RingShape &s, int chunks, StepPlace &at) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -1383,17 +1444,17 @@ __device__ __forceinline__ bool step_place(const int32_t *positions, const RingS
     const int slots = s.window + s.sinks;
     at.slot = ring_slot(p, s.window, s.sinks);
     at.n = p < slots ? p + 1 : slots;
-    at.worker = rank * kStepWarps + (threadIdx.x >> 5);
-    at.workers = blocks * kStepWarps;
+    at.worker = rank * WARPS + (threadIdx.x >> 5);
+    at.workers = blocks * WARPS;
     return true;
 }
 
 // The new token's row into its slot, by the first chunk's first block; the readers of the slot take the token's own row.
-template <typename T>
+template <typename T, int WARPS>
 __device__ __forceinline__ void step_store(const T *kn, const T *vn, T *kc, T *vc, const StepPlace &at, const RingShape &s) {
-    if (at.first_head == at.kh * (s.heads / s.kv_heads) && at.worker < kStepWarps) {
+    if (at.first_head == at.kh * (s.heads / s.kv_heads) && at.worker < WARPS) {
         constexpr int E = 16 / (int) sizeof(T);
-        for (int c = threadIdx.x; c < s.dim / E; c += 32 * kStepWarps) {
+        for (int c = threadIdx.x; c < s.dim / E; c += 32 * WARPS) {
             reinterpret_cast<uint4 *>(kc + (int64_t) at.slot * s.dim)[c] = reinterpret_cast<const uint4 *>(kn)[c];
             reinterpret_cast<uint4 *>(vc + (int64_t) at.slot * s.dim)[c] = reinterpret_cast<const uint4 *>(vn)[c];
         }
@@ -1417,21 +1478,21 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
 // of the reduction, in an order that Q shares. Of V it reads chunk g (g + 8) of the rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and pairs
 // the halves of two rows: word i of a chunk is rows g and g + 8 of the i-th 16 output columns. So K and V go from memory to
 // operands with no stop in shared memory; P^T turns around in registers.
-template <int DP, int NT>
-__global__ void __launch_bounds__(32 * kStepWarps, DP == 64 ? 4 : (NT == 1 ? 3 : 2))
+template <int WARPS, int DP, int NT>
+__global__ void __launch_bounds__(32 * WARPS, (DP == 64 ? 16 : (NT == 1 ? 12 : 8)) / WARPS)
 window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const int32_t *positions, __half *k_cache, __half *v_cache,
                        __half *context, const __grid_constant__ RingShape s, int chunks) {
     constexpr int HEADS = 8 * NT, KC = DP / 32, VC = DP / 64;
-    __shared__ StepPartial<HEADS, DP> part;
+    __shared__ StepPartial<WARPS, HEADS, DP> part;
     StepPlace at;
-    if (!step_place<HEADS>(positions, s, chunks, at)) {
+    if (!step_place<WARPS, HEADS>(positions, s, chunks, at)) {
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t slots = s.window + s.sinks;
     const __half *kn = k + at.b * s.kv_stride + (int64_t) at.kh * s.dim, *vn = v + at.b * s.kv_stride + (int64_t) at.kh * s.dim;
     __half *kc = k_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim, *vc = v_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim;
-    step_store<__half>(kn, vn, kc, vc, at, s);
+    step_store<__half, WARPS>(kn, vn, kc, vc, at, s);
 
     uint32_t qf[NT][KC][4];
 #pragma unroll
@@ -1592,26 +1653,26 @@ window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const 
             }
         }
     }
-    step_join<__half, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
+    step_join<__half, WARPS, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
 }
 
 // float32: LPK lanes share a key, four columns each, so that a warp reads 32 / LPK whole rows per instruction; every group of
 // lanes keeps a softmax of its own over its keys, HEADS heads at once.
-template <int LPK, int HEADS>
-__global__ void __launch_bounds__(32 * kStepWarps)
+template <int WARPS, int LPK, int HEADS>
+__global__ void __launch_bounds__(32 * WARPS)
 window_step_f32_kernel(const float *q, const float *k, const float *v, const int32_t *positions, float *k_cache, float *v_cache, float *context,
                        const __grid_constant__ RingShape s, int chunks) {
     constexpr int DP = 4 * LPK, GROUPS = 32 / LPK, U = HEADS == 1 ? 8 : 4;   // U: rows per lane group in flight
-    __shared__ StepPartial<HEADS, DP> part;
+    __shared__ StepPartial<WARPS, HEADS, DP> part;
     StepPlace at;
-    if (!step_place<HEADS>(positions, s, chunks, at)) {
+    if (!step_place<WARPS, HEADS>(positions, s, chunks, at)) {
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LPK, col = 4 * (lane % LPK);
     const int64_t slots = s.window + s.sinks;
     const float *kn = k + at.b * s.kv_stride + (int64_t) at.kh * s.dim, *vn = v + at.b * s.kv_stride + (int64_t) at.kh * s.dim;
     float *kc = k_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim, *vc = v_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim;
-    step_store<float>(kn, vn, kc, vc, at, s);
+    step_store<float, WARPS>(kn, vn, kc, vc, at, s);
     const bool mine = col < s.dim;
     const float c2 = s.scale * kLog2e;
     float4 qf[HEADS], o[HEADS];
@@ -1689,30 +1750,33 @@ window_step_f32_kernel(const float *q, const float *k, const float *v, const int
             *reinterpret_cast<float2 *>(&part.o[warp][h][col + 2]) = make_float2(r[3], r[4]);
         }
     }
-    step_join<float, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
+    step_join<float, WARPS, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
 }
 
-// Blocks of a cluster: enough of them to fill the GPU twice, none with less than 64 slots for its four warps.
+// Blocks of a cluster: enough of them to fill the GPU twice, none with less than 64 slots.
 inline int step_cluster(int64_t units, int64_t slots) {
     int blocks = 1;
-    while (blocks < 8 && units * blocks < 2 * 148 && slots > 64 * blocks) {
+    while (blocks < kStepBlocks && units * blocks < 2 * 148 && slots > 64 * blocks) {
         blocks *= 2;
     }
     return blocks;
 }
 
 template <typename T, int HEADS, typename Kernel>
-int step_launch(Kernel kernel, const T *q, const T *k, const T *v, const int32_t *positions, T *k_cache, T *v_cache, T *context,
+int step_launch(Kernel four, Kernel eight, bool has_eight, const T *q, const T *k, const T *v, const int32_t *positions, T *k_cache, T *v_cache, T *context,
                 const RingShape &s, cudaStream_t stream) {
     const int chunks = (s.heads / s.kv_heads + HEADS - 1) / HEADS;
-    const int64_t units = (int64_t) s.batch * s.kv_heads * chunks;
-    const int cluster = step_cluster(units, (int64_t) s.window + s.sinks);
+    const int64_t units = (int64_t) s.batch * s.kv_heads * chunks, slots = (int64_t) s.window + s.sinks;
+    const int cluster = step_cluster(units, slots);
     if (units * cluster > 0x7fffffffLL) {
         return CUBK_ERR_UNSUPPORTED;
     }
+    // Eight warps a block where even full clusters leave SMs with less than two blocks and the slots are many: what a stream's
+    // rows take then is set by the loads an SM has in flight.
+    const bool wide = has_eight && units * cluster < 2 * 148 && slots >= 128 * cluster;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned) (units * cluster));
-    config.blockDim = dim3(32 * kStepWarps);
+    config.blockDim = dim3(wide ? 256 : 128);
     config.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -1720,7 +1784,7 @@ int step_launch(Kernel kernel, const T *q, const T *k, const T *v, const int32_t
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     config.attrs = &attr;
     config.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, q, k, v, positions, k_cache, v_cache, context, s, chunks);
+    const cudaError_t err = cudaLaunchKernelEx(&config, wide ? eight : four, q, k, v, positions, k_cache, v_cache, context, s, chunks);
     if (err != cudaSuccess) {
         (void) cudaGetLastError();
         set_last_error(err);
@@ -1733,21 +1797,27 @@ int step_launch(Kernel kernel, const T *q, const T *k, const T *v, const int32_t
 inline int step_vectors(const __half *q, const __half *k, const __half *v, const int32_t *positions, __half *k_cache, __half *v_cache,
                         __half *context, const RingShape &s, cudaStream_t stream) {
     const int share = s.heads / s.kv_heads;
+    // the parts of eight warps with 16 heads of 128 do not fit a block's static shared memory
+#define STEP_F16(DP, NT)                                                                                                                  \
+    step_launch<__half, 8 * NT>(window_step_f16_kernel<4, DP, NT>, window_step_f16_kernel<DP * NT == 256 ? 4 : 8, DP, NT>, DP * NT < 256, q, \
+                                k, v, positions, k_cache, v_cache, context, s, stream)
     if (s.dim <= 64) {
-        return share <= 8 ? step_launch<__half, 8>(window_step_f16_kernel<64, 1>, q, k, v, positions, k_cache, v_cache, context, s, stream)
-                          : step_launch<__half, 16>(window_step_f16_kernel<64, 2>, q, k, v, positions, k_cache, v_cache, context, s, stream);
+        return share <= 8 ? STEP_F16(64, 1) : STEP_F16(64, 2);
     }
-    return share <= 8 ? step_launch<__half, 8>(window_step_f16_kernel<128, 1>, q, k, v, positions, k_cache, v_cache, context, s, stream)
-                      : step_launch<__half, 16>(window_step_f16_kernel<128, 2>, q, k, v, positions, k_cache, v_cache, context, s, stream);
+    return share <= 8 ? STEP_F16(128, 1) : STEP_F16(128, 2);
+#undef STEP_F16
 }
 
 inline int step_vectors(const float *q, const float *k, const float *v, const int32_t *positions, float *k_cache, float *v_cache, float *context,
                         const RingShape &s, cudaStream_t stream) {
     const int share = s.heads / s.kv_heads;
-#define STEP_F32(LPK)                                                                                                                       \
-    (share == 1 ? step_launch<float, 1>(window_step_f32_kernel<LPK, 1>, q, k, v, positions, k_cache, v_cache, context, s, stream)            \
-                : step_launch<float, 4>(window_step_f32_kernel<LPK, 4>, q, k, v, positions, k_cache, v_cache, context, s, stream))
-    return s.dim <= 32 ? STEP_F32(8) : s.dim <= 64 ? STEP_F32(16) : STEP_F32(32);
+#define STEP_F32(LPK, HEADS)                                                                                                             \
+    step_launch<float, HEADS>(window_step_f32_kernel<4, LPK, HEADS>, window_step_f32_kernel<8, LPK, HEADS>, true, q, k, v, positions,   \
+                              k_cache, v_cache, context, s, stream)
+    if (share == 1) {
+        return s.dim <= 32 ? STEP_F32(8, 1) : s.dim <= 64 ? STEP_F32(16, 1) : STEP_F32(32, 1);
+    }
+    return s.dim <= 32 ? STEP_F32(8, 4) : s.dim <= 64 ? STEP_F32(16, 4) : STEP_F32(32, 4);
 #undef STEP_F32
 }
 
