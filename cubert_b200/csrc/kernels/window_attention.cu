@@ -1753,10 +1753,16 @@ window_step_f32_kernel(const float *q, const float *k, const float *v, const int
     step_join<float, WARPS, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
 }
 
-// Blocks of a cluster: enough of them to fill the GPU twice, none with less than 64 slots.
-inline int step_cluster(int64_t units, int64_t slots) {
+// Blocks of a cluster: doubled until the grid has two blocks per SM, and on to about five while every warp keeps 6 KB of keys (below
+// that a block's start and join cost more than its share of the loads brings: 9 streams of 32 / 8 heads of 128 with 715 slots take 9.8 us
+// in clusters of four, 13.9 in eights; 16 of 12 heads of 64 with 1024 slots 13.1 in twos, 11.0 in fours).
+inline int step_cluster(int64_t units, int64_t slots, int64_t row_bytes) {
     int blocks = 1;
-    while (blocks < kStepBlocks && units * blocks < 2 * 148 && slots > 64 * blocks) {
+    while (blocks < kStepBlocks && slots > 64 * blocks) {
+        const int64_t grid = units * blocks * 2, warp_bytes = slots * row_bytes / (blocks * 2 * 4);
+        if (grid > 2 * 148 && (grid > 5 * 148 + 74 || warp_bytes < 6 * 1024)) {
+            break;
+        }
         blocks *= 2;
     }
     return blocks;
@@ -1767,13 +1773,14 @@ int step_launch(Kernel four, Kernel eight, bool has_eight, const T *q, const T *
                 const RingShape &s, cudaStream_t stream) {
     const int chunks = (s.heads / s.kv_heads + HEADS - 1) / HEADS;
     const int64_t units = (int64_t) s.batch * s.kv_heads * chunks, slots = (int64_t) s.window + s.sinks;
-    const int cluster = step_cluster(units, slots);
+    const int cluster = step_cluster(units, slots, (int64_t) s.dim * (int) sizeof(T));
     if (units * cluster > 0x7fffffffLL) {
         return CUBK_ERR_UNSUPPORTED;
     }
-    // Eight warps a block where even full clusters leave SMs with less than two blocks and the slots are many: what a stream's
-    // rows take then is set by the loads an SM has in flight.
-    const bool wide = has_eight && units * cluster < 2 * 148 && slots >= 128 * cluster;
+    // Eight warps a block where even full clusters leave half of the SMs without one: what a stream takes then is set by the loads an
+    // SM has in flight (one stream of 32 / 8 heads of 128 with 4096 slots: 13.6 us with four warps, 10.6 with eight; with blocks on most
+    // SMs four are the better: 4 streams of 16 / 4 heads, 14.2 against 17.0).
+    const bool wide = has_eight && units * cluster <= 74 && slots >= 128 * cluster;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned) (units * cluster));
     config.blockDim = dim3(wide ? 256 : 128);
