@@ -463,6 +463,10 @@ struct WindowTc {
     // Softmax warps in whole groups of four, and one more group for the others (the last of it idle), which hands most of its
     // registers to them. Launched with 65536 / (THREADS x blocks per SM) each: 128 x 256 >= 192 x 128 + 56 x 128, 168 x 384 >= 224 x 256 + 56 x 128.
     static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
+    // The context's rows leave through the place of the item's queries by TMA, or as 16-byte stores from registers. TMA holds the queries
+    // of the item after the next back until they have left: 8192 tokens, 32 heads of 128: 265 us against 277, but 4 x 4096 tokens, 16
+    // heads of 64, window 513, whose items are short: 88 against 84.
+    static constexpr bool ROWS_BY_TMA = NQ == 2;
     static constexpr int LAUNCH_REGS = NQ == 1 ? 128 : 168, SOFTMAX_REGS = NQ == 1 ? 192 : 224, OTHER_REGS = 56;
     static_assert(LAUNCH_REGS * THREADS >= SOFTMAX_REGS * 32 * SOFTMAX_WARPS + OTHER_REGS * 128, "a group that asks for more would wait forever");
     static constexpr int WEIGHTS = NQ * KEYS, CONTEXT = WEIGHTS + NQ * KEYS / 2;   // columns of tensor memory behind the scores
@@ -598,6 +602,13 @@ __device__ __forceinline__ int taken_block(const void *answer) {
     return got != 0 ? (int) x : -1;
 }
 
+// A warp's 32 rows x 64 columns from a swizzled tile to the context; rows and columns outside the tensor are not written.
+__device__ __forceinline__ void tma_rows(const CUtensorMap *map, const void *src, int column, int row, int head, int batch) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(column),
+                 "r"(row), "r"(head), "r"(batch)
+                 : "memory");
+}
+
 // Bits lo .. hi - 1 of a word that stands for positions base .. base + 31.
 __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int base) {
     const int a = min(max(lo - base, 0), 32), b = min(max(hi - base, 0), 32);
@@ -636,7 +647,7 @@ struct WindowItem {
 template <int DP, int NQ>
 __global__ void __launch_bounds__(WindowTc<DP, NQ>::THREADS, NQ == 1 ? 2 : 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                 const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context, const __grid_constant__ WindowShape s,
+                 const __grid_constant__ CUtensorMap o_map, bool row_vectors, const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context, const __grid_constant__ WindowShape s,
                  int row_blocks, int pair_heads) {
     typedef WindowTc<DP, NQ> C;
     extern __shared__ unsigned char tc_raw[];
@@ -669,7 +680,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         mbar_init(&s_takes, 1);
         for (int i = 0; i < C::QUERIES; ++i) {
             mbar_init(&s_qfull[i], 1);
-            mbar_init(&s_qempty[i], NQ);
+            mbar_init(&s_qempty[i], NQ + (C::ROWS_BY_TMA ? C::SOFTMAX_WARPS : 0));   // its products are done, and it has served the rows
         }
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&s_kfull[i], 1);
@@ -704,7 +715,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 s_items[turn & 3] = item;
                 s_turns = turn + 1;
             }
-            const int lo = w.row0 > s.before ? w.row0 - s.before : 0;
+            const int lo = w.row0 > s.before ? (w.row0 - s.before) & ~3 : 0;   // whole words of the mask
             const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
             const int sinks_end = min(s.sinks, lo), sink_steps = (sinks_end + C::KEYS - 1) / C::KEYS;
             const int steps = sink_steps + (hi - lo + C::KEYS - 1) / C::KEYS;
@@ -726,6 +737,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             for (int base = 0; base <= steps && ok; base += 32) {
                 if (kept != nullptr) {   // four keys a lane, eight steps in flight
                     const int candidates = min(32, steps - base);
+                    const bool words = s.seq % 4 == 0 && (reinterpret_cast<uintptr_t>(mask) & 3) == 0;   // of four keys: none reaches past its row
                     __syncwarp();
                     for (int c0 = 0; c0 < candidates; c0 += 8) {
                         uint32_t four[8];
@@ -734,14 +746,13 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                             const int at = base + c0 + u;
                             const int j = (at < sink_steps ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS) + 4 * lane;
                             const int left = c0 + u < candidates && 4 * lane < C::KEYS ? (at < sink_steps ? sinks_end : hi) - j : 0;
-                            const int8_t *from = kept + j;
                             four[u] = 0;
-                            if (left >= 4 && (reinterpret_cast<uintptr_t>(from) & 3) == 0) {
-                                four[u] = *reinterpret_cast<const uint32_t *>(from);
+                            if (words) {
+                                four[u] = left > 0 ? *reinterpret_cast<const uint32_t *>(kept + j) & (left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u) : 0u;
                             } else {
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    four[u] |= e < left ? (uint32_t) (uint8_t) from[e] << (8 * e) : 0u;
+                                    four[u] |= e < left ? (uint32_t) (uint8_t) kept[j + e] << (8 * e) : 0u;
                                 }
                             }
                         }
@@ -954,7 +965,6 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const uint32_t lanes = (uint32_t) (32 * (warp & 3)) << 16;
         const uint32_t t_s = tmem + t * C::KEYS + lanes, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2) + lanes, t_o = tmem + C::CONTEXT + t * DP + lanes;
         const float c = s.scale * kLog2e;
-        const bool vec = (reinterpret_cast<uintptr_t>(context) & 15) == 0 && s.context_stride % 8 == 0;
         bool ok = true;
         int step = 0;
         for (int turn = 0;; ++step, ++turn) {
@@ -1100,6 +1110,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             const float inv = total == 0.f ? 0.f : 1.f / total;
             float most = 0.f;
             __half *out = context + ((int64_t) work.b * s.seq + i) * s.context_stride + (int64_t) h * s.dim;
+            unsigned char *q_tile = s_qt + ((turn % C::QUERIES) * NQ + t) * C::TILE_BYTES;
             uint32_t o[DP / 16][16];
 #pragma unroll
             for (int x = 0; x < DP / 16; ++x) {
@@ -1132,20 +1143,41 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                         const __half2 hv = __float22half2_rn(a);
                         w[e] = *reinterpret_cast<const uint32_t *>(&hv);
                     }
-                    if (i < s.seq) {
-                        if (vec) {
-                            *reinterpret_cast<uint4 *>(out + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
-                        } else {
-                            const __half *hw = reinterpret_cast<const __half *>(w);
+                    if (C::ROWS_BY_TMA && row_vectors) {   // into the place of this item's queries, which no product reads any more
+                        const int r = 32 * (warp & 3) + lane;
+                        *reinterpret_cast<uint4 *>(q_tile + (x / 8) * kHalfTileBytes + r * 128 + ((x % 8) ^ (r & 7)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else if (i < s.seq && row_vectors) {
+                        *reinterpret_cast<uint4 *>(out + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
+                    } else if (i < s.seq) {
+                        const __half *hw = reinterpret_cast<const __half *>(w);
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) {
-                                out[8 * x + u] = hw[u];
-                            }
+                        for (int u = 0; u < 8; ++u) {
+                            out[8 * x + u] = hw[u];
                         }
                     }
                 }
             }
+            if (C::ROWS_BY_TMA) {
+                const int first_row = work.tile_row[t] + 32 * (warp & 3);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if (row_vectors && first_row < s.seq) {
+                        for (int x = 0; 64 * x < s.dim; ++x) {
+                            tma_rows(&o_map, q_tile + x * kHalfTileBytes + 32 * (warp & 3) * 128, 64 * x, first_row, h, work.b);
+                        }
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    }
+                    mbar_arrive(&s_qempty[turn % C::QUERIES]);
+                }
+                __syncwarp();
+            }
             unsigned bad = __ballot_sync(0xffffffffu, i < s.seq && !(most <= 65504.f));
+            if (C::ROWS_BY_TMA && bad != 0 && lane == 0) {   // the rows just sent have to be there before they are written again
+                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            }
+            __syncwarp();
             while (bad != 0) {
                 const int from = __ffs(bad) - 1;
                 bad &= bad - 1;
@@ -1201,7 +1233,7 @@ inline bool window_map(CUtensorMap *map, const __half *p, int dim, int seq, int 
 }
 
 template <int DP, int NQ>
-int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, const __half *q, const __half *k, const __half *v,
+int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm, const CUtensorMap &om, bool row_vectors, const __half *q, const __half *k, const __half *v,
                      const int8_t *mask, __half *context, const WindowShape &s, cudaStream_t stream) {
     typedef WindowTc<DP, NQ> C;
     static std::atomic<uint64_t> prepared{0};   // devices on which the kernel may use its shared memory
@@ -1224,7 +1256,7 @@ int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
     if (items > 0x7fffffffLL) {
         return CUBK_ERR_UNSUPPORTED;
     }
-    window_tc_kernel<DP, NQ><<<(unsigned) items, C::THREADS, C::SMEM_BYTES, stream>>>(qm, km, vm, q, k, v, mask, context, s, row_blocks, pair);
+    window_tc_kernel<DP, NQ><<<(unsigned) items, C::THREADS, C::SMEM_BYTES, stream>>>(qm, km, vm, om, row_vectors, q, k, v, mask, context, s, row_blocks, pair);
     return check_launch();
 }
 
@@ -1233,15 +1265,20 @@ int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
 // largest product): the caller takes another kernel.
 inline int window_tc(const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context, const WindowShape &s,
                      cudaStream_t stream) {
-    CUtensorMap qm, km, vm;
+    CUtensorMap qm, km, vm, om;
     const int keys = s.dim <= 64 ? WindowTc<64, 1>::KEYS : WindowTc<128, 2>::KEYS;
     if (s.dim > 128 || !(s.scale > 0.f) || !window_map(&qm, q, s.dim, s.seq, s.heads, s.batch, s.q_stride, kTileRows) ||
         !window_map(&km, k, s.dim, s.seq, s.kv_heads, s.batch, s.kv_stride, keys) ||
         !window_map(&vm, v, s.dim, s.seq, s.kv_heads, s.batch, s.kv_stride, keys)) {
         return CUBK_ERR_UNSUPPORTED;
     }
-    return s.dim <= 64 ? window_tc_launch<64, 1>(qm, km, vm, q, k, v, mask, context, s, stream)
-                       : window_tc_launch<128, 2>(qm, km, vm, q, k, v, mask, context, s, stream);
+    // a context whose rows or heads do not start on 16-byte boundaries is written element by element
+    const bool row_vectors = window_map(&om, context, s.dim, s.seq, s.heads, s.batch, s.context_stride, 32);
+    if (!row_vectors) {
+        om = qm;
+    }
+    return s.dim <= 64 ? window_tc_launch<64, 1>(qm, km, vm, om, row_vectors, q, k, v, mask, context, s, stream)
+                       : window_tc_launch<128, 2>(qm, km, vm, om, row_vectors, q, k, v, mask, context, s, stream);
 }
 
 template <typename T>
