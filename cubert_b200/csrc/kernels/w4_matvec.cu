@@ -12,8 +12,6 @@
 // applied to float32 sums of whole groups and nothing is rounded but those sums.
 //   binary16 x: operands as they are.  e4m3 x: exact in binary16; their scales meet the float32 sums.
 //   float32 x: split exactly into three bfloat16 parts (8 bits of mantissa each), three products.
-#include <cuda_fp8.h>
-
 #include "common.cuh"
 
 namespace cubk {
@@ -512,6 +510,7 @@ int w4_matvec_launch(const typename XLoad<X>::Elem *x, const float *x_scales, in
     // one block per SM, by its registers; asked with all of the shared memory so that the answer holds for every plan
     const int resident = resident_blocks(w4_matvec_kernel<T, X, TT, GROUP>, 32 * kW4Warps, 227 * 1024, &cache, true);
     if (resident <= 0) {
+        set_last_error(cudaErrorLaunchOutOfResources);
         return CUBK_ERR_LAUNCH;
     }
     const W4Plan plan = w4_plan(k, S::LIMIT, S::X_TILE + S::SCALES, S::CARRY);

@@ -1,12 +1,8 @@
-// K8: attention with a sliding window and first tokens that stay visible (sinks).
+// K8, whole sequences: attention with a sliding window and first tokens that stay visible (sinks).
 //
-// Whole sequences: query i sees key j when the key is kept, j <= i + after, and j >= i - before or j < sinks.
-// Single tokens: keys and values live in a ring of sinks + window slots per stream; the slot of position p is p
-// below sinks and sinks + (p - sinks) % window from there on, so the slots that hold anything are the first
-// min(p + 1, sinks + window) and every one of them is visible to p.
-// Softmax statistics and all sums are float32. A key that a query does not see contributes nothing at all, whatever
-// bits its rows hold; a query that sees no key gets zeros.
-#include <cooperative_groups.h>
+// Query i sees key j when the key is kept, j <= i + after, and j >= i - before or j < sinks. Softmax statistics and all sums
+// are float32. A key that a query does not see contributes nothing at all, whatever bits its rows hold; a query that sees no
+// key gets zeros.
 #include <cuda.h>
 
 #include <limits.h>
@@ -14,88 +10,9 @@
 #include <atomic>
 #include <type_traits>
 
-#include "common.cuh"
+#include "window_row.cuh"
 
 namespace cubk {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kWindowMaxDim = 256;
-constexpr int kWindowRowWarps = 4;
-
-// ---------------------------------------------------------------- one query row per warp
-// Any head dimension up to 256, any strides: 32 keys at a time, a key per lane for the scores, a column (or several)
-// per lane for the context. `key(j)` and `value(j)` give the addresses of row j, `seen(j)` says whether it counts.
-template <typename T, typename Key, typename Value, typename Seen>
-__device__ void window_row(const T *q, float *s_q, int dim, float scale, int sinks_end, int lo, int hi, Key key, Value value, Seen seen,
-                           T *context) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    for (int c = lane; c < dim; c += 32) {
-        s_q[c] = to_float<T>(q[c]);
-    }
-    __syncwarp();
-    float o[kWindowMaxDim / 32];
-#pragma unroll
-    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
-        o[i] = 0.f;
-    }
-    float top = -INFINITY, total = 0.f;
-    for (int part = 0; part < 2; ++part) {
-        const int begin = part == 0 ? 0 : lo, end = part == 0 ? sinks_end : hi;
-        for (int j0 = begin; j0 < end; j0 += 32) {
-            const int j = j0 + lane;
-            const bool use = j < end && seen(j);
-            float s = -INFINITY;
-            if (use) {
-                const T *kr = key(j);
-                float a0 = 0.f, a1 = 0.f;
-                int c = 0;
-                for (; c + 1 < dim; c += 2) {
-                    a0 = fmaf(s_q[c], to_float<T>(kr[c]), a0);
-                    a1 = fmaf(s_q[c + 1], to_float<T>(kr[c + 1]), a1);
-                }
-                if (c < dim) {
-                    a0 = fmaf(s_q[c], to_float<T>(kr[c]), a0);
-                }
-                s = scale * kLog2e * (a0 + a1);
-            }
-            unsigned visible = __ballot_sync(0xffffffffu, use);
-            const float next = fmaxf(top, group_max<32>(s));
-            if (visible == 0 || next == -INFINITY) {
-                if (!__any_sync(0xffffffffu, use && !(s == -INFINITY))) {   // a NaN score goes on below
-                    continue;
-                }
-            }
-            const float shrink = top == -INFINITY ? 0.f : fast_exp2(top - next);
-            const float p = use ? fast_exp2(s - next) : 0.f;
-            top = next;
-            total = total * shrink + group_sum<32>(p);
-#pragma unroll
-            for (int i = 0; i < kWindowMaxDim / 32; ++i) {
-                o[i] *= shrink;
-            }
-            while (visible != 0) {
-                const int from = __ffs(visible) - 1;
-                visible &= visible - 1;
-                const float w = __shfl_sync(0xffffffffu, p, from);
-                const T *vr = value(j0 + from);
-#pragma unroll
-                for (int i = 0; i < kWindowMaxDim / 32; ++i) {
-                    if (lane + 32 * i < dim) {
-                        o[i] = fmaf(w, to_float<T>(vr[lane + 32 * i]), o[i]);
-                    }
-                }
-            }
-        }
-    }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
-        if (lane + 32 * i < dim) {
-            context[lane + 32 * i] = from_float<T>(o[i] * inv);
-        }
-    }
-}
 
 struct WindowShape {
     int batch, seq, heads, kv_heads, dim;
@@ -422,27 +339,30 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 // ---------------------------------------------------------------- whole sequences on tcgen05 (binary16)
 // A work item is NQ tiles of 128 query rows: two heads that share their keys, or consecutive rows of one head. The grid has a block
 // per item; a block that runs takes over items of blocks that have not started yet (cluster launch control), loading and multiplying
-// ahead into the next while the last one's rows are written: no block waits for its first loads but the first on each SM, and masks
-// that make items unequal cost nothing. Per step of up
-// to KEYS keys and per tile: S = Q.K^T (tcgen05.mma, float32 accumulators in tensor memory), softmax by 128 threads that own
-// a row each (tensor-memory lane = query row, so no shuffles), P back into tensor memory as binary16, O += P.V with P as the
-// tensor-memory operand. Warps: 4 NQ for the softmax, NQ that issue the MMAs of a tile, one that chooses the steps and loads K
-// and V with TMA (128-byte swizzle; V is read as it lies, as an MN-major operand).
+// ahead into the next while the last one's rows are written, so that only the first block on an SM waits for its first loads. Per
+// step of up to KEYS keys and per tile: S = Q.K^T (tcgen05.mma, float32 accumulators in tensor memory), softmax by 128 threads that
+// own a row each (tensor-memory lane = query row, so no shuffles), P back into tensor memory as binary16, O += P.V with P as the
+// tensor-memory operand. Warps: 4 NQ for the softmax, NQ that issue the MMAs of a tile, one that takes items, chooses their steps and
+// loads Q, K and V with TMA (128-byte swizzle; V is read as it lies, as an MN-major operand).
 //   * The scores' place is free as soon as a row is in registers, so the next step's scores are computed while this step's
 //     exponentials are; the weights have a place of their own, so their product runs under the next step's softmax. KEYS is what
 //     fits beside the contexts: 128 for heads of up to 64 (two blocks of one tile share an SM), 80 for 128 (one of two tiles).
-//   * Steps of an item: first the sinks below the window, then the window, then one without keys that ends it. A step whose keys are all masked is left out; one that every row of
-//     a tile sees whole skips the masking.
+//   * Steps of an item: first the sinks below the window, then the window, then one without keys that ends it. A step whose keys are
+//     all masked is left out; one that every row of a tile sees whole skips the masking.
 //   * The running maximum of a row is raised only when a step's maximum exceeds it by 2^8 (a weight is then at most 256, far
 //     inside binary16, and the sums are float32), so that O is read back and scaled in few steps.
 //   * Weights of unseen keys are exactly 0, but 0 times an infinity or NaN in an unseen V row is NaN: a row that comes out not
 //     finite is computed again by one warp over its visible keys alone.
+// Bound by the softmax: per 128 x 128 tile the exponentials take 1024 cycles of an SM's special-function unit and the products 512 of
+// its tensor cores (heads of 64; 1024 for heads of 128), a step 1500. Measured: 8192 tokens, 32 / 8 heads of 128, window 2048: 265 to
+// 290 us by the clock under the power cap (840 to 910 TFLOP/s); 4 x 4096 tokens, 16 heads of 64, no window 400 us, window 513 and ragged
+// lengths 85 us (5 steps an item: half of that goes into the ends of items). Tried and slower: two threads a row, part of the
+// exponentials by polynomial, scores of 96 keys twice, masks gathered by a warp of their own.
 // Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, frees its tensor memory and
 // returns.
 constexpr int kTileRows = 128;
 constexpr int kHalfTileBytes = kTileRows * 128;    // 128 rows x 64 binary16
 constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 2
-constexpr float kRaiseBy = 8.f;                    // log2 of the largest weight
 
 struct WindowStep {
     int item, j0;
@@ -460,8 +380,9 @@ struct WindowTc {
     static constexpr int HALF_KV = KEYS * 128, KV_BYTES = HALVES * HALF_KV;
     static constexpr int STAGES = 2, QUERIES = 2;            // tiles of K and V, and of Q, on their way or in use
     static constexpr int SOFTMAX_WARPS = 4 * NQ;
-    // Softmax warps in whole groups of four, and one more group for the others (the last of it idle), which hands most of its
-    // registers to them. Launched with 65536 / (THREADS x blocks per SM) each: 128 x 256 >= 192 x 128 + 56 x 128, 168 x 384 >= 224 x 256 + 56 x 128.
+    // Softmax warps in whole groups of four, and one more group for the others (one or two of it idle), which hands most of its
+    // registers to them: a row's scores stay in registers, 128 of them. Launched with 65536 / (THREADS x blocks per SM) each:
+    // 128 x 256 >= 192 x 128 + 56 x 128, 168 x 384 >= 224 x 256 + 56 x 128.
     static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
     // The context's rows leave through the place of the item's queries by TMA, or as 16-byte stores from registers. TMA holds the queries
     // of the item after the next back until they have left: 8192 tokens, 32 heads of 128: 265 us against 277, but 4 x 4096 tokens, 16
@@ -647,8 +568,8 @@ struct WindowItem {
 template <int DP, int NQ>
 __global__ void __launch_bounds__(WindowTc<DP, NQ>::THREADS, NQ == 1 ? 2 : 1)
 window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                 const __grid_constant__ CUtensorMap o_map, bool row_vectors, const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context, const __grid_constant__ WindowShape s,
-                 int row_blocks, int pair_heads) {
+                 const __grid_constant__ CUtensorMap o_map, bool row_vectors, const __half *q, const __half *k, const __half *v,
+                 const int8_t *mask, __half *context, const __grid_constant__ WindowShape s, int row_blocks, int pair_heads) {
     typedef WindowTc<DP, NQ> C;
     extern __shared__ unsigned char tc_raw[];
     __shared__ uint64_t s_qfull[C::QUERIES], s_qempty[C::QUERIES], s_kfull[C::STAGES], s_kempty[C::STAGES], s_vfull[C::STAGES], s_vempty[C::STAGES];
@@ -704,260 +625,260 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     // Every barrier below completes one phase per step (or item), whatever the step is, so `step` and `turn`, which count through
     // all items, give their parities.
     if (warp >= C::SOFTMAX_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
-    if (warp == C::SOFTMAX_WARPS + NQ) {
-        // ---- steps and loads
-        bool ok = true;
-        int step = 0, turn = 0;
-        for (int item = blockIdx.x; item >= 0 && ok; ++turn) {
-            const WindowItem<NQ> w(item, s, row_blocks, pair_heads);
-            if (lane == 0) {
-                s_items[turn & 3] = item;
-                s_turns = turn + 1;
-            }
-            const int lo = w.row0 > s.before ? (w.row0 - s.before) & ~3 : 0;   // whole words of the mask
-            const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
-            const int sinks_end = min(s.sinks, lo), sink_steps = (sinks_end + C::KEYS - 1) / C::KEYS;
-            const int steps = sink_steps + (hi - lo + C::KEYS - 1) / C::KEYS;
-            const int8_t *kept = mask != nullptr ? mask + (int64_t) w.b * s.seq : nullptr;
-            const int qb = turn % C::QUERIES;
-            if (turn >= C::QUERIES) {
-                ok = wait_together(&s_qempty[qb], (turn / C::QUERIES - 1) & 1);
-            }
-            if (ok && lane == 0) {
-                mbar_arrive_expect(&s_qfull[qb], NQ * C::TILE_BYTES);
-                for (int t = 0; t < NQ; ++t) {
-                    for (int x = 0; x < C::HALVES; ++x) {
-                        tma_tile(s_qt + (qb * NQ + t) * C::TILE_BYTES + x * kHalfTileBytes, &q_map, 64 * x, w.tile_row[t], w.tile_head[t], w.b,
-                                 &s_qfull[qb]);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+        if (warp == C::SOFTMAX_WARPS + NQ) {
+            // ---- items, steps and loads
+            bool ok = true;
+            int step = 0, turn = 0;
+            for (int item = blockIdx.x; item >= 0 && ok; ++turn) {
+                const WindowItem<NQ> w(item, s, row_blocks, pair_heads);
+                if (lane == 0) {
+                    s_items[turn & 3] = item;
+                    s_turns = turn + 1;
+                }
+                const int lo = w.row0 > s.before ? (w.row0 - s.before) & ~3 : 0;   // whole words of the mask
+                const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
+                const int sinks_end = min(s.sinks, lo), sink_steps = (sinks_end + C::KEYS - 1) / C::KEYS;
+                const int steps = sink_steps + (hi - lo + C::KEYS - 1) / C::KEYS;
+                const int8_t *kept = mask != nullptr ? mask + (int64_t) w.b * s.seq : nullptr;
+                const int qb = turn % C::QUERIES;
+                if (turn >= C::QUERIES) {
+                    ok = wait_together(&s_qempty[qb], (turn / C::QUERIES - 1) & 1);
+                }
+                if (ok && lane == 0) {
+                    mbar_arrive_expect(&s_qfull[qb], NQ * C::TILE_BYTES);
+                    for (int t = 0; t < NQ; ++t) {
+                        for (int x = 0; x < C::HALVES; ++x) {
+                            tma_tile(s_qt + (qb * NQ + t) * C::TILE_BYTES + x * kHalfTileBytes, &q_map, 64 * x, w.tile_row[t], w.tile_head[t], w.b,
+                                     &s_qfull[qb]);
+                        }
                     }
                 }
-            }
-            // 32 candidates at a time, one per lane; then those that hold a kept key, and the item's end, one after another.
-            for (int base = 0; base <= steps && ok; base += 32) {
-                if (kept != nullptr) {   // four keys a lane, eight steps in flight
-                    const int candidates = min(32, steps - base);
-                    const bool words = s.seq % 4 == 0 && (reinterpret_cast<uintptr_t>(mask) & 3) == 0;   // of four keys: none reaches past its row
-                    __syncwarp();
-                    for (int c0 = 0; c0 < candidates; c0 += 8) {
-                        uint32_t four[8];
+                // 32 candidates at a time, one per lane; then those that hold a kept key, and the item's end, one after another.
+                for (int base = 0; base <= steps && ok; base += 32) {
+                    if (kept != nullptr) {   // four keys a lane, eight steps in flight
+                        const int candidates = min(32, steps - base);
+                        const bool words = s.seq % 4 == 0 && (reinterpret_cast<uintptr_t>(mask) & 3) == 0;   // of four keys: none reaches past its row
+                        __syncwarp();
+                        for (int c0 = 0; c0 < candidates; c0 += 8) {
+                            uint32_t four[8];
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            const int at = base + c0 + u;
-                            const int j = (at < sink_steps ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS) + 4 * lane;
-                            const int left = c0 + u < candidates && 4 * lane < C::KEYS ? (at < sink_steps ? sinks_end : hi) - j : 0;
-                            four[u] = 0;
-                            if (words) {
-                                four[u] = left > 0 ? *reinterpret_cast<const uint32_t *>(kept + j) & (left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u) : 0u;
-                            } else {
+                            for (int u = 0; u < 8; ++u) {
+                                const int at = base + c0 + u;
+                                const int j = (at < sink_steps ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS) + 4 * lane;
+                                const int left = c0 + u < candidates && 4 * lane < C::KEYS ? (at < sink_steps ? sinks_end : hi) - j : 0;
+                                four[u] = 0;
+                                if (words) {
+                                    four[u] = left > 0 ? *reinterpret_cast<const uint32_t *>(kept + j) & (left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u) : 0u;
+                                } else {
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    four[u] |= e < left ? (uint32_t) (uint8_t) kept[j + e] << (8 * e) : 0u;
+                                    for (int e = 0; e < 4; ++e) {
+                                        four[u] |= e < left ? (uint32_t) (uint8_t) kept[j + e] << (8 * e) : 0u;
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) {
+                                // any bit of a byte -> its lowest; the four lowest bits side by side; eight lanes' to a word
+                                uint32_t v = four[u] | four[u] >> 4;
+                                v |= v >> 2;
+                                v |= v >> 1;
+                                v = ((v & 0x01010101u) * 0x01020408u >> 24 & 15u) << (4 * (lane & 7));
+                                v |= __shfl_xor_sync(0xffffffffu, v, 1);
+                                v |= __shfl_xor_sync(0xffffffffu, v, 2);
+                                v |= __shfl_xor_sync(0xffffffffu, v, 4);
+                                if ((lane & 7) == 0 && c0 + u < candidates) {
+                                    s_bits[c0 + u][lane >> 3] = v;
                                 }
                             }
                         }
+                        __syncwarp();
+                    }
+                    const int at = base + lane;
+                    const bool in_sinks = at < sink_steps;
+                    const int keys = at < steps ? min((in_sinks ? sinks_end : hi) - (in_sinks ? at : at - sink_steps) * C::KEYS - (in_sinks ? 0 : lo), C::KEYS) : 0;
+                    WindowStep d;
+                    d.item = item;
+                    d.j0 = in_sinks ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS;
+                    d.columns = keys == 0 ? 0 : keys <= 16 ? 16 : C::KEYS;
+                    d.flags = 0;
+                    int count = 0;
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) {
-                            // any bit of a byte -> its lowest; the four lowest bits side by side; eight lanes' to a word
-                            uint32_t v = four[u] | four[u] >> 4;
-                            v |= v >> 2;
-                            v |= v >> 1;
-                            v = ((v & 0x01010101u) * 0x01020408u >> 24 & 15u) << (4 * (lane & 7));
-                            v |= __shfl_xor_sync(0xffffffffu, v, 1);
-                            v |= __shfl_xor_sync(0xffffffffu, v, 2);
-                            v |= __shfl_xor_sync(0xffffffffu, v, 4);
-                            if ((lane & 7) == 0 && c0 + u < candidates) {
-                                s_bits[c0 + u][lane >> 3] = v;
+                    for (int u = 0; u < 4; ++u) {
+                        d.kept[u] = keys == 0 ? 0 : kept != nullptr ? s_bits[lane][u] : range_bits(0, keys, 32 * u);
+                        count += __popc(d.kept[u]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < NQ; ++t) {
+                        const int first = w.tile_row[t], last = min(first + kTileRows, s.seq) - 1;
+                        const int t_lo = first > s.before ? first - s.before : 0;
+                        const int t_hi = s.after < s.seq - 1 - last ? last + s.after + 1 : s.seq;
+                        if (count > 0 && first < s.seq && d.j0 < t_hi && (d.j0 + keys > t_lo || d.j0 < s.sinks)) {
+                            d.flags |= 1u << t;
+                        }
+                        const bool whole = count == d.columns && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
+                                           (last - s.before <= d.j0 || d.j0 + keys <= s.sinks);
+                        if (!whole) {
+                            d.flags |= 16u << t;
+                        }
+                    }
+                    unsigned todo = __ballot_sync(0xffffffffu, (d.flags & 15u) != 0 || at == steps);
+                    while (todo != 0 && ok) {
+                        const int from = __ffs(todo) - 1;
+                        todo &= todo - 1;
+                        const int j0 = __shfl_sync(0xffffffffu, d.j0, from);
+                        const bool end = base + from == steps;
+                        if (end && lane == 0) {   // the next item: not earlier, so that blocks finish together
+                            mbar_arrive_expect(&s_takes, 16);
+                            take_block(&s_taken[turn & 1], &s_takes);
+                        }
+                        const int st = step % C::STAGES;
+                        const uint32_t before = (step / C::STAGES - 1) & 1;
+                        if (step >= C::STAGES) {
+                            ok = wait_together(&s_kempty[st], before);
+                        }
+                        if (lane == from) {
+                            s_steps[step % kStepSlots] = d;
+                        }
+                        __syncwarp();
+                        if (ok && lane == 0) {
+                            if (!end) {
+                                mbar_arrive_expect(&s_kfull[st], C::KV_BYTES);
+                                for (int x = 0; x < C::HALVES; ++x) {
+                                    tma_tile(s_kt + st * C::KV_BYTES + x * C::HALF_KV, &k_map, 64 * x, j0, w.kh, w.b, &s_kfull[st]);
+                                }
+                            } else {
+                                mbar_arrive(&s_kfull[st]);
                             }
                         }
-                    }
-                    __syncwarp();
-                }
-                const int at = base + lane;
-                const bool in_sinks = at < sink_steps;
-                const int keys = at < steps ? min((in_sinks ? sinks_end : hi) - (in_sinks ? at : at - sink_steps) * C::KEYS - (in_sinks ? 0 : lo), C::KEYS) : 0;
-                WindowStep d;
-                d.item = item;
-                d.j0 = in_sinks ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS;
-                d.columns = keys == 0 ? 0 : keys <= 16 ? 16 : C::KEYS;
-                d.flags = 0;
-                int count = 0;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    d.kept[u] = keys == 0 ? 0 : kept != nullptr ? s_bits[lane][u] : range_bits(0, keys, 32 * u);
-                    count += __popc(d.kept[u]);
-                }
-#pragma unroll
-                for (int t = 0; t < NQ; ++t) {
-                    const int first = w.tile_row[t], last = min(first + kTileRows, s.seq) - 1;
-                    const int t_lo = first > s.before ? first - s.before : 0;
-                    const int t_hi = s.after < s.seq - 1 - last ? last + s.after + 1 : s.seq;
-                    if (count > 0 && first < s.seq && d.j0 < t_hi && (d.j0 + keys > t_lo || d.j0 < s.sinks)) {
-                        d.flags |= 1u << t;
-                    }
-                    const bool whole = count == d.columns && (s.after >= s.seq || d.j0 + keys - 1 <= first + s.after) &&
-                                       (last - s.before <= d.j0 || d.j0 + keys <= s.sinks);
-                    if (!whole) {
-                        d.flags |= 16u << t;
-                    }
-                }
-                unsigned todo = __ballot_sync(0xffffffffu, (d.flags & 15u) != 0 || at == steps);
-                while (todo != 0 && ok) {
-                    const int from = __ffs(todo) - 1;
-                    todo &= todo - 1;
-                    const int j0 = __shfl_sync(0xffffffffu, d.j0, from);
-                    const bool end = base + from == steps;
-                    if (end && lane == 0) {   // the next item: not earlier, so that blocks finish together
-                        mbar_arrive_expect(&s_takes, 16);
-                        take_block(&s_taken[turn & 1], &s_takes);
-                    }
-                    const int st = step % C::STAGES;
-                    const uint32_t before = (step / C::STAGES - 1) & 1;
-                    if (step >= C::STAGES) {
-                        ok = wait_together(&s_kempty[st], before);
-                    }
-                    if (lane == from) {
-                        s_steps[step % kStepSlots] = d;
-                    }
-                    __syncwarp();
-                    if (ok && lane == 0) {
-                        if (!end) {
-                            mbar_arrive_expect(&s_kfull[st], C::KV_BYTES);
-                            for (int x = 0; x < C::HALVES; ++x) {
-                                tma_tile(s_kt + st * C::KV_BYTES + x * C::HALF_KV, &k_map, 64 * x, j0, w.kh, w.b, &s_kfull[st]);
-                            }
-                        } else {
-                            mbar_arrive(&s_kfull[st]);
+                        __syncwarp();
+                        if (ok && step >= C::STAGES) {
+                            ok = wait_together(&s_vempty[st], before);
                         }
-                    }
-                    __syncwarp();
-                    if (ok && step >= C::STAGES) {
-                        ok = wait_together(&s_vempty[st], before);
-                    }
-                    if (ok && lane == 0) {
-                        if (!end) {
-                            mbar_arrive_expect(&s_vfull[st], C::KV_BYTES);
-                            for (int x = 0; x < C::HALVES; ++x) {
-                                tma_tile(s_vt + st * C::KV_BYTES + x * C::HALF_KV, &v_map, 64 * x, j0, w.kh, w.b, &s_vfull[st]);
-                            }
-                        } else {
-                            mbar_arrive(&s_vfull[st]);
-                        }
-                    }
-                    __syncwarp();
-                    step += ok ? 1 : 0;
-                }
-            }
-            ok = ok && wait_together(&s_takes, turn & 1);
-            item = ok ? taken_block(&s_taken[turn & 1]) : -1;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the answer is read before its place is written again
-        }
-        if (ok) {   // the end of all
-            const int st = step % C::STAGES;
-            if (step >= C::STAGES) {
-                ok = wait_together(&s_kempty[st], (step / C::STAGES - 1) & 1);
-            }
-            if (ok && lane == 0) {
-                s_steps[step % kStepSlots].columns = -1;
-                s_steps[step % kStepSlots].flags = 0;
-                mbar_arrive(&s_kfull[st]);
-            }
-            __syncwarp();
-        }
-        if (!ok) {   // the copies in flight land before the block's shared memory goes
-            if (turn > 0 && wait_together(&s_takes, (turn - 1) & 1) && lane == 0 && taken_block(&s_taken[(turn - 1) & 1]) >= 0) {
-                s_items[turn & 3] = taken_block(&s_taken[(turn - 1) & 1]);   // taken over and not begun
-                s_turns = turn + 1;
-            }
-            for (int i = max(turn - C::QUERIES, 0); i <= turn; ++i) {
-                (void) wait_together(&s_qfull[i % C::QUERIES], (i / C::QUERIES) & 1);
-            }
-            for (int i = max(step - C::STAGES, 0); i <= step; ++i) {
-                (void) wait_together(&s_kfull[i % C::STAGES], (i / C::STAGES) & 1);
-                (void) wait_together(&s_vfull[i % C::STAGES], (i / C::STAGES) & 1);
-            }
-        }
-    } else if (warp < C::SOFTMAX_WARPS + NQ) {
-        // ---- matrix products of a tile: the warp walks together (its addresses stay in uniform registers), one lane issues
-        const int t = warp - C::SOFTMAX_WARPS;
-        const uint32_t ksteps = (uint32_t) (s.dim + 15) / 16;
-        const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((2 * ksteps) << 17) | ((kTileRows >> 4) << 24);   // N: the dimension, in 16s
-        const bool leader = elect_one();
-        const uint64_t q_desc = swizzled_desc(smem_addr(s_qt + t * C::TILE_BYTES), 16), k_desc = swizzled_desc(smem_addr(s_kt), 16);
-        const uint64_t v_desc = swizzled_desc(smem_addr(s_vt), C::HALF_KV);
-        const uint32_t t_s = tmem + t * C::KEYS, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2), t_o = tmem + C::CONTEXT + t * DP;
-        bool ok = true, started = false;   // started: O holds something of this item
-        int columns_before = 0, step = 0, turn = 0;
-        uint32_t flags_before = 0;
-        bool new_item = true;
-        uint64_t qd = 0;
-        for (; ok; ++step) {
-            const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES, qb = turn % C::QUERIES;
-            ok = wait_together(&s_kfull[st], (step / C::STAGES) & 1);
-            const int columns = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].columns, 0);
-            const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0) >> t;
-            if (new_item && columns >= 0) {
-                ok = ok && wait_together(&s_qfull[qb], (turn / C::QUERIES) & 1);
-                qd = q_desc + (uint64_t) (qb * NQ * (C::TILE_BYTES / 16));
-                new_item = false;
-            }
-            if (step > 0) {
-                ok = ok && wait_together(&s_sfree[t], (step - 1) & 1);
-                tmem_fence_after();
-            }
-            if (ok && leader) {
-                if ((flags & 1u) != 0) {
-                    const uint64_t kd = k_desc + (uint64_t) (st * (C::KV_BYTES / 16));
-                    const uint32_t idesc_s = (1u << 4) | ((uint32_t) (columns / 8) << 17) | ((kTileRows >> 4) << 24);
-#pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk) {
-                        if (kk < (int) ksteps) {
-                            mma_ss(t_s, qd + ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16, kd + ((kk >> 2) * C::HALF_KV + (kk & 3) * 32) / 16,
-                                   idesc_s, kk > 0);
-                        }
-                    }
-                }
-                mma_commit(&s_sfull[t]);
-                mbar_arrive(&s_sfull[t]);
-                if (columns >= 0) {
-                    mma_commit(&s_kempty[st]);
-                }
-                if (columns == 0) {
-                    mma_commit(&s_qempty[qb]);
-                }
-            }
-            __syncwarp();
-            if (columns < 0) {
-                break;
-            }
-            if (step > 0) {   // O += P.V of the step before; of one that ended an item, only the wait until O has been read
-                ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
-                tmem_fence_after();
-                const bool takes_part = (flags_before & 1u) != 0;
-                if (ok && leader) {
-                    if (takes_part) {
-                        const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
-#pragma unroll
-                        for (int kk = 0; kk < C::KEYS / 16; ++kk) {
-                            if (16 * kk < columns_before) {
-                                mma_ts(t_o, t_p + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || started);
+                        if (ok && lane == 0) {
+                            if (!end) {
+                                mbar_arrive_expect(&s_vfull[st], C::KV_BYTES);
+                                for (int x = 0; x < C::HALVES; ++x) {
+                                    tma_tile(s_vt + st * C::KV_BYTES + x * C::HALF_KV, &v_map, 64 * x, j0, w.kh, w.b, &s_vfull[st]);
+                                }
+                            } else {
+                                mbar_arrive(&s_vfull[st]);
                             }
                         }
+                        __syncwarp();
+                        step += ok ? 1 : 0;
                     }
-                    mma_commit(&s_ofull[t]);
-                    mma_commit(&s_vempty[st_before]);
                 }
-                started = columns_before != 0 && (started || takes_part);
+                ok = ok && wait_together(&s_takes, turn & 1);
+                item = ok ? taken_block(&s_taken[turn & 1]) : -1;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the answer is read before its place is written again
+            }
+            if (ok) {   // the end of all
+                const int st = step % C::STAGES;
+                if (step >= C::STAGES) {
+                    ok = wait_together(&s_kempty[st], (step / C::STAGES - 1) & 1);
+                }
+                if (ok && lane == 0) {
+                    s_steps[step % kStepSlots].columns = -1;
+                    s_steps[step % kStepSlots].flags = 0;
+                    mbar_arrive(&s_kfull[st]);
+                }
                 __syncwarp();
             }
-            columns_before = columns;
-            flags_before = flags;
-            if (columns == 0) {
-                new_item = true;
-                ++turn;
+            if (!ok) {   // the copies in flight land before the block's shared memory goes
+                if (turn > 0 && wait_together(&s_takes, (turn - 1) & 1) && lane == 0 && taken_block(&s_taken[(turn - 1) & 1]) >= 0) {
+                    s_items[turn & 3] = taken_block(&s_taken[(turn - 1) & 1]);   // taken over and not begun
+                    s_turns = turn + 1;
+                }
+                for (int i = max(turn - C::QUERIES, 0); i <= turn; ++i) {
+                    (void) wait_together(&s_qfull[i % C::QUERIES], (i / C::QUERIES) & 1);
+                }
+                for (int i = max(step - C::STAGES, 0); i <= step; ++i) {
+                    (void) wait_together(&s_kfull[i % C::STAGES], (i / C::STAGES) & 1);
+                    (void) wait_together(&s_vfull[i % C::STAGES], (i / C::STAGES) & 1);
+                }
+            }
+        } else if (warp < C::SOFTMAX_WARPS + NQ) {
+            // ---- matrix products of a tile: the warp walks together (its addresses stay in uniform registers), one lane issues
+            const int t = warp - C::SOFTMAX_WARPS;
+            const uint32_t ksteps = (uint32_t) (s.dim + 15) / 16;
+            const uint32_t idesc_o = (1u << 4) | (1u << 16) | ((2 * ksteps) << 17) | ((kTileRows >> 4) << 24);   // N: the dimension, in 16s
+            const bool leader = elect_one();
+            const uint64_t q_desc = swizzled_desc(smem_addr(s_qt + t * C::TILE_BYTES), 16), k_desc = swizzled_desc(smem_addr(s_kt), 16);
+            const uint64_t v_desc = swizzled_desc(smem_addr(s_vt), C::HALF_KV);
+            const uint32_t t_s = tmem + t * C::KEYS, t_p = tmem + C::WEIGHTS + t * (C::KEYS / 2), t_o = tmem + C::CONTEXT + t * DP;
+            bool ok = true, started = false;   // started: O holds something of this item
+            int columns_before = 0, step = 0, turn = 0;
+            uint32_t flags_before = 0;
+            bool new_item = true;
+            uint64_t qd = 0;
+            for (; ok; ++step) {
+                const int st = step % C::STAGES, st_before = (step + C::STAGES - 1) % C::STAGES, qb = turn % C::QUERIES;
+                ok = wait_together(&s_kfull[st], (step / C::STAGES) & 1);
+                const int columns = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].columns, 0);
+                const uint32_t flags = __shfl_sync(0xffffffffu, s_steps[step % kStepSlots].flags, 0) >> t;
+                if (new_item && columns >= 0) {
+                    ok = ok && wait_together(&s_qfull[qb], (turn / C::QUERIES) & 1);
+                    qd = q_desc + (uint64_t) (qb * NQ * (C::TILE_BYTES / 16));
+                    new_item = false;
+                }
+                if (step > 0) {
+                    ok = ok && wait_together(&s_sfree[t], (step - 1) & 1);
+                    tmem_fence_after();
+                }
+                if (ok && leader) {
+                    if ((flags & 1u) != 0) {
+                        const uint64_t kd = k_desc + (uint64_t) (st * (C::KV_BYTES / 16));
+                        const uint32_t idesc_s = (1u << 4) | ((uint32_t) (columns / 8) << 17) | ((kTileRows >> 4) << 24);
+#pragma unroll
+                        for (int kk = 0; kk < DP / 16; ++kk) {
+                            if (kk < (int) ksteps) {
+                                mma_ss(t_s, qd + ((kk >> 2) * kHalfTileBytes + (kk & 3) * 32) / 16, kd + ((kk >> 2) * C::HALF_KV + (kk & 3) * 32) / 16,
+                                       idesc_s, kk > 0);
+                            }
+                        }
+                    }
+                    mma_commit(&s_sfull[t]);
+                    mbar_arrive(&s_sfull[t]);
+                    if (columns >= 0) {
+                        mma_commit(&s_kempty[st]);
+                    }
+                    if (columns == 0) {
+                        mma_commit(&s_qempty[qb]);
+                    }
+                }
+                __syncwarp();
+                if (columns < 0) {
+                    break;
+                }
+                if (step > 0) {   // O += P.V of the step before; of one that ended an item, only the wait until O has been read
+                    ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
+                    tmem_fence_after();
+                    const bool takes_part = (flags_before & 1u) != 0;
+                    if (ok && leader) {
+                        if (takes_part) {
+                            const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
+#pragma unroll
+                            for (int kk = 0; kk < C::KEYS / 16; ++kk) {
+                                if (16 * kk < columns_before) {
+                                    mma_ts(t_o, t_p + 8 * kk, vd + 128 * kk, idesc_o, kk > 0 || started);
+                                }
+                            }
+                        }
+                        mma_commit(&s_ofull[t]);
+                        mma_commit(&s_vempty[st_before]);
+                    }
+                    started = columns_before != 0 && (started || takes_part);
+                    __syncwarp();
+                }
+                columns_before = columns;
+                flags_before = flags;
+                if (columns == 0) {
+                    new_item = true;
+                    ++turn;
+                }
             }
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
         // ---- softmax: a row per thread
@@ -1240,7 +1161,14 @@ int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err == cudaSuccess && (dev >= 64 || ((prepared.load(std::memory_order_acquire) >> dev) & 1ull) == 0)) {
-        err = cudaFuncSetAttribute(window_tc_kernel<DP, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+        cudaFuncAttributes attr;
+        err = cudaFuncGetAttributes(&attr, window_tc_kernel<DP, NQ>);
+        if (err == cudaSuccess && attr.numRegs < C::LAUNCH_REGS) {
+            return CUBK_ERR_UNSUPPORTED;   // compiled to fewer registers than its groups of warps share out among themselves
+        }
+        if (err == cudaSuccess) {
+            err = cudaFuncSetAttribute(window_tc_kernel<DP, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+        }
         if (err == cudaSuccess && dev < 64) {
             prepared.fetch_or(1ull << dev, std::memory_order_release);
         }
@@ -1313,634 +1241,6 @@ int window_attention(const T *q, const T *k, const T *v, int64_t q_stride, int64
     return check_launch();
 }
 
-// ---------------------------------------------------------------- ring caches
-struct RingShape {
-    int batch, heads, kv_heads, dim;
-    int window, sinks;
-    float scale;
-    int64_t q_stride, kv_stride, context_stride;
-};
-
-__device__ __forceinline__ int ring_slot(int p, int window, int sinks) {
-    return p < sinks ? p : sinks + (p - sinks) % window;
-}
-
-// One (stream, head) per warp. The new token's key and value are read where they came from, never from the slot that the
-// warp of the group's first head writes.
-template <typename T>
-__global__ void __launch_bounds__(32 * kWindowRowWarps)
-window_step_rows_kernel(const T *q, const T *k, const T *v, const int32_t *positions, T *k_cache, T *v_cache, T *context, RingShape s) {
-    __shared__ float s_q[kWindowRowWarps][kWindowMaxDim];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t total = (int64_t) s.batch * s.heads;
-    const int slots = s.window + s.sinks, share = s.heads / s.kv_heads;
-    for (int64_t r = (int64_t) blockIdx.x * kWindowRowWarps + warp; r < total; r += (int64_t) gridDim.x * kWindowRowWarps) {
-        const int64_t b = r / s.heads;
-        const int h = (int) (r - b * s.heads), kh = h / share;
-        const int p = positions[b];
-        if (p < 0) {
-            continue;
-        }
-        const int slot = ring_slot(p, s.window, s.sinks);
-        const int n = p < slots ? p + 1 : slots;
-        const T *kn = k + b * s.kv_stride + (int64_t) kh * s.dim, *vn = v + b * s.kv_stride + (int64_t) kh * s.dim;
-        T *kc = k_cache + (b * s.kv_heads + kh) * slots * s.dim, *vc = v_cache + (b * s.kv_heads + kh) * slots * s.dim;
-        if (h == kh * share) {
-            for (int c = lane; c < s.dim; c += 32) {
-                kc[(int64_t) slot * s.dim + c] = kn[c];
-                vc[(int64_t) slot * s.dim + c] = vn[c];
-            }
-        }
-        window_row<T>(q + b * s.q_stride + (int64_t) h * s.dim, s_q[warp], s.dim, s.scale, 0, 0, n,
-                      [&](int j) { return j == slot ? kn : kc + (int64_t) j * s.dim; },
-                      [&](int j) { return j == slot ? vn : vc + (int64_t) j * s.dim; }, [&](int) { return true; },
-                      context + b * s.context_stride + (int64_t) h * s.dim);
-    }
-}
-
-// ---- single tokens, 16-byte rows: a cluster of blocks per (stream, kv head)
-// The keys of a stream are cut into blocks that the warps of the cluster take in turn, each with a softmax of its own over
-// what it took; at the end the blocks read one another's partial sums through distributed shared memory and every block
-// writes its share of the context. Nothing is staged in device memory, so calls need no workspace and no order among them,
-// and the sums are added in the same order every time. The kernel is bound by the cache's bytes.
-template <int WARPS, int HEADS, int DP>
-struct StepPartial {
-    float o[WARPS][HEADS][DP + 2];   // two columns of padding spread the rows over the banks
-    float2 stat[WARPS][HEADS];       // maximum (log2 domain) and sum
-};
-
-constexpr int kStepBlocks = 8;   // of a cluster at most
-
-// Parts (maximum, sum, weighted sum of values) joined into one; a part without keys has the sum 0 and counts for nothing.
-template <int N>
-__device__ __forceinline__ float3 join_parts(const float2 (&stat)[N], const float (&o)[N]) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        top = fmaxf(top, stat[i].x);
-    }
-    float sum = 0.f, total = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float weight = stat[i].x == -INFINITY ? 0.f : fast_exp2(stat[i].x - top);
-        if (stat[i].y != 0.f) {
-            total = fmaf(weight, stat[i].y, total);
-            sum = fmaf(weight, o[i], sum);
-        }
-    }
-    return make_float3(top, total, sum);
-}
-
-// First the warps of a block, in its own shared memory, then the blocks: each output element's parts are loaded together.
-template <typename T, int WARPS, int HEADS, int DP>
-__device__ __forceinline__ void step_join(StepPartial<WARPS, HEADS, DP> *part, int heads_here, int dim, T *out) {
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int blocks = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
-    constexpr int PER_THREAD = (HEADS * DP + 32 * WARPS - 1) / (32 * WARPS);
-    float3 joined[PER_THREAD];
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < PER_THREAD; ++u) {
-        const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
-        if (h < heads_here) {
-            float2 stat[WARPS];
-            float o[WARPS];
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                stat[w] = part->stat[w][h];
-                o[w] = part->o[w][h][x];
-            }
-            joined[u] = join_parts<WARPS>(stat, o);
-        }
-    }
-    if (blocks == 1) {
-#pragma unroll
-        for (int u = 0; u < PER_THREAD; ++u) {
-            const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
-            if (h < heads_here && x < dim) {
-                out[h * dim + x] = from_float<T>(joined[u].y == 0.f ? 0.f : joined[u].z / joined[u].y);
-            }
-        }
-        return;
-    }
-    __syncthreads();   // every warp's part has been read: the first one's place takes the block's
-#pragma unroll
-    for (int u = 0; u < PER_THREAD; ++u) {
-        const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
-        if (h < heads_here) {
-            part->o[0][h][x] = joined[u].z;
-            if (x == 0) {
-                part->stat[0][h] = make_float2(joined[u].x, joined[u].y);
-            }
-        }
-    }
-    cluster.sync();
-    for (int e = rank * (32 * WARPS) + threadIdx.x; e < heads_here * dim; e += blocks * 32 * WARPS) {
-        const int h = e / dim, x = e - h * dim;
-        float2 stat[kStepBlocks];
-        float o[kStepBlocks];
-#pragma unroll
-        for (int r = 0; r < kStepBlocks; ++r) {
-            stat[r] = make_float2(-INFINITY, 0.f);
-            o[r] = 0.f;
-            if (r < blocks) {
-                const StepPartial<WARPS, HEADS, DP> *from = cluster.map_shared_rank(part, r);
-                stat[r] = from->stat[0][h];
-                o[r] = from->o[0][h][x];
-            }
-        }
-        const float3 all = join_parts<kStepBlocks>(stat, o);
-        out[e] = from_float<T>(all.y == 0.f ? 0.f : all.z / all.y);
-    }
-    cluster.sync();   // nobody leaves while its sums are read
-}
-
-struct StepPlace {
-    int b, kh, first_head, heads_here, slot, n;
-    int worker, workers;   // this warp among the cluster's
-};
-
-template <int WARPS, int HEADS>
-__device__ __forceinline__ bool step_place(const int32_t *positions, const RingShape &s, int chunks, StepPlace &at) {
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int blocks = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
-    const int64_t unit = blockIdx.x / blocks;
-    const int share = s.heads / s.kv_heads;
-    const int chunk = (int) (unit % chunks);
-    const int64_t pair = unit / chunks;
-    at.b = (int) (pair / s.kv_heads);
-    at.kh = (int) (pair - (int64_t) at.b * s.kv_heads);
-    at.first_head = at.kh * share + chunk * HEADS;
-    at.heads_here = min(HEADS, share - chunk * HEADS);
-    const int p = positions[at.b];
-    if (p < 0) {
-        return false;
-    }
-    const int slots = s.window + s.sinks;
-    at.slot = ring_slot(p, s.window, s.sinks);
-    at.n = p < slots ? p + 1 : slots;
-    at.worker = rank * WARPS + (threadIdx.x >> 5);
-    at.workers = blocks * WARPS;
-    return true;
-}
-
-// The new token's row into its slot, by the first chunk's first block; the readers of the slot take the token's own row.
-template <typename T, int WARPS>
-__device__ __forceinline__ void step_store(const T *kn, const T *vn, T *kc, T *vc, const StepPlace &at, const RingShape &s) {
-    if (at.first_head == at.kh * (s.heads / s.kv_heads) && at.worker < WARPS) {
-        constexpr int E = 16 / (int) sizeof(T);
-        for (int c = threadIdx.x; c < s.dim / E; c += 32 * WARPS) {
-            reinterpret_cast<uint4 *>(kc + (int64_t) at.slot * s.dim)[c] = reinterpret_cast<const uint4 *>(kn)[c];
-            reinterpret_cast<uint4 *>(vc + (int64_t) at.slot * s.dim)[c] = reinterpret_cast<const uint4 *>(vn)[c];
-        }
-    }
-}
-
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
-    uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-    return d;
-}
-
-// Binary16: S^T = K.Q^T and O^T += V^T.P^T on warp-level matrix instructions, 16 keys x 8 NT heads a block of keys. Lane
-// (g, t) = (lane / 4, lane % 4) reads 16 bytes (chunk t, t + 4, ..) of the K rows g and g + 8: eight columns that are two steps
-// of the reduction, in an order that Q shares. Of V it reads chunk g (g + 8) of the rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and pairs
-// the halves of two rows: word i of a chunk is rows g and g + 8 of the i-th 16 output columns. So K and V go from memory to
-// operands with no stop in shared memory; P^T turns around in registers.
-template <int WARPS, int DP, int NT>
-__global__ void __launch_bounds__(32 * WARPS, (DP == 64 ? 16 : (NT == 1 ? 12 : 8)) / WARPS)
-window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const int32_t *positions, __half *k_cache, __half *v_cache,
-                       __half *context, const __grid_constant__ RingShape s, int chunks) {
-    constexpr int HEADS = 8 * NT, KC = DP / 32, VC = DP / 64;
-    __shared__ StepPartial<WARPS, HEADS, DP> part;
-    StepPlace at;
-    if (!step_place<WARPS, HEADS>(positions, s, chunks, at)) {
-        return;
-    }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int64_t slots = s.window + s.sinks;
-    const __half *kn = k + at.b * s.kv_stride + (int64_t) at.kh * s.dim, *vn = v + at.b * s.kv_stride + (int64_t) at.kh * s.dim;
-    __half *kc = k_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim, *vc = v_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim;
-    step_store<__half, WARPS>(kn, vn, kc, vc, at, s);
-
-    uint32_t qf[NT][KC][4];
-#pragma unroll
-    for (int m = 0; m < NT; ++m) {
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int col = 8 * (t + 4 * c), head = 8 * m + g;
-            uint4 r = make_uint4(0, 0, 0, 0);
-            if (head < at.heads_here && col < s.dim) {
-                r = ld_param(q + at.b * s.q_stride + (int64_t) (at.first_head + head) * s.dim + col);
-            }
-            qf[m][c][0] = r.x, qf[m][c][1] = r.y, qf[m][c][2] = r.z, qf[m][c][3] = r.w;
-        }
-    }
-    float o[NT][VC][4][4];
-    float top[NT][2], total[NT][2];
-#pragma unroll
-    for (int m = 0; m < NT; ++m) {
-        top[m][0] = top[m][1] = -INFINITY;
-        total[m][0] = total[m][1] = 0.f;
-#pragma unroll
-        for (int x = 0; x < VC; ++x) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                o[m][x][i][0] = o[m][x][i][1] = o[m][x][i][2] = o[m][x][i][3] = 0.f;
-            }
-        }
-    }
-    const float c2 = s.scale * kLog2e;
-    const int key_blocks = (at.n + 15) / 16;
-    for (int kb = at.worker; kb < key_blocks; kb += at.workers) {
-        const int j0 = kb * 16;
-        uint4 kr[2][KC], vr[4][VC];
-        const bool whole = j0 + 16 <= at.n && (at.slot < j0 || at.slot >= j0 + 16);
-        if (whole) {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const __half *row = kc + (int64_t) (j0 + g + 8 * r) * s.dim;
-#pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const int col = 8 * (t + 4 * c);
-                    kr[r][c] = col < s.dim ? ld_stream(row + col) : make_uint4(0, 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const __half *row = vc + (int64_t) (j0 + 2 * t + (r & 1) + 8 * (r >> 1)) * s.dim;
-#pragma unroll
-                for (int x = 0; x < VC; ++x) {
-                    const int col = 8 * (g + 8 * x);
-                    vr[r][x] = col < s.dim ? ld_stream(row + col) : make_uint4(0, 0, 0, 0);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int j = j0 + g + 8 * r;
-                const __half *row = j == at.slot ? kn : kc + (int64_t) j * s.dim;
-#pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    const int col = 8 * (t + 4 * c);
-                    kr[r][c] = j < at.n && col < s.dim ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0, 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = j0 + 2 * t + (r & 1) + 8 * (r >> 1);
-                const __half *row = j == at.slot ? vn : vc + (int64_t) j * s.dim;
-#pragma unroll
-                for (int x = 0; x < VC; ++x) {
-                    const int col = 8 * (g + 8 * x);
-                    vr[r][x] = j < at.n && col < s.dim ? *reinterpret_cast<const uint4 *>(row + col) : make_uint4(0, 0, 0, 0);
-                }
-            }
-        }
-        float sc[NT][4];
-#pragma unroll
-        for (int m = 0; m < NT; ++m) {
-            sc[m][0] = sc[m][1] = sc[m][2] = sc[m][3] = 0.f;
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                mma_f16(sc[m], kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, qf[m][c][0], qf[m][c][1]);
-                mma_f16(sc[m], kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, qf[m][c][2], qf[m][c][3]);
-            }
-        }
-        bool raise = false;
-#pragma unroll
-        for (int m = 0; m < NT; ++m) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {   // e: head 2 t + e % 2, key g + 8 (e / 2)
-                sc[m][e] = j0 + g + 8 * (e >> 1) < at.n ? sc[m][e] * c2 : -INFINITY;
-                raise = raise || sc[m][e] - top[m][e & 1] > kRaiseBy;
-            }
-        }
-        if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-            for (int m = 0; m < NT; ++m) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float here = fmaxf(fmaxf(sc[m][e], sc[m][e + 2]), top[m][e]);
-                    here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 4));
-                    here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 8));
-                    here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 16));
-                    const float shrink = top[m][e] == here ? 1.f : fast_exp2(top[m][e] - here);
-                    top[m][e] = here;
-                    total[m][e] *= shrink;
-#pragma unroll
-                    for (int x = 0; x < VC; ++x) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            o[m][x][i][e] *= shrink;
-                            o[m][x][i][e + 2] *= shrink;
-                        }
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < NT; ++m) {
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[e] = sc[m][e] == -INFINITY ? 0.f : fast_exp2(sc[m][e] - top[m][e & 1]);
-                total[m][e & 1] += p[e];
-            }
-            const __half2 lo = __floats2half2_rn(p[0], p[1]), hi = __floats2half2_rn(p[2], p[3]);
-            const uint32_t b0 = transpose_8x8(*reinterpret_cast<const uint32_t *>(&lo)), b1 = transpose_8x8(*reinterpret_cast<const uint32_t *>(&hi));
-#pragma unroll
-            for (int x = 0; x < VC; ++x) {
-                const uint32_t w0[4] = {vr[0][x].x, vr[0][x].y, vr[0][x].z, vr[0][x].w}, w1[4] = {vr[1][x].x, vr[1][x].y, vr[1][x].z, vr[1][x].w};
-                const uint32_t w2[4] = {vr[2][x].x, vr[2][x].y, vr[2][x].z, vr[2][x].w}, w3[4] = {vr[3][x].x, vr[3][x].y, vr[3][x].z, vr[3][x].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    mma_f16(o[m][x][i], __byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x5410),
-                            __byte_perm(w2[i], w3[i], 0x7632), b0, b1);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < NT; ++m) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float sum = total[m][e];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-            const int head = 8 * m + 2 * t + e;
-            if (g == 0) {
-                part.stat[warp][head] = make_float2(top[m][e], sum);
-            }
-#pragma unroll
-            for (int x = 0; x < VC; ++x) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    *reinterpret_cast<float2 *>(&part.o[warp][head][8 * (g + 8 * x) + 2 * i]) = make_float2(o[m][x][i][e], o[m][x][i][e + 2]);
-                }
-            }
-        }
-    }
-    step_join<__half, WARPS, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
-}
-
-// float32: LPK lanes share a key, four columns each, so that a warp reads 32 / LPK whole rows per instruction; every group of
-// lanes keeps a softmax of its own over its keys, HEADS heads at once.
-template <int WARPS, int LPK, int HEADS>
-__global__ void __launch_bounds__(32 * WARPS)
-window_step_f32_kernel(const float *q, const float *k, const float *v, const int32_t *positions, float *k_cache, float *v_cache, float *context,
-                       const __grid_constant__ RingShape s, int chunks) {
-    constexpr int DP = 4 * LPK, GROUPS = 32 / LPK, U = HEADS == 1 ? 8 : 4;   // U: rows per lane group in flight
-    __shared__ StepPartial<WARPS, HEADS, DP> part;
-    StepPlace at;
-    if (!step_place<WARPS, HEADS>(positions, s, chunks, at)) {
-        return;
-    }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LPK, col = 4 * (lane % LPK);
-    const int64_t slots = s.window + s.sinks;
-    const float *kn = k + at.b * s.kv_stride + (int64_t) at.kh * s.dim, *vn = v + at.b * s.kv_stride + (int64_t) at.kh * s.dim;
-    float *kc = k_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim, *vc = v_cache + ((int64_t) at.b * s.kv_heads + at.kh) * slots * s.dim;
-    step_store<float, WARPS>(kn, vn, kc, vc, at, s);
-    const bool mine = col < s.dim;
-    const float c2 = s.scale * kLog2e;
-    float4 qf[HEADS], o[HEADS];
-    float top[HEADS], total[HEADS];
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h) {
-        qf[h] = mine && h < at.heads_here
-                    ? __ldg(reinterpret_cast<const float4 *>(q + at.b * s.q_stride + (int64_t) (at.first_head + h) * s.dim + col))
-                    : make_float4(0.f, 0.f, 0.f, 0.f);
-        o[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-        top[h] = -INFINITY;
-        total[h] = 0.f;
-    }
-    const int per_block = GROUPS * U, key_blocks = (at.n + per_block - 1) / per_block;
-    for (int kb = at.worker; kb < key_blocks; kb += at.workers) {
-        float4 kr[U], vr[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int j = kb * per_block + u * GROUPS + group;
-            const float *krow = j == at.slot ? kn : kc + (int64_t) j * s.dim, *vrow = j == at.slot ? vn : vc + (int64_t) j * s.dim;
-            const bool in = mine && j < at.n;
-            kr[u] = in ? *reinterpret_cast<const float4 *>(krow + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-            vr[u] = in ? *reinterpret_cast<const float4 *>(vrow + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int h = 0; h < HEADS; ++h) {
-            float sc[U];
-            float here = top[h];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float d = fmaf(qf[h].x, kr[u].x, qf[h].y * kr[u].y) + fmaf(qf[h].z, kr[u].z, qf[h].w * kr[u].w);
-#pragma unroll
-                for (int m = LPK / 2; m > 0; m >>= 1) {
-                    d += __shfl_xor_sync(0xffffffffu, d, m);
-                }
-                sc[u] = kb * per_block + u * GROUPS + group < at.n ? d * c2 : -INFINITY;
-                here = fmaxf(here, sc[u]);
-            }
-            const float shrink = top[h] == here ? 1.f : fast_exp2(top[h] - here);
-            top[h] = here;
-            total[h] *= shrink;
-            o[h].x *= shrink, o[h].y *= shrink, o[h].z *= shrink, o[h].w *= shrink;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float p = sc[u] == -INFINITY ? 0.f : fast_exp2(sc[u] - here);
-                total[h] += p;
-                o[h].x = fmaf(p, vr[u].x, o[h].x);
-                o[h].y = fmaf(p, vr[u].y, o[h].y);
-                o[h].z = fmaf(p, vr[u].z, o[h].z);
-                o[h].w = fmaf(p, vr[u].w, o[h].w);
-            }
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < HEADS; ++h) {
-        float all = top[h];
-#pragma unroll
-        for (int m = LPK; m < 32; m <<= 1) {
-            all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, m));
-        }
-        const float shrink = top[h] == all ? 1.f : (top[h] == -INFINITY ? 0.f : fast_exp2(top[h] - all));
-        float r[5] = {total[h] * shrink, o[h].x * shrink, o[h].y * shrink, o[h].z * shrink, o[h].w * shrink};
-#pragma unroll
-        for (int m = LPK; m < 32; m <<= 1) {
-#pragma unroll
-            for (int i = 0; i < 5; ++i) {
-                r[i] += __shfl_xor_sync(0xffffffffu, r[i], m);
-            }
-        }
-        if (group == 0) {
-            if (lane == 0) {
-                part.stat[warp][h] = make_float2(all, r[0]);
-            }
-            *reinterpret_cast<float2 *>(&part.o[warp][h][col]) = make_float2(r[1], r[2]);
-            *reinterpret_cast<float2 *>(&part.o[warp][h][col + 2]) = make_float2(r[3], r[4]);
-        }
-    }
-    step_join<float, WARPS, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
-}
-
-// Blocks of a cluster: doubled until the grid has two blocks per SM, and on to about five while every warp keeps 6 KB of keys (below
-// that a block's start and join cost more than its share of the loads brings: 9 streams of 32 / 8 heads of 128 with 715 slots take 9.8 us
-// in clusters of four, 13.9 in eights; 16 of 12 heads of 64 with 1024 slots 13.1 in twos, 11.0 in fours).
-inline int step_cluster(int64_t units, int64_t slots, int64_t row_bytes) {
-    int blocks = 1;
-    while (blocks < kStepBlocks && slots > 64 * blocks) {
-        const int64_t grid = units * blocks * 2, warp_bytes = slots * row_bytes / (blocks * 2 * 4);
-        if (grid > 2 * 148 && (grid > 5 * 148 + 74 || warp_bytes < 6 * 1024)) {
-            break;
-        }
-        blocks *= 2;
-    }
-    return blocks;
-}
-
-template <typename T, int HEADS, typename Kernel>
-int step_launch(Kernel four, Kernel eight, bool has_eight, const T *q, const T *k, const T *v, const int32_t *positions, T *k_cache, T *v_cache, T *context,
-                const RingShape &s, cudaStream_t stream) {
-    const int chunks = (s.heads / s.kv_heads + HEADS - 1) / HEADS;
-    const int64_t units = (int64_t) s.batch * s.kv_heads * chunks, slots = (int64_t) s.window + s.sinks;
-    const int cluster = step_cluster(units, slots, (int64_t) s.dim * (int) sizeof(T));
-    if (units * cluster > 0x7fffffffLL) {
-        return CUBK_ERR_UNSUPPORTED;
-    }
-    // Eight warps a block where even full clusters leave half of the SMs without one: what a stream takes then is set by the loads an
-    // SM has in flight (one stream of 32 / 8 heads of 128 with 4096 slots: 13.6 us with four warps, 10.6 with eight; with blocks on most
-    // SMs four are the better: 4 streams of 16 / 4 heads, 14.2 against 17.0).
-    const bool wide = has_eight && units * cluster <= 74 && slots >= 128 * cluster;
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned) (units * cluster));
-    config.blockDim = dim3(wide ? 256 : 128);
-    config.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned) cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    config.attrs = &attr;
-    config.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&config, wide ? eight : four, q, k, v, positions, k_cache, v_cache, context, s, chunks);
-    if (err != cudaSuccess) {
-        (void) cudaGetLastError();
-        set_last_error(err);
-        return CUBK_ERR_LAUNCH;
-    }
-    return CUBK_OK;
-}
-
-// Rows and heads that start on 16-byte boundaries, head dimension up to 128.
-inline int step_vectors(const __half *q, const __half *k, const __half *v, const int32_t *positions, __half *k_cache, __half *v_cache,
-                        __half *context, const RingShape &s, cudaStream_t stream) {
-    const int share = s.heads / s.kv_heads;
-    // the parts of eight warps with 16 heads of 128 do not fit a block's static shared memory
-#define STEP_F16(DP, NT)                                                                                                                  \
-    step_launch<__half, 8 * NT>(window_step_f16_kernel<4, DP, NT>, window_step_f16_kernel<DP * NT == 256 ? 4 : 8, DP, NT>, DP * NT < 256, q, \
-                                k, v, positions, k_cache, v_cache, context, s, stream)
-    if (s.dim <= 64) {
-        return share <= 8 ? STEP_F16(64, 1) : STEP_F16(64, 2);
-    }
-    return share <= 8 ? STEP_F16(128, 1) : STEP_F16(128, 2);
-#undef STEP_F16
-}
-
-inline int step_vectors(const float *q, const float *k, const float *v, const int32_t *positions, float *k_cache, float *v_cache, float *context,
-                        const RingShape &s, cudaStream_t stream) {
-    const int share = s.heads / s.kv_heads;
-#define STEP_F32(LPK, HEADS)                                                                                                             \
-    step_launch<float, HEADS>(window_step_f32_kernel<4, LPK, HEADS>, window_step_f32_kernel<8, LPK, HEADS>, true, q, k, v, positions,   \
-                              k_cache, v_cache, context, s, stream)
-    if (share == 1) {
-        return s.dim <= 32 ? STEP_F32(8, 1) : s.dim <= 64 ? STEP_F32(16, 1) : STEP_F32(32, 1);
-    }
-    return s.dim <= 32 ? STEP_F32(8, 4) : s.dim <= 64 ? STEP_F32(16, 4) : STEP_F32(32, 4);
-#undef STEP_F32
-}
-
-template <typename T>
-int window_attention_step(const T *q, const T *k, const T *v, int64_t q_stride, int64_t kv_stride, const int32_t *positions, int batch,
-                          int heads, int kv_heads, int dim, int window, int sinks, float scale, T *k_cache, T *v_cache, T *context,
-                          int64_t context_stride, cudaStream_t stream) {
-    if (q == nullptr || k == nullptr || v == nullptr || positions == nullptr || k_cache == nullptr || v_cache == nullptr ||
-        context == nullptr || batch < 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || window <= 0 || sinks < 0 || heads % kv_heads != 0 ||
-        q_stride < (int64_t) heads * dim || kv_stride < (int64_t) kv_heads * dim || context_stride < (int64_t) heads * dim) {
-        return CUBK_ERR_INVALID_ARG;
-    }
-    if (dim > kWindowMaxDim || window > 0x3fffffff || sinks > 0x3fffffff) {
-        return CUBK_ERR_UNSUPPORTED;
-    }
-    if (batch == 0) {
-        return CUBK_OK;
-    }
-    const RingShape s = {batch, heads, kv_heads, dim, window, sinks, scale, q_stride, kv_stride, context_stride};
-    constexpr int E = 16 / (int) sizeof(T);
-    if (dim <= 128 && dim % E == 0 && q_stride % E == 0 && kv_stride % E == 0 && aligned16(q) && aligned16(k) && aligned16(v) &&
-        aligned16(k_cache) && aligned16(v_cache)) {
-        const int rc = step_vectors(q, k, v, positions, k_cache, v_cache, context, s, stream);
-        if (rc != CUBK_ERR_UNSUPPORTED) {
-            return rc;
-        }
-    }
-    const int64_t groups = ((int64_t) batch * heads + kWindowRowWarps - 1) / kWindowRowWarps;
-    const unsigned blocks = (unsigned) (groups < 148 * 64 ? groups : 148 * 64);
-    window_step_rows_kernel<T><<<blocks, 32 * kWindowRowWarps, 0, stream>>>(q, k, v, positions, k_cache, v_cache, context, s);
-    return check_launch();
-}
-
-// Keys and values of a prompt's last tokens (and its sinks) into the ring: one warp per (token, kv head). Of the tokens that
-// share a slot only the last is written, so no two warps write the same row.
-template <typename T>
-__global__ void __launch_bounds__(256)
-window_cache_fill_kernel(const T *k, const T *v, int64_t kv_stride, const int32_t *lengths, int batch, int seq, int kv_heads, int dim,
-                         int window, int sinks, T *k_cache, T *v_cache) {
-    const int lane = threadIdx.x & 31;
-    const int slots = window + sinks;
-    const int64_t total = (int64_t) batch * seq * kv_heads;
-    for (int64_t r = (int64_t) blockIdx.x * 8 + (threadIdx.x >> 5); r < total; r += (int64_t) gridDim.x * 8) {
-        const int64_t token = r / kv_heads;
-        const int kh = (int) (r - token * kv_heads);
-        const int64_t b = token / seq;
-        const int j = (int) (token - b * seq);
-        const int length = lengths != nullptr ? min(lengths[b], seq) : seq;
-        if (j >= length || (j >= sinks && j < length - window)) {
-            continue;
-        }
-        const int64_t to = ((b * kv_heads + kh) * slots + ring_slot(j, window, sinks)) * dim, from = token * kv_stride + (int64_t) kh * dim;
-        for (int c = lane; c < dim; c += 32) {
-            k_cache[to + c] = k[from + c];
-            v_cache[to + c] = v[from + c];
-        }
-    }
-}
-
-template <typename T>
-int window_cache_fill(const T *k, const T *v, int64_t kv_stride, const int32_t *lengths, int batch, int seq, int kv_heads, int dim,
-                      int window, int sinks, T *k_cache, T *v_cache, cudaStream_t stream) {
-    if (k == nullptr || v == nullptr || k_cache == nullptr || v_cache == nullptr || batch < 0 || seq < 0 || kv_heads <= 0 || dim <= 0 ||
-        window <= 0 || sinks < 0 || kv_stride < (int64_t) kv_heads * dim) {
-        return CUBK_ERR_INVALID_ARG;
-    }
-    if (dim > kWindowMaxDim || window > 0x3fffffff || sinks > 0x3fffffff) {
-        return CUBK_ERR_UNSUPPORTED;
-    }
-    if (batch == 0 || seq == 0) {
-        return CUBK_OK;
-    }
-    const int64_t groups = ((int64_t) batch * seq * kv_heads + 7) / 8;
-    const unsigned blocks = (unsigned) (groups < 148 * 32 ? groups : 148 * 32);
-    window_cache_fill_kernel<T><<<blocks, 256, 0, stream>>>(k, v, kv_stride, lengths, batch, seq, kv_heads, dim, window, sinks, k_cache,
-                                                            v_cache);
-    return check_launch();
-}
-
 }  // namespace cubk
 
 extern "C" {
@@ -1958,33 +1258,6 @@ int cubk_window_attention_f16(const void *q, const void *k, const void *v, int64
     return cubk::window_attention<__half>((const __half *) q, (const __half *) k, (const __half *) v, q_stride, kv_stride, mask, batch, seq,
                                           heads, kv_heads, head_dim, before, after, sinks, scale, (__half *) context, context_stride,
                                           (cudaStream_t) stream);
-}
-
-int cubk_window_attention_step_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride,
-                                   const int32_t *positions, int batch, int heads, int kv_heads, int head_dim, int window, int sinks,
-                                   float scale, float *k_cache, float *v_cache, float *context, int64_t context_stride, void *stream) {
-    return cubk::window_attention_step<float>(q, k, v, q_stride, kv_stride, positions, batch, heads, kv_heads, head_dim, window, sinks,
-                                              scale, k_cache, v_cache, context, context_stride, (cudaStream_t) stream);
-}
-
-int cubk_window_attention_step_f16(const void *q, const void *k, const void *v, int64_t q_stride, int64_t kv_stride,
-                                   const int32_t *positions, int batch, int heads, int kv_heads, int head_dim, int window, int sinks,
-                                   float scale, void *k_cache, void *v_cache, void *context, int64_t context_stride, void *stream) {
-    return cubk::window_attention_step<__half>((const __half *) q, (const __half *) k, (const __half *) v, q_stride, kv_stride, positions,
-                                               batch, heads, kv_heads, head_dim, window, sinks, scale, (__half *) k_cache,
-                                               (__half *) v_cache, (__half *) context, context_stride, (cudaStream_t) stream);
-}
-
-int cubk_window_cache_fill_f32(const float *k, const float *v, int64_t kv_stride, const int32_t *lengths, int batch, int seq, int kv_heads,
-                               int head_dim, int window, int sinks, float *k_cache, float *v_cache, void *stream) {
-    return cubk::window_cache_fill<float>(k, v, kv_stride, lengths, batch, seq, kv_heads, head_dim, window, sinks, k_cache, v_cache,
-                                          (cudaStream_t) stream);
-}
-
-int cubk_window_cache_fill_f16(const void *k, const void *v, int64_t kv_stride, const int32_t *lengths, int batch, int seq, int kv_heads,
-                               int head_dim, int window, int sinks, void *k_cache, void *v_cache, void *stream) {
-    return cubk::window_cache_fill<__half>((const __half *) k, (const __half *) v, kv_stride, lengths, batch, seq, kv_heads, head_dim,
-                                           window, sinks, (__half *) k_cache, (__half *) v_cache, (cudaStream_t) stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,88 @@
+// One query row of windowed attention per warp: what every shape and alignment falls back to, and what computes rows again
+// that came out not finite.
+#pragma once
+
+#include "common.cuh"
+
+namespace cubk {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaiseBy = 8.f;   // log2 of the largest weight before a running maximum is raised
+constexpr int kWindowMaxDim = 256;
+constexpr int kWindowRowWarps = 4;
+
+// Any head dimension up to 256, any strides: 32 keys at a time, a key per lane for the scores, a column (or several)
+// per lane for the context. `key(j)` and `value(j)` give the addresses of row j, `seen(j)` says whether it counts.
+template <typename T, typename Key, typename Value, typename Seen>
+__device__ void window_row(const T *q, float *s_q, int dim, float scale, int sinks_end, int lo, int hi, Key key, Value value, Seen seen,
+                           T *context) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    for (int c = lane; c < dim; c += 32) {
+        s_q[c] = to_float<T>(q[c]);
+    }
+    __syncwarp();
+    float o[kWindowMaxDim / 32];
+#pragma unroll
+    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+        o[i] = 0.f;
+    }
+    float top = -INFINITY, total = 0.f;
+    for (int part = 0; part < 2; ++part) {
+        const int begin = part == 0 ? 0 : lo, end = part == 0 ? sinks_end : hi;
+        for (int j0 = begin; j0 < end; j0 += 32) {
+            const int j = j0 + lane;
+            const bool use = j < end && seen(j);
+            float s = -INFINITY;
+            if (use) {
+                const T *kr = key(j);
+                float a0 = 0.f, a1 = 0.f;
+                int c = 0;
+                for (; c + 1 < dim; c += 2) {
+                    a0 = fmaf(s_q[c], to_float<T>(kr[c]), a0);
+                    a1 = fmaf(s_q[c + 1], to_float<T>(kr[c + 1]), a1);
+                }
+                if (c < dim) {
+                    a0 = fmaf(s_q[c], to_float<T>(kr[c]), a0);
+                }
+                s = scale * kLog2e * (a0 + a1);
+            }
+            unsigned visible = __ballot_sync(0xffffffffu, use);
+            const float next = fmaxf(top, group_max<32>(s));
+            if (visible == 0 || next == -INFINITY) {
+                if (!__any_sync(0xffffffffu, use && !(s == -INFINITY))) {   // a NaN score goes on below
+                    continue;
+                }
+            }
+            const float shrink = top == -INFINITY ? 0.f : fast_exp2(top - next);
+            const float p = use ? fast_exp2(s - next) : 0.f;
+            top = next;
+            total = total * shrink + group_sum<32>(p);
+#pragma unroll
+            for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+                o[i] *= shrink;
+            }
+            while (visible != 0) {
+                const int from = __ffs(visible) - 1;
+                visible &= visible - 1;
+                const float w = __shfl_sync(0xffffffffu, p, from);
+                const T *vr = value(j0 + from);
+#pragma unroll
+                for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+                    if (lane + 32 * i < dim) {
+                        o[i] = fmaf(w, to_float<T>(vr[lane + 32 * i]), o[i]);
+                    }
+                }
+            }
+        }
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+        if (lane + 32 * i < dim) {
+            context[lane + 32 * i] = from_float<T>(o[i] * inv);
+        }
+    }
+}
+
+}  // namespace cubk

@@ -7,6 +7,10 @@ by at most n 2^-24 of the sum of their magnitudes, a sum on the tensor cores by 
 additions may cut instead of round).
 """
 import math
+import os
+import random
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -574,6 +578,57 @@ def test_cache_fill_writes_the_named_slots_only(t):
     assert torch.equal(vc, v.reshape(batch, seq, kv_heads, dim).permute(0, 2, 1, 3))
 
 
+@pytest.mark.parametrize("seed", range(48))
+def test_window_attention_of_random_shapes(seed):
+    r = random.Random(seed)
+    t = TYPES[seed % 2]
+    dim = r.choice([8, 16, 24, 32, 40, 64, 64, 72, 96, 128, 128, 50])
+    kv_heads = r.choice([1, 2, 3])
+    heads = kv_heads * r.choice([1, 2, 3, 4])
+    seq = r.choice([1, 2, 15, 16, 17, 63, 64, 65, 79, 81, 127, 128, 129, 255, 257, 300, 511, 700])
+    batch = r.choice([1, 2, 3])
+    before, after = r.choice([0, 1, 15, 16, 17, 100, 127, 128, 1000]), r.choice([0, 0, 1, 15, 64, 128, 1000])
+    sinks = r.choice([0, 1, 4, 15, 16, 17, 33, 129, 300])
+    q, k, v, m = window_inputs(seed, batch, seq, heads, kv_heads, dim, r.choice([None, "prefix", "holes"]), t, r.choice([0, 0, 8]))
+    args = (batch, seq, heads, kv_heads, dim, before, after, sinks, r.choice([dim ** -0.5, 1.0, 0.01]))
+    check_window(window_attention(q, k, v, m, *args, t), window64(q, k, v, m, *args), t, str((args, m is not None)))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_window_attention_step_beyond_32_bit_offsets(t):
+    """A cache of more than 2^31 elements: the last stream's last head is where it should be."""
+    batch, heads, kv_heads, dim, window, sinks = 3, 4, 2, 128, 2900000, 4
+    slots = window + sinks
+    assert batch * kv_heads * slots * dim > 2 ** 31
+    dt = G.TORCH_DTYPE[t]
+    kc, vc = torch.zeros((batch, kv_heads, slots, dim), dtype=dt, device="cuda"), torch.zeros((batch, kv_heads, slots, dim), dtype=dt, device="cuda")
+    g = gen(4)
+    pos = torch.tensor([-1, 3, 10 * slots + 7], dtype=torch.int32, device="cuda")
+    at = sinks + (10 * slots + 7 - sinks) % window
+    kc[2, 1, -500:], vc[2, 1, -500:] = normal(g, 500, dim, t=t), normal(g, 500, dim, t=t)
+    kc[2, :, :, 0] = -8.0                                        # the other slots count for little
+    kc[2, 1, -500:, 0] = 8.0
+    qkv = normal(g, batch, (heads + 2 * kv_heads) * dim, t=t)
+    q, k, v = (a.clone() for a in (qkv[:, :heads * dim], qkv[:, heads * dim:(heads + kv_heads) * dim], qkv[:, (heads + kv_heads) * dim:]))
+    q[2].view(heads, dim)[:, 0] = 8.0
+    k[2].view(kv_heads, dim)[:, 0] = 8.0
+    ctx = torch.zeros((batch, heads * dim), dtype=dt, device="cuda")
+    step(q, k, v, pos, batch, heads, kv_heads, dim, window, sinks, dim ** -0.5, kc, vc, ctx, t)
+    assert torch.equal(kc[2, :, at], k[2].view(kv_heads, dim)) and torch.equal(vc[2, 1, at], v[2].view(kv_heads, dim)[1])
+    # scores away from the last 500 slots are exactly -64 / sqrt(128): their weights are counted, not listed
+    s = torch.cat((kc[2, 1, -500:], kc[2, 1, at:at + 1])).double() @ q[2].view(heads, dim)[2:].double().t() * dim ** -0.5      # [501, 2]
+    others = slots - 501
+    top = s.amax(0)
+    w = torch.exp(s - top)
+    total = w.sum(0) + others * torch.exp(-64 * dim ** -0.5 - top)
+    want = (w.t() @ torch.cat((vc[2, 1, -500:], vc[2, 1, at:at + 1])).double()) / total[:, None]
+    got = ctx[2].view(heads, dim)[2:].double()
+    # weights and values of the few that count, as in check_window; the sums take in 2.9 million equal terms
+    bar = (2.0 ** -10 if t == "f16" else 2.0 ** -16) * (w.t() @ torch.cat((vc[2, 1, -500:], vc[2, 1, at:at + 1])).double().abs() / total[:, None])
+    assert at < slots - 500 and bool(((got - want).abs() <= bar + 1e-6).all())
+    assert float(ctx[0].abs().max()) == 0 and torch.isfinite(ctx.float()).all()
+
+
 # ============================================================================ together, streams, graphs
 
 class Layer:
@@ -675,3 +730,58 @@ def test_captured_layers_share_nothing_and_replay(t):
             for name in ("out", "res", "kc", "vc"):
                 assert torch.equal(getattr(eager[i], name), getattr(caught[i], name)), (turn, i, name)
     del graphs
+
+
+FIRST_CALLS = """
+import sys, torch
+sys.path.insert(0, %r)
+sys.path.insert(0, %r)
+import test_norm_w4_window_gpu as M
+torch.cuda.init()
+g = M.gen(1)
+work = []
+for t in M.TYPES:
+    for dim in (64, 128, 48, 5):
+        q, k, v, m = M.window_inputs(dim, 2, 200, 4, 2, dim, "holes", t)
+        args = (2, 200, 4, 2, dim, 40, 9, 3, 0.2)
+        ctx = torch.zeros((400, 4 * dim), dtype=q.dtype, device="cuda")
+        work.append((lambda q=q, k=k, v=v, m=m, args=args, t=t, ctx=ctx: M.window_attention(q, k, v, m, *args, t, ctx=ctx), ctx))
+        kc, vc = torch.zeros((3, 2, 70, dim), dtype=q.dtype, device="cuda"), torch.zeros((3, 2, 70, dim), dtype=q.dtype, device="cuda")
+        c2, pos = torch.zeros((3, 4 * dim), dtype=q.dtype, device="cuda"), torch.tensor([5, 69, 700], dtype=torch.int32, device="cuda")
+        work.append((lambda q=q, k=k, v=v, kc=kc, vc=vc, c2=c2, pos=pos, dim=dim, t=t: M.step(q[:3], k[:3], v[:3], pos, 3, 4, 2, dim, 66, 4, 0.2, kc, vc, c2, t), c2))
+    for n, k in ((40, 300), (2000, 1024)):
+        for rows in (1, 12, 40):
+            packed = M.pack(torch.randint(-8, 8, (n, k), generator=g, device="cuda", dtype=torch.int8))
+            scales, x = M.normal(g, -(-k // 64), n, t=t), M.normal(g, rows, k, t=t)
+            out = torch.zeros((rows, n), dtype=x.dtype, device="cuda")
+            work.append((lambda x=x, packed=packed, scales=scales, n=n, t=t, out=out: M.matvec(x, packed, scales, 64, n, None, t, out=out), out))
+    for ch in (64, 1024, 1001, 9000):
+        x = M.normal(g, 7, ch, t=t)
+        total, out = torch.zeros_like(x), torch.zeros_like(x)
+        work.append((lambda x=x, total=total, out=out, t=t: M.rms_norm(x, None, x[0], 1e-6, t, total=total, out=out), out))
+torch.cuda.synchronize()
+s = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=s):       # the process's first call of each kernel
+    for f, _ in work:
+        f()
+for _, out in work:
+    out.zero_()
+graph.replay()
+torch.cuda.synchronize()
+caught = [out.clone() for _, out in work]
+for f, _ in work:
+    f()
+torch.cuda.synchronize()
+assert all(torch.equal(a, out) for a, (_, out) in zip(caught, work))
+assert all(bool((a != 0).any()) for a in caught)
+del graph
+print("FIRST CALLS CAPTURED")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    here = os.path.dirname(os.path.abspath(__file__))
+    run = subprocess.run([sys.executable, "-c", FIRST_CALLS % (here, os.path.dirname(here))], stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                         text=True, timeout=300)
+    assert run.returncode == 0 and "FIRST CALLS CAPTURED" in run.stdout, run.stdout[-3000:]
