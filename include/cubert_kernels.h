@@ -20,7 +20,8 @@
  *   - A fast path is taken when pointers are 16-byte aligned and the row length is a
  *     multiple of 16 bytes; any other shape or alignment runs a slower generic kernel
  *     with identical results.
- *   - `stream` is a `cudaStream_t` passed as `void *` (as the reference does).
+ *   - `stream` is a `cudaStream_t` passed as `void *` (as the reference does). The stream and every buffer belong to
+ *     the device that is current on the calling thread.
  */
 #ifndef CUBERT_KERNELS_H
 #define CUBERT_KERNELS_H
@@ -303,7 +304,7 @@ int cubk_residual_rms_norm_e4m3_f16(const void *x, const void *residual, const v
  * whose products are float32 or binary16 library calls (src/cuBERT/op/Dense.cpp:41-52). Any number of rows is
  * computed; from about a hundred on, a library product on unpacked weights is the better call.
  * x [rows, k], bias [n] (or NULL), out [rows, n] and the scales [ceil(k / group), n] in the storage type. Sums are
- * float32; a code times its scale is never rounded.
+ * float32; a code times its scale is never rounded. out must not overlap the operands.
  * The _e4m3 calls take x as the 8-bit codes and scales K6 writes: code_scales [rows] (code_group = 0) or
  * [rows, ceil(k / 128)] (code_group = 128).
  * packed: cubk_w4_packed_bytes(n, k) bytes on a 16-byte boundary and scales on a 4-byte one (CUBK_ERR_UNSUPPORTED
@@ -338,7 +339,12 @@ int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int cod
  * Token s of sequence b is row b * seq + s of q, k, v and context; rows are q_stride (q), kv_stride (k and v) and
  * context_stride elements apart, so the three may be parts of one projection's output. Head h of a row is at column
  * h * head_dim and reads key/value head h / (heads / kv_heads); heads must be a multiple of kv_heads. head_dim is 1
- * to 256 (CUBK_ERR_UNSUPPORTED beyond). mask int8 [batch, seq]. context must not overlap the inputs. */
+ * to 256 (CUBK_ERR_UNSUPPORTED beyond). mask int8 [batch, seq]. context must not overlap the inputs.
+ *   _f16, head_dim a multiple of 8 up to 128, q, k, v on 16-byte boundaries, strides multiples of 8, scale > 0: tcgen05 with
+ *     scores, weights and contexts in tensor memory; weights are rounded to binary16. Every wait is bounded (0.2 s): a
+ *     block that gives up writes NaN into the rows it has not finished.
+ *   otherwise, head_dim up to 128: the float32 pipes, 64 x 64 tiles.
+ *   head_dim above 128: one row per warp. */
 int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
                               int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,
                               float *context, int64_t context_stride, void *stream);
