@@ -480,4 +480,11 @@ __device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &f) {
     return (t + ((n - t) >> 1)) >> (f.shift - 1);
 }
 
+// The larger of two values; NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 }  // namespace cubk

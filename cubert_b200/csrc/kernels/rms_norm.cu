@@ -13,13 +13,6 @@ constexpr float kE4m3Max = 448.f;
 // A group whose largest |y| is below this is stored as zeros with scale 0: 448 / max|y| must stay finite.
 constexpr float kTinyGroup = 7.888609e-31f;   // 2^-100
 
-// The larger of two values; NaN if either is (a row that holds a NaN must not come out as zeros).
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // Two float32 values to e4m3, round to nearest even, beyond +-448 to +-448; `lo` in the low byte.
 __device__ __forceinline__ uint16_t e4m3_pair(float lo, float hi) {
     uint16_t d;

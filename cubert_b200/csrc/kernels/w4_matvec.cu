@@ -568,7 +568,8 @@ __device__ __forceinline__ uint32_t w4_word(const int (&c)[8]) {
     return w;
 }
 
-// Codes by rounding to nearest even under the group's scale = max|w| / 7, rounded to the storage type first.
+// Codes by rounding to nearest even under the group's scale = max|w| / 7, rounded to the storage type first. A group that holds a NaN
+// or an infinity gets a scale that is not finite and codes 0, so that its products are NaN.
 template <typename T>
 __global__ void __launch_bounds__(256)
 w4_quantize_kernel(const T *weights, int n, int k, int group, int kblocks, int64_t words, uint32_t *packed, T *scales) {
@@ -584,17 +585,17 @@ w4_quantize_kernel(const T *weights, int n, int k, int group, int kblocks, int64
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         v[e] = row < n && k0 + e < k ? to_float<T>(weights[(size_t) row * k + k0 + e]) : 0.f;
-        top = fmaxf(top, fabsf(v[e]));
+        top = max_nan(top, fabsf(v[e]));
     }
     for (int o = 1; o < group / 8; o <<= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
     const T stored = from_float<T>(top / 7.f);
     const float scale = to_float<T>(stored);
     int c[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float q = scale > 0.f ? rintf(v[e] / scale) : 0.f;
+        const float q = scale > 0.f && scale < INFINITY ? rintf(v[e] / scale) : 0.f;
         c[e] = (int) fminf(fmaxf(q, -8.f), 7.f);
     }
     packed[w4_word_index(row, wc, kblocks)] = w4_word(c);

@@ -308,12 +308,14 @@ int cubk_residual_rms_norm_e4m3_f16(const void *x, const void *residual, const v
  * The _e4m3 calls take x as the 8-bit codes and scales K6 writes: code_scales [rows] (code_group = 0) or
  * [rows, ceil(k / 128)] (code_group = 128).
  * packed: cubk_w4_packed_bytes(n, k) bytes on a 16-byte boundary and scales on a 4-byte one (CUBK_ERR_UNSUPPORTED
- * otherwise; k and n up to 2^30), laid out once by one of the calls below, in tiles of 16 rows x 128 columns (1 KB), those of the same 16 rows next to each other. Row
- * r of a tile is 16 little-endian 32-bit words from byte 64 r; word 4 t + j holds columns 32 j + 8 t .. + 7, column
- * 2 i of them in bits 4 i .. 4 i + 3 and column 2 i + 1 in bits 16 + 4 i .. 16 + 4 i + 3, as code + 8. Rows and columns
- * past the matrix hold code 0 (8).
+ * otherwise; k and n up to 2^30), laid out once by one of the calls below, in tiles of 16 rows x 128 columns (1 KB),
+ * those of the same 16 rows next to each other. Row r of a tile is 16 little-endian 32-bit words from byte 64 r; word
+ * 4 t + j holds columns 32 j + 8 t .. + 7, column 2 i of them in bits 4 i .. 4 i + 3 and column 2 i + 1 in bits
+ * 16 + 4 i .. 16 + 4 i + 3, as code + 8. Rows and columns past the matrix hold code 0 (8).
  *   cubk_w4_quantize_*  rounds weights [n, k] to codes: scale = max|w| / 7 over a group of a row, rounded to the
- *                       storage type; code = w / scale to the nearest whole number (a tie to the even one)
+ *                       storage type; code = w / scale to the nearest whole number (a tie to the even one), at
+ *                       most 7 and at least -8; a NaN or an infinity in a group makes its scale NaN or infinite,
+ *                       its codes 0 and so its products NaN
  *   cubk_w4_pack        takes codes [n, k], one int8 in -8..7 each, from elsewhere */
 size_t cubk_w4_packed_bytes(int n, int k);
 int cubk_w4_quantize_f32(const float *weights, int n, int k, int group, void *packed, float *scales, void *stream);

@@ -302,6 +302,42 @@ def test_w4_matvec_not_finite_rows_and_buffers(t):
     assert ok_x() and ok_out() and ok_p()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_w4_quantize_keeps_nan_and_infinities(group, t):
+    """A weight that is not finite must not come out as a plausible code: its group's products are NaN, the others what they were."""
+    g = gen(group)
+    n, k, rows = 37, 300, 3
+    w = normal(g, n, k, std=0.02, t=t)
+    x = normal(g, rows, k, t=t)
+    hit = {(2, 5): float("nan"), (17, 299): float("inf"), (36, 130): float("-inf"), (20, 0): float("nan")}
+
+    def quantized():
+        packed = torch.empty(kernels.load().cubk_w4_packed_bytes(n, k), dtype=torch.uint8, device="cuda")
+        scales = torch.zeros((-(-k // group), n), dtype=w.dtype, device="cuda")
+        kernels.check(G.fn("w4_quantize", t)(G.ptr(w), n, k, group, G.ptr(packed), G.ptr(scales), G.stream()))
+        return packed, scales
+
+    packed, scales = quantized()
+    clean, clean_codes = matvec(x, packed, scales, group, n, None, t), unpack(packed, n, k)[:n, :k]
+    for (r, c), v in hit.items():
+        w[r, c] = v
+    packed, got = quantized()
+    codes = unpack(packed, n, k)[:n, :k]
+    same = np.ones((n, k), bool)
+    for (r, c), v in hit.items():
+        first = c // group * group
+        assert not torch.isfinite(got[c // group, r]) and torch.isnan(got[c // group, r]).item() == math.isnan(v)
+        assert not codes[r, first:first + group].any()
+        got[c // group, r] = scales[c // group, r]
+        same[r, first:first + group] = False
+    assert torch.equal(got, scales) and np.array_equal(codes[same], clean_codes[same])
+    packed, scales = quantized()
+    out = matvec(x, packed, scales, group, n, None, t)
+    rest = [r for r in range(n) if r not in {r for r, _ in hit}]
+    assert torch.isnan(out[:, sorted({r for r, _ in hit})]).all() and torch.equal(out[:, rest], clean[:, rest])
+
+
 # ============================================================================ K8
 
 def window_attention(q, k, v, mask, batch, seq, heads, kv_heads, dim, before, after, sinks, scale, t, ctx=None):
