@@ -351,18 +351,25 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 //     all masked is left out; one that every row of a tile sees whole skips the masking.
 //   * The running maximum of a row is raised only when a step's maximum exceeds it by 2^8 (a weight is then at most 256, far
 //     inside binary16, and the sums are float32), so that O is read back and scaled in few steps.
-//   * Weights of unseen keys are exactly 0, but 0 times an infinity or NaN in an unseen V row is NaN: a row that comes out not
-//     finite is computed again by one warp over its visible keys alone.
+//   * Weights of unseen keys are exactly 0, but 0 times an infinity or NaN in an unseen V row is NaN. V rows of masked keys, and of
+//     those outside the item's keys, are cleared in shared memory while the weights are awaited. That leaves keys that some rows of a
+//     tile see and others do not: a row that comes out not finite from finite scores is computed again by one warp over its visible
+//     keys alone (a visible score of infinity or NaN makes the row NaN as it is). That takes long, and others wait for the warp
+//     with bounded waits, so it happens behind the block's last item, and a block with such rows takes over no more items.
 // Bound by the softmax: per 128 x 128 tile the exponentials take 1024 cycles of an SM's special-function unit and the products 512 of
 // its tensor cores (heads of 64; 1024 for heads of 128), a step 1500. Measured: 8192 tokens, 32 / 8 heads of 128, window 2048: 265 to
 // 290 us by the clock under the power cap (840 to 910 TFLOP/s); 4 x 4096 tokens, 16 heads of 64, no window 400 us, window 513 and ragged
-// lengths 85 us (5 steps an item: half of that goes into the ends of items). Tried and slower: two threads a row, part of the
+// lengths 86 us (3 steps an item that ran: half of that goes into the ends of items; without clearing unseen V rows 84). A row computed
+// again reads its keys two bytes at a time: 40000 rows of 2 heads over 20000 keys each take about half a second. Tried and slower: two threads a row, part of the
 // exponentials by polynomial, scores of 96 keys twice, masks gathered by a warp of their own.
 // Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, frees its tensor memory and
 // returns.
 constexpr int kTileRows = 128;
 constexpr int kHalfTileBytes = kTileRows * 128;    // 128 rows x 64 binary16
 constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 2
+// Items of a warp with rows to compute again. The queries of item X are loaded once every warp has read the last scores of item X - 2, and
+// so has noted the rows of item X - 4; the next item is asked for after that. With the first such rows in item T, none follows T + 4.
+constexpr int kAgainItems = 8;
 
 struct WindowStep {
     int item, j0;
@@ -386,7 +393,7 @@ struct WindowTc {
     static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
     // The context's rows leave through the place of the item's queries by TMA, or as 16-byte stores from registers. TMA holds the queries
     // of the item after the next back until they have left: 8192 tokens, 32 heads of 128: 265 us against 277, but 4 x 4096 tokens, 16
-    // heads of 64, window 513, whose items are short: 88 against 84.
+    // heads of 64, window 513, whose items are short: 88 against 84 before unseen V rows were cleared.
     static constexpr bool ROWS_BY_TMA = NQ == 2;
     static constexpr int LAUNCH_REGS = NQ == 1 ? 128 : 168, SOFTMAX_REGS = NQ == 1 ? 192 : 224, OTHER_REGS = 56;
     static_assert(LAUNCH_REGS * THREADS >= SOFTMAX_REGS * 32 * SOFTMAX_WARPS + OTHER_REGS * 128, "a group that asks for more would wait forever");
@@ -537,6 +544,26 @@ __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int base) {
     return below_b & ~below_a;
 }
 
+// Zeros into the rows of a swizzled tile of V whose bits are not set (whole rows, so that the swizzle does not matter), for the MMAs
+// that the warp issues next. Two warps may clear the same tile, one while the other's MMAs read it: they write what is there.
+template <int KEYS, int HALVES>
+__device__ __forceinline__ void clear_rows(unsigned char *tile, const uint32_t (&kept)[4], int columns) {
+    const int lane = threadIdx.x & 31;
+    const bool gap = lane < 4 && (range_bits(0, columns, 32 * lane) & ~kept[lane & 3]) != 0;
+    if (__any_sync(0xffffffffu, gap)) {
+        for (int j = lane >> 3; j < columns; j += 4) {   // eight lanes a row
+            if ((kept[j >> 5] >> (j & 31) & 1u) == 0) {
+#pragma unroll
+                for (int x = 0; x < HALVES; ++x) {
+                    *reinterpret_cast<uint4 *>(tile + x * KEYS * 128 + j * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+    }
+}
+
 // One row again over its visible keys alone (rows whose tile held an infinity or NaN).
 __device__ __noinline__ void window_row_again(const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context,
                                               const WindowShape *s, float *s_q, int b, int i, int h) {
@@ -580,6 +607,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     __shared__ uint32_t s_tmem;
     __shared__ WindowStep s_steps[kStepSlots];
     __shared__ float s_row[C::SOFTMAX_WARPS][kWindowMaxDim];
+    __shared__ int4 s_again[C::SOFTMAX_WARPS][kAgainItems];   // rows to compute again: sequence, first row, head, which of 32
+    __shared__ int s_agains[C::SOFTMAX_WARPS];
+    __shared__ volatile int s_stop;                           // no more items
     __shared__ uint32_t s_bits[32][4];   // kept keys of 32 candidate steps
     unsigned char *tiles = tc_raw + ((1024u - (smem_addr(tc_raw) & 1023u)) & 1023u);
     unsigned char *s_qt = tiles, *s_kt = tiles + C::QUERIES * NQ * C::TILE_BYTES, *s_vt = s_kt + C::STAGES * C::KV_BYTES;
@@ -598,6 +628,10 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     if (threadIdx.x == 32) {
         s_turns = 0;
         s_first_bad = INT_MAX;
+        s_stop = 0;
+        for (int w = 0; w < C::SOFTMAX_WARPS; ++w) {
+            s_agains[w] = 0;
+        }
         mbar_init(&s_takes, 1);
         for (int i = 0; i < C::QUERIES; ++i) {
             mbar_init(&s_qfull[i], 1);
@@ -630,6 +664,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             // ---- items, steps and loads
             bool ok = true;
             int step = 0, turn = 0;
+            bool asked = true;
             for (int item = blockIdx.x; item >= 0 && ok; ++turn) {
                 const WindowItem<NQ> w(item, s, row_blocks, pair_heads);
                 if (lane == 0) {
@@ -728,9 +763,12 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                         todo &= todo - 1;
                         const int j0 = __shfl_sync(0xffffffffu, d.j0, from);
                         const bool end = base + from == steps;
-                        if (end && lane == 0) {   // the next item: not earlier, so that blocks finish together
-                            mbar_arrive_expect(&s_takes, 16);
-                            take_block(&s_taken[turn & 1], &s_takes);
+                        if (end) {   // the next item: not earlier, so that blocks finish together
+                            asked = __all_sync(0xffffffffu, s_stop == 0) != 0;
+                            if (asked && lane == 0) {
+                                mbar_arrive_expect(&s_takes, 16);
+                                take_block(&s_taken[turn & 1], &s_takes);
+                            }
                         }
                         const int st = step % C::STAGES;
                         const uint32_t before = (step / C::STAGES - 1) & 1;
@@ -769,8 +807,8 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                         step += ok ? 1 : 0;
                     }
                 }
-                ok = ok && wait_together(&s_takes, turn & 1);
-                item = ok ? taken_block(&s_taken[turn & 1]) : -1;
+                ok = ok && (!asked || wait_together(&s_takes, turn & 1));
+                item = ok && asked ? taken_block(&s_taken[turn & 1]) : -1;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the answer is read before its place is written again
             }
             if (ok) {   // the end of all
@@ -852,9 +890,13 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     break;
                 }
                 if (step > 0) {   // O += P.V of the step before; of one that ended an item, only the wait until O has been read
-                    ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1) && wait_together(&s_pfull[t], (step - 1) & 1);
-                    tmem_fence_after();
                     const bool takes_part = (flags_before & 1u) != 0;
+                    ok = ok && wait_together(&s_vfull[st_before], ((step - 1) / C::STAGES) & 1);
+                    if (ok && takes_part && (flags_before & 16u) != 0) {
+                        clear_rows<C::KEYS, C::HALVES>(s_vt + st_before * C::KV_BYTES, s_steps[(step - 1) % kStepSlots].kept, columns_before);
+                    }
+                    ok = ok && wait_together(&s_pfull[t], (step - 1) & 1);
+                    tmem_fence_after();
                     if (ok && leader) {
                         if (takes_part) {
                             const uint64_t vd = v_desc + (uint64_t) (st_before * (C::KV_BYTES / 16));
@@ -1094,15 +1136,25 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 }
                 __syncwarp();
             }
-            unsigned bad = __ballot_sync(0xffffffffu, i < s.seq && !(most <= 65504.f));
-            if (C::ROWS_BY_TMA && bad != 0 && lane == 0) {   // the rows just sent have to be there before they are written again
+            const unsigned bad = __ballot_sync(0xffffffffu, i < s.seq && total == total && !(most <= 65504.f));
+            if (bad != 0 && lane == 0) {
+                const int n = s_agains[warp];
+                s_again[warp][n % kAgainItems] = make_int4(work.b, i, h, (int) bad);
+                s_agains[warp] = n + 1;
+                s_stop = 1;
+            }
+            __syncwarp();
+        }
+        if (s_agains[warp] > 0) {
+            if (C::ROWS_BY_TMA && lane == 0) {   // the rows sent have to be there before they are written again
                 asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
             }
             __syncwarp();
-            while (bad != 0) {
-                const int from = __ffs(bad) - 1;
-                bad &= bad - 1;
-                window_row_again(q, k, v, mask, context, &s, s_row[warp], work.b, i - lane + from, h);
+            for (int n = 0; n < s_agains[warp]; ++n) {
+                const int4 rows = s_again[warp][n % kAgainItems];
+                for (unsigned bad = (unsigned) rows.w; bad != 0; bad &= bad - 1) {
+                    window_row_again(q, k, v, mask, context, &s, s_row[warp], rows.x, rows.y + __ffs(bad) - 1, rows.z);
+                }
             }
         }
     }

@@ -488,6 +488,72 @@ def test_window_attention_keys_out_of_sight_may_hold_anything(dim, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("dim,kv_heads", [(64, 12), (128, 6), (128, 12)])
+def test_window_attention_not_finite_values_among_many_items(dim, kv_heads, t):
+    """One column of one kept value is NaN in every other sequence, and padding holds anything: rows that see the key have NaN in that
+    column alone, the others and the other sequences what they had, however many items a block works through."""
+    batch, seq, heads = 4, 1300, 12
+    q, k, v, m = window_inputs(77 + dim, batch, seq, heads, kv_heads, dim, None, t)
+    q, k, v = q.clone(), k.clone(), v.clone()
+    m = torch.ones((batch, seq), dtype=torch.int8, device="cuda")
+    for b, length in enumerate((1300, 1211, 640, 77)):
+        m[b, length:] = 0
+    args = (batch, seq, heads, kv_heads, dim, 200, 0, 3, dim ** -0.5)
+    off = (m == 0).reshape(-1)
+    k[off], v[off] = 0, 0
+    clean = window_attention(q, k, v, m, *args, t)
+    k[off], v[off] = float("nan"), float("inf")
+    assert torch.equal(clean, window_attention(q, k, v, m, *args, t))
+    hit = {1: 600, 3: 50}
+    for b, j in hit.items():
+        v[b * seq + j, dim - 3::dim] = 0
+    ref = window64(q, k, v, m, *args)
+    for b, j in hit.items():
+        v[b * seq + j, dim - 3::dim] = float("nan")
+    got = window_attention(q, k, v, m, *args, t)
+    nan = torch.zeros((batch, seq, heads, dim), dtype=torch.bool, device="cuda")
+    for b, j in hit.items():
+        nan[b, j:j + 201, :, dim - 3] = True
+    nan = nan.reshape(batch * seq, heads * dim)
+    assert torch.equal(torch.isnan(got), nan)
+    check_window(got.masked_fill(nan, 0), tuple(a.masked_fill(nan, 0) for a in ref), t)
+    same = torch.ones((batch, seq), dtype=torch.bool, device="cuda")
+    same[1, 600 // 128 * 128:] = False
+    same[3] = False
+    assert torch.equal(got[same.reshape(-1)], clean[same.reshape(-1)])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_attention_long_rows_computed_again_leave_the_others_alone(dim):
+    """A NaN in a value that every later token sees: many long rows are computed again, and no wait for them runs out."""
+    batch, seq, heads, key = 2, 40000, 2, 100
+    g = gen(dim)
+    q, k, v = (normal(g, batch * seq, heads * dim, t="f16") for _ in range(3))
+    args = (batch, seq, heads, heads, dim, seq, 0, 0, dim ** -0.5)
+    clean = window_attention(q, k, v, None, *args, "f16")
+    v[key, 3::dim] = float("nan")
+    got = window_attention(q, k, v, None, *args, "f16")
+    nan = torch.zeros((batch, seq, heads, dim), dtype=torch.bool, device="cuda")
+    nan[0, key:, :, 3] = True
+    assert torch.equal(torch.isnan(got).view(batch, seq, heads, dim), nan)
+    assert torch.equal(got[seq:], clean[seq:])
+    v[key, 3::dim] = 0
+    for i in (0, 50, 99, 100, 101, 127, 128, 5000, 20011, 39999):
+        for h in range(heads):
+            at = slice(h * dim, (h + 1) * dim)
+            qd, kd, vd = q[i, at].double(), k[:i + 1, at].double(), v[:i + 1, at].double()
+            p = torch.softmax(kd @ qd * dim ** -0.5, 0)
+            want, pv = p @ vd, p @ vd.abs()
+            # float32 scores (dim sums, the exponential) move a weight and the sum by twice this; weights and result rounded to binary16
+            scores = 2 * (dim + 8) * 2.0 ** -23 * float((kd.abs() @ qd.abs()).max() * dim ** -0.5) + 2.0 ** -20
+            bar = pv * (scores + 2.0 ** -11 * (1 + 2.0 ** -6)) + 2.0 ** -25 * (vd.abs().sum(0) + 1) + 2.0 ** -11 * want.abs()
+            row = got[i, at].double()
+            if i >= key:
+                row[3], want[3] = 0, 0
+            within(row, want, bar, "row %d of head %d" % (i, h))
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_window_attention_large_scores(t):
     """Scores of some thousands: the running maximum moves far; the largest weight wins."""
     q, k, v, m = window_inputs(21, 1, 700, 2, 2, 64, None, t)
