@@ -359,9 +359,9 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 // Bound by the softmax: per 128 x 128 tile the exponentials take 1024 cycles of an SM's special-function unit and the products 512 of
 // its tensor cores (heads of 64; 1024 for heads of 128), a step 1500. Measured: 8192 tokens, 32 / 8 heads of 128, window 2048: 265 to
 // 290 us by the clock under the power cap (840 to 910 TFLOP/s); 4 x 4096 tokens, 16 heads of 64, no window 400 us, window 513 and ragged
-// lengths 86 us (3 steps an item that ran: half of that goes into the ends of items; without clearing unseen V rows 84). A row computed
-// again reads its keys two bytes at a time: 40000 rows of 2 heads over 20000 keys each take about half a second. Tried and slower: two threads a row, part of the
-// exponentials by polynomial, scores of 96 keys twice, masks gathered by a warp of their own.
+// lengths 86 us (3 steps an item that ran: half of that goes into the ends of items; without clearing unseen V rows 84). Rows computed
+// again are far slower: one causal sequence of 40000 tokens, 2 heads of 64, all of it from token 100 on: 542 ms (1.2 ms without). Tried
+// and slower: two threads a row, part of the exponentials by polynomial, scores of 96 keys twice, masks gathered by a warp of their own.
 // Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, frees its tensor memory and
 // returns.
 constexpr int kTileRows = 128;

@@ -38,6 +38,19 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
                 const T *kr = key(j);
                 float a0 = 0.f, a1 = 0.f;
                 int c = 0;
+                if ((reinterpret_cast<uintptr_t>(kr) & 15u) == 0) {
+                    constexpr int E = 16 / (int) sizeof(T);
+#pragma unroll 4
+                    for (; c + E <= dim; c += E) {
+                        const uint4 raw = *reinterpret_cast<const uint4 *>(kr + c);
+                        const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+                        for (int x = 0; x < E; x += 2) {
+                            a0 = fmaf(s_q[c + x], to_float<T>(e[x]), a0);
+                            a1 = fmaf(s_q[c + x + 1], to_float<T>(e[x + 1]), a1);
+                        }
+                    }
+                }
                 for (; c + 1 < dim; c += 2) {
                     a0 = fmaf(s_q[c], to_float<T>(kr[c]), a0);
                     a1 = fmaf(s_q[c + 1], to_float<T>(kr[c + 1]), a1);
@@ -62,15 +75,26 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
             for (int i = 0; i < kWindowMaxDim / 32; ++i) {
                 o[i] *= shrink;
             }
-            while (visible != 0) {
-                const int from = __ffs(visible) - 1;
-                visible &= visible - 1;
-                const float w = __shfl_sync(0xffffffffu, p, from);
-                const T *vr = value(j0 + from);
+            while (visible != 0) {   // the rows of four keys on their way at a time
+                float w[4], e[4][kWindowMaxDim / 32];
 #pragma unroll
-                for (int i = 0; i < kWindowMaxDim / 32; ++i) {
-                    if (lane + 32 * i < dim) {
-                        o[i] = fmaf(w, to_float<T>(vr[lane + 32 * i]), o[i]);
+                for (int u = 0; u < 4; ++u) {
+                    const bool on = visible != 0;
+                    const int from = on ? __ffs(visible) - 1 : 0;
+                    visible &= visible - 1;
+                    w[u] = __shfl_sync(0xffffffffu, p, from);
+                    w[u] = on ? w[u] : 0.f;
+                    const T *vr = value(j0 + from);
+#pragma unroll
+                    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+                        e[u][i] = on && lane + 32 * i < dim ? to_float<T>(vr[lane + 32 * i]) : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+                        o[i] = fmaf(w[u], e[u][i], o[i]);
                     }
                 }
             }
