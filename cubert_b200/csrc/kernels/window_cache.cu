@@ -57,7 +57,9 @@ window_step_rows_kernel(const T *q, const T *k, const T *v, const int32_t *posit
 // The keys of a stream are cut into blocks that the warps of the cluster take in turn, each with a softmax of its own over
 // what it took; at the end the blocks read one another's partial sums through distributed shared memory and every block
 // writes its share of the context. Nothing is staged in device memory, so calls need no workspace and no order among them,
-// and the sums are added in the same order every time. The kernel is bound by the cache's bytes.
+// and the sums are added in the same order every time. The kernels are bound by the cache's bytes: 32 streams of 32 / 8 heads of 128
+// over 2048 slots, binary16, take 39.9 us (5.3 TB/s, 0.82 of what a copy reaches). Small grids are bound by the loads an SM has in
+// flight and by two cluster barriers: one such stream with 4096 slots 10.7 us, one float32 stream of 12 heads of 64 with 512 slots 4.5.
 template <int WARPS, int HEADS, int DP>
 struct StepPartial {
     float o[WARPS][HEADS][DP + 2];   // two columns of padding spread the rows over the banks
@@ -389,7 +391,8 @@ window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const 
 }
 
 // float32: LPK lanes share a key, four columns each, so that a warp reads 32 / LPK whole rows per instruction; every group of
-// lanes keeps a softmax of its own over its keys, HEADS heads at once.
+// lanes keeps a softmax of its own over its keys, HEADS heads at once. Per key and head a lane has four multiply-adds for the score
+// and log2(LPK) shuffles with an addition each for its sum.
 template <int WARPS, int LPK, int HEADS>
 __global__ void __launch_bounds__(32 * WARPS)
 window_step_f32_kernel(const float *q, const float *k, const float *v, const int32_t *positions, float *k_cache, float *v_cache, float *context,
