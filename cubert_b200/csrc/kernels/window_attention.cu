@@ -278,14 +278,14 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
         const float all = group_sum<16>(total[r]);
         const float inv = all == 0.f ? 0.f : 1.f / all;
         const int i = row0 + 8 * rg + r;
-        bool finite = true;
+        bool finite = true;   // or NaN as it is, from a visible score
         T *out = context + (first + i) * s.context_stride + (int64_t) h * s.dim;
 #pragma unroll
         for (int c = 0; c < 4 * VC; ++c) {
             const int col = 64 * (c / 4) + 4 * cg + c % 4;
             const float x = ((r & 1) ? o[r / 2][c].y : o[r / 2][c].x) * inv;
             if (col < s.dim) {
-                finite = finite && fabsf(x) <= most;
+                finite = finite && (fabsf(x) <= most || all != all);
                 if (i < s.seq) {
                     out[col] = from_float<T>(x);
                 }
