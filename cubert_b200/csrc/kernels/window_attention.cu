@@ -360,7 +360,7 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 // Bound by the softmax: per 128 x 128 tile the exponentials take 1024 cycles of an SM's special-function unit and the products 512 of
 // its tensor cores (heads of 64; 1024 for heads of 128), a step 1500. Measured: 8192 tokens, 32 / 8 heads of 128, window 2048: 265 to
 // 290 us by the clock under the power cap (840 to 910 TFLOP/s); 4 x 4096 tokens, 16 heads of 64, no window 400 us, window 513 and ragged
-// lengths 86 us (3 steps an item that ran: half of that goes into the ends of items; without clearing unseen V rows 84). Rows computed
+// lengths 81 us (3 steps an item that ran; half of it goes into the ends of items). Rows computed
 // again are far slower: one causal sequence of 40000 tokens, 2 heads of 64, all of it from token 100 on: 542 ms (1.2 ms without). Tried
 // and slower: two threads a row, part of the exponentials by polynomial, scores of 96 keys twice, masks gathered by a warp of their own.
 // Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, frees its tensor memory and
@@ -394,7 +394,7 @@ struct WindowTc {
     static constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
     // The context's rows leave through the place of the item's queries by TMA, or as 16-byte stores from registers. TMA holds the queries
     // of the item after the next back until they have left: 8192 tokens, 32 heads of 128: 265 us against 277, but 4 x 4096 tokens, 16
-    // heads of 64, window 513, whose items are short: 88 against 84 before unseen V rows were cleared.
+    // heads of 64, window 513, whose items are short: 88 against 84 as the kernel was then.
     static constexpr bool ROWS_BY_TMA = NQ == 2;
     static constexpr int LAUNCH_REGS = NQ == 1 ? 128 : 168, SOFTMAX_REGS = NQ == 1 ? 192 : 224, OTHER_REGS = 56;
     static_assert(LAUNCH_REGS * THREADS >= SOFTMAX_REGS * 32 * SOFTMAX_WARPS + OTHER_REGS * 128, "a group that asks for more would wait forever");
@@ -672,7 +672,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     s_items[turn & 3] = item;
                     s_turns = turn + 1;
                 }
-                const int lo = w.row0 > s.before ? (w.row0 - s.before) & ~3 : 0;   // whole words of the mask
+                const int lo = w.row0 > s.before ? (w.row0 - s.before) & ~15 : 0;   // whole vectors of the mask
                 const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
                 const int sinks_end = min(s.sinks, lo), sink_steps = (sinks_end + C::KEYS - 1) / C::KEYS;
                 const int steps = sink_steps + (hi - lo + C::KEYS - 1) / C::KEYS;
@@ -692,39 +692,72 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 }
                 // 32 candidates at a time, one per lane; then those that hold a kept key, and the item's end, one after another.
                 for (int base = 0; base <= steps && ok; base += 32) {
-                    if (kept != nullptr) {   // four keys a lane, eight steps in flight
+                    // Sixteen keys a lane and load where the mask's rows allow it, else four or one: 4 x 4096 tokens, window 513, ragged
+                    // lengths: 81.2 us by sixteens, 86.0 by fours.
+                    if (kept != nullptr) {
                         const int candidates = min(32, steps - base);
                         const bool words = s.seq % 4 == 0 && (reinterpret_cast<uintptr_t>(mask) & 3) == 0;   // of four keys: none reaches past its row
+                        const bool vectors = C::KEYS % 16 == 0 && s.seq % 16 == 0 && (reinterpret_cast<uintptr_t>(mask) & 15) == 0;   // of sixteen
                         __syncwarp();
-                        for (int c0 = 0; c0 < candidates; c0 += 8) {
-                            uint32_t four[8];
+                        if (vectors) {
+                            constexpr int PER = C::KEYS / 16;   // lanes a step
+                            for (int c0 = 0; c0 < candidates * PER; c0 += 64) {
+                                uint4 raw[2];
+                                int left[2];
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) {
-                                const int at = base + c0 + u;
-                                const int j = (at < sink_steps ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS) + 4 * lane;
-                                const int left = c0 + u < candidates && 4 * lane < C::KEYS ? (at < sink_steps ? sinks_end : hi) - j : 0;
-                                four[u] = 0;
-                                if (words) {
-                                    four[u] = left > 0 ? *reinterpret_cast<const uint32_t *>(kept + j) & (left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u) : 0u;
-                                } else {
+                                for (int u = 0; u < 2; ++u) {
+                                    const int x = c0 + 32 * u + lane, at = base + x / PER;
+                                    const int j = (at < sink_steps ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS) + 16 * (x % PER);
+                                    left[u] = x < candidates * PER ? (at < sink_steps ? sinks_end : hi) - j : 0;
+                                    raw[u] = left[u] > 0 ? *reinterpret_cast<const uint4 *>(kept + j) : make_uint4(0, 0, 0, 0);
+                                }
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) {
-                                        four[u] |= e < left ? (uint32_t) (uint8_t) kept[j + e] << (8 * e) : 0u;
+                                for (int u = 0; u < 2; ++u) {
+                                    const int x = c0 + 32 * u + lane;
+                                    const uint32_t q4[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                                    uint32_t bits = 0;
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {   // any bit of a byte -> its highest; the four highest bits side by side
+                                        const uint32_t v = (((q4[e] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | q4[e]) & 0x80808080u;
+                                        bits |= ((v >> 7) * 0x01020408u >> 24 & 15u) << (4 * e);
+                                    }
+                                    bits &= left[u] >= 16 ? 0xffffu : left[u] > 0 ? (1u << left[u]) - 1u : 0u;
+                                    if (x < candidates * PER) {
+                                        reinterpret_cast<uint16_t *>(s_bits[x / PER])[x % PER] = (uint16_t) bits;
                                     }
                                 }
                             }
+                        } else {
+                            for (int c0 = 0; c0 < candidates; c0 += 8) {
+                                uint32_t four[8];
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) {
-                                // any bit of a byte -> its lowest; the four lowest bits side by side; eight lanes' to a word
-                                uint32_t v = four[u] | four[u] >> 4;
-                                v |= v >> 2;
-                                v |= v >> 1;
-                                v = ((v & 0x01010101u) * 0x01020408u >> 24 & 15u) << (4 * (lane & 7));
-                                v |= __shfl_xor_sync(0xffffffffu, v, 1);
-                                v |= __shfl_xor_sync(0xffffffffu, v, 2);
-                                v |= __shfl_xor_sync(0xffffffffu, v, 4);
-                                if ((lane & 7) == 0 && c0 + u < candidates) {
-                                    s_bits[c0 + u][lane >> 3] = v;
+                                for (int u = 0; u < 8; ++u) {
+                                    const int at = base + c0 + u;
+                                    const int j = (at < sink_steps ? at * C::KEYS : lo + (at - sink_steps) * C::KEYS) + 4 * lane;
+                                    const int left = c0 + u < candidates && 4 * lane < C::KEYS ? (at < sink_steps ? sinks_end : hi) - j : 0;
+                                    four[u] = 0;
+                                    if (words) {
+                                        four[u] = left > 0 ? *reinterpret_cast<const uint32_t *>(kept + j) & (left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u) : 0u;
+                                    } else {
+#pragma unroll
+                                        for (int e = 0; e < 4; ++e) {
+                                            four[u] |= e < left ? (uint32_t) (uint8_t) kept[j + e] << (8 * e) : 0u;
+                                        }
+                                    }
+                                }
+#pragma unroll
+                                for (int u = 0; u < 8; ++u) {
+                                    // any bit of a byte -> its lowest; the four lowest bits side by side; eight lanes' to a word
+                                    uint32_t v = four[u] | four[u] >> 4;
+                                    v |= v >> 2;
+                                    v |= v >> 1;
+                                    v = ((v & 0x01010101u) * 0x01020408u >> 24 & 15u) << (4 * (lane & 7));
+                                    v |= __shfl_xor_sync(0xffffffffu, v, 1);
+                                    v |= __shfl_xor_sync(0xffffffffu, v, 2);
+                                    v |= __shfl_xor_sync(0xffffffffu, v, 4);
+                                    if ((lane & 7) == 0 && c0 + u < candidates) {
+                                        s_bits[c0 + u][lane >> 3] = v;
+                                    }
                                 }
                             }
                         }
@@ -741,7 +774,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     int count = 0;
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        d.kept[u] = keys == 0 ? 0 : kept != nullptr ? s_bits[lane][u] : range_bits(0, keys, 32 * u);
+                        d.kept[u] = keys == 0 ? 0 : kept != nullptr ? s_bits[lane][u] & range_bits(0, keys, 32 * u) : range_bits(0, keys, 32 * u);
                         count += __popc(d.kept[u]);
                     }
 #pragma unroll

@@ -488,6 +488,30 @@ def test_window_attention_keys_out_of_sight_may_hold_anything(dim, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("seq,dim", [(16, 64), (256, 64), (1296, 64), (1296, 128), (1300, 128), (1301, 64)])
+@pytest.mark.parametrize("before,after,sinks", [(101, 7, 3), (300, 0, 140), (5000, 5000, 0)])
+def test_window_attention_masks_of_any_alignment_and_byte(seq, dim, before, after, sinks, t):
+    """Any byte but 0 keeps a key, wherever the mask starts; long runs of masked keys between."""
+    batch, heads = 2, 2
+    q, k, v, _ = window_inputs(seq + dim, batch, seq, heads, heads, dim, None, t)
+    g = gen(seq)
+    values = torch.tensor([0, 1, -1, -128, 127, 64, 2, 0], dtype=torch.int8, device="cuda")
+    m = values[torch.randint(0, 8, (batch, seq), generator=g, device="cuda")]
+    m[1, 200:700] = 0
+    args = (batch, seq, heads, heads, dim, before, after, sinks, dim ** -0.5)
+    got = None
+    for shift in (0, 1, 4, 8, 16):
+        room = torch.full((batch * seq + 64,), 77, dtype=torch.int8, device="cuda")
+        here = room[shift:shift + batch * seq].view(batch, seq)
+        here.copy_(m)
+        out = window_attention(q, k, v, here, *args, t)
+        if got is None:
+            check_window(out, window64(q, k, v, m, *args), t)
+        assert got is None or torch.equal(out, got)
+        got = out
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("dim,kv_heads", [(64, 12), (128, 6), (128, 12)])
 def test_window_attention_not_finite_values_among_many_items(dim, kv_heads, t):
     """One column of one kept value is NaN in every other sequence, and padding holds anything: rows that see the key have NaN in that
