@@ -521,10 +521,29 @@ int w4_matvec_launch(const typename XLoad<X>::Elem *x, const float *x_scales, in
     const W4Plan plan = w4_plan(k, S::LIMIT, S::X_TILE + S::SCALES, S::CARRY);
     const int smem = S::RING + plan.slice * (S::X_TILE + S::SCALES) + (plan.slices > 1 ? plan.round * S::CARRY : 0);
     const int tiles = (n + kW4Tile - 1) / kW4Tile;
-    const dim3 grid((unsigned) (tiles < resident ? tiles : resident), (unsigned) ((rows + 8 * TT - 1) / (8 * TT)));
+    // one wave: blocks of different rows read the same codes at the same time (64 x 4096 by 11008 with a wave per 32 rows 63.1 us, in one 44.5)
+    const int row_blocks = (rows + 8 * TT - 1) / (8 * TT), across = resident / row_blocks > 1 ? resident / row_blocks : 1;
+    const dim3 grid((unsigned) (tiles < across ? tiles : across), (unsigned) row_blocks);
     w4_matvec_kernel<T, X, TT, GROUP><<<grid, 32 * kW4Warps, smem, stream>>>(x, x_scales, x_groups, rows, k, (const uint8_t *) packed, scales,
                                                                              n, bias, out, vec, plan);
     return check_launch();
+}
+
+// Eight rows of x a block, or sixteen (one more product per expanded code; 16 x 4096 by 30522: 24.8 us). Eight also where their blocks
+// make one wave, so that more SMs share the laying out of x (24 x 6144 by 139: 30.3 us in blocks of 32 rows, 8.1 in blocks of eight), and
+// where sixteen rows of x do not fit into shared memory at once and eight do (16 x 8192 by 8192: 22.7 and 20.2). More than
+// sixteen are slower at every size tried: 64 x 4096 by 11008 44.5 us by 32 rows, 30.8 by 16; 32 x 768 by 2304 6.0 and 4.5.
+template <typename T, XKind X, int GROUP>
+int w4_matvec_rows(const typename XLoad<X>::Elem *x, const float *x_scales, int x_groups, int rows, int k, const void *packed,
+                   const T *scales, int n, const T *bias, T *out, bool vec, cudaStream_t stream) {
+    const int64_t tiles = (n + kW4Tile - 1) / kW4Tile, kblocks = (k + kW4Block - 1) / kW4Block, eights = ((int64_t) rows + 7) / 8;
+    typedef W4Smem<T, X, 1, GROUP> One;
+    typedef W4Smem<T, X, 2, GROUP> Two;
+    const bool only_eight_fit = kblocks * (Two::X_TILE + Two::SCALES) > Two::LIMIT && kblocks * (One::X_TILE + One::SCALES) <= One::LIMIT;
+    if (rows <= 8 || tiles * eights <= 148 || (only_eight_fit && eights <= 65535)) {
+        return w4_matvec_launch<T, X, 1, GROUP>(x, x_scales, x_groups, rows, k, packed, scales, n, bias, out, vec, stream);
+    }
+    return w4_matvec_launch<T, X, 2, GROUP>(x, x_scales, x_groups, rows, k, packed, scales, n, bias, out, vec, stream);
 }
 
 template <typename T, XKind X>
@@ -534,7 +553,7 @@ int w4_matvec(const typename XLoad<X>::Elem *x, const float *x_scales, int x_gro
         (group != 32 && group != 64 && group != 128) || (X == X_E4M3 && (x_scales == nullptr || (x_group != 0 && x_group != 128)))) {
         return CUBK_ERR_INVALID_ARG;
     }
-    if (!aligned16(packed) || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0 || (rows + 31) / 32 > 65535 || k > (1 << 30) || n > (1 << 30)) {
+    if (!aligned16(packed) || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0 || ((int64_t) rows + 15) / 16 > 65535 || k > (1 << 30) || n > (1 << 30)) {
         return CUBK_ERR_UNSUPPORTED;
     }
     if (rows == 0) {
@@ -544,17 +563,9 @@ int w4_matvec(const typename XLoad<X>::Elem *x, const float *x_scales, int x_gro
     // whole vectors: of eight columns, of float32 four
     const bool vec = k % (X == X_F32 ? 4 : 8) == 0 && reinterpret_cast<uintptr_t>(x) % (kLane < 16 ? kLane : 16) == 0;
     const int x_groups = X == X_E4M3 && x_group != 0 ? (k + kW4Block - 1) / kW4Block : 1;
-#define W4_GROUP(TT, GROUP) w4_matvec_launch<T, X, TT, GROUP>(x, x_scales, x_groups, rows, k, packed, scales, n, bias, out, vec, stream)
-#define W4(TT) (group == 32 ? W4_GROUP(TT, 32) : group == 64 ? W4_GROUP(TT, 64) : W4_GROUP(TT, 128))
-    if (rows <= 8) {
-        return W4(1);
-    }
-    if (rows <= 16) {
-        return W4(2);
-    }
-    return W4(4);
+#define W4(GROUP) w4_matvec_rows<T, X, GROUP>(x, x_scales, x_groups, rows, k, packed, scales, n, bias, out, vec, stream)
+    return group == 32 ? W4(32) : group == 64 ? W4(64) : W4(128);
 #undef W4
-#undef W4_GROUP
 }
 
 // ---------------------------------------------------------------- laying the weights out

@@ -301,8 +301,9 @@ int cubk_residual_rms_norm_e4m3_f16(const void *x, const void *residual, const v
 /* ---- K7: products of a few rows with 4-bit weights --------------------------------------------------
  * out[m,n] = sum_k x[m,k] * code[n,k] * scale[k / group, n] (+ bias[n]),  code in -8..7,  group 32, 64 or 128
  * For requests of a few tokens, whose dense products do nothing but read weights. No counterpart in the reference,
- * whose products are float32 or binary16 library calls (src/cuBERT/op/Dense.cpp:41-52). Any number of rows is
- * computed; from about a hundred on, a library product on unpacked weights is the better call.
+ * whose products are float32 or binary16 library calls (src/cuBERT/op/Dense.cpp:41-52). Up to 1048560 rows are computed
+ * (CUBK_ERR_UNSUPPORTED beyond), but with more than a few a library product of binary16 weights, where there is room for
+ * them, takes no longer: from 16 rows on at 4096 by 4096, from about 28 at 4096 by 11008; a third of the time at 128 rows.
  * x [rows, k], bias [n] (or NULL), out [rows, n] and the scales [ceil(k / group), n] in the storage type. Sums are
  * float32; a code times its scale is never rounded. out must not overlap the operands.
  * The _e4m3 calls take x as the 8-bit codes and scales K6 writes: code_scales [rows] (code_group = 0) or

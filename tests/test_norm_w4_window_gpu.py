@@ -221,7 +221,8 @@ def check_matvec(got, x64, codes, scales, group, bias, t, what=""):
 
 
 W4_SHAPES = [(1, 128, 16), (1, 768, 2304), (8, 1024, 1000), (3, 1000, 777), (2, 1, 1), (5, 37, 17), (9, 512, 100), (16, 4096, 64), (17, 768, 33),
-             (33, 200, 50), (64, 1024, 256), (70, 640, 48), (1, 8192, 96), (4, 2056, 4096), (130, 96, 16)]
+             (33, 200, 50), (64, 1024, 256), (70, 640, 48), (1, 8192, 96), (4, 2056, 4096), (130, 96, 16),
+             (24, 6144, 139), (64, 3272, 1201), (16, 8192, 2500), (40, 12300, 800), (2401, 64, 40)]
 
 
 @pytest.mark.parametrize("t", TYPES)

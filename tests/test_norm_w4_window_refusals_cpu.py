@@ -31,7 +31,7 @@ def test_w4_matvec():
     good = (A, 2, 256, A, A, 64, 32, A, A, None)   # x, rows, k, packed, scales, group, n, bias, out, stream
     refused("w4_matvec", good, [(0, None, INVALID), (3, None, INVALID), (4, None, INVALID), (8, None, INVALID), (1, -1, INVALID), (2, 0, INVALID),
                                 (6, 0, INVALID), (5, 0, INVALID), (5, 48, INVALID), (5, 256, INVALID), (3, A + 8, UNSUPPORTED), (4, A + 2, UNSUPPORTED), (2, 2 ** 30 + 1, UNSUPPORTED),
-                                (6, 2 ** 30 + 1, UNSUPPORTED), (1, 0, 0)])
+                                (6, 2 ** 30 + 1, UNSUPPORTED), (1, 16 * 65535 + 1, UNSUPPORTED), (1, 0, 0)])
     good = (A, A, 0, 2, 256, A, A, 64, 32, A, A, None)   # codes, code_scales, code_group, rows, ...
     refused("w4_matvec_e4m3", good, [(0, None, INVALID), (1, None, INVALID), (2, 64, INVALID), (3, -1, INVALID), (5, None, INVALID),
                                      (6, None, INVALID), (10, None, INVALID), (5, A + 4, UNSUPPORTED), (7, 16, INVALID), (3, 0, 0)])
