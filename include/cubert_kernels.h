@@ -347,7 +347,7 @@ int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int cod
  *     scores, weights and contexts in tensor memory; weights are rounded to binary16. Every wait is bounded (0.2 s): a
  *     block that gives up writes NaN into the rows it has not finished.
  *   otherwise, head_dim up to 128: the float32 pipes, 64 x 64 tiles.
- *   head_dim above 128: one row per warp. */
+ *   head_dim above 128, and up to 6 (binary16) or 12 (float32) tokens a sequence: one row per warp. */
 int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
                               int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,
                               float *context, int64_t context_stride, void *stream);

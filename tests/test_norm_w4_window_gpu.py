@@ -412,6 +412,12 @@ WINDOWS = [
     (2, 64, 2, 2, 96, 16, 16, 1, "prefix"),
     (1, 2049, 2, 1, 64, 700, 0, 4, None),
     (1, 1, 2, 2, 128, 5, 5, 5, "none kept"),
+    (3, 6, 4, 2, 64, 2, 1, 1, "holes"),
+    (70, 7, 4, 2, 128, 4, 0, 2, "prefix"),
+    (5, 12, 3, 1, 64, 5, 2, 3, "holes"),
+    (300, 12, 2, 2, 32, 100, 0, 0, "prefix"),
+    (2, 13, 6, 3, 128, 6, 6, 1, "holes"),
+    (1000, 2, 12, 12, 64, 1, 0, 0, "prefix"),
     (2, 260, 2, 2, 64, 40, 3, 0, "none kept"),
 ]
 
