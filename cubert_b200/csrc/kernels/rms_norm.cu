@@ -396,6 +396,9 @@ int residual_rms_norm(const T *x, const T *residual, const T *gamma, int64_t row
         (E4M3 && group != 0 && group != 128)) {
         return CUBK_ERR_INVALID_ARG;
     }
+    if (channels > (1 << 30)) {   // column arithmetic is 32-bit
+        return CUBK_ERR_UNSUPPORTED;
+    }
     if (rows == 0) {
         return CUBK_OK;
     }

@@ -288,7 +288,7 @@ int cubk_pooler_head_f16(const void *x, const void *pooler_bias, const void *wei
  * scales [rows]) or over blocks of 128 columns (group = 128, scales [rows, ceil(channels / 128)], the last block as
  * short as the row leaves it). A group whose largest |y| is below 2^-100 is stored as zeros with scale 0. A NaN in a
  * group makes its scale and codes NaN. The e4m3 codes are what cubk_w4_matvec_e4m3_* and 8-bit library products read.
- * eps >= 0; a row of zeros under eps = 0 gives NaN. */
+ * eps >= 0; a row of zeros under eps = 0 gives NaN. channels up to 2^30 (CUBK_ERR_UNSUPPORTED beyond). */
 int cubk_residual_rms_norm_f32(const float *x, const float *residual, const float *gamma, int64_t rows, int channels, float eps,
                                float *sum, float *out, void *stream);
 int cubk_residual_rms_norm_f16(const void *x, const void *residual, const void *gamma, int64_t rows, int channels, float eps,
