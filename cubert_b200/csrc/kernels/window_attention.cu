@@ -64,6 +64,13 @@ struct WindowPlain {
     static constexpr int BYTES = FLOATS * 4;
 };
 
+// Bits lo .. hi - 1 of a word that stands for positions base .. base + 31.
+__device__ __forceinline__ uint32_t range_bits(int lo, int hi, int base) {
+    const int a = min(max(lo - base, 0), 32), b = min(max(hi - base, 0), 32);
+    const uint32_t below_b = b == 32 ? 0xffffffffu : (1u << b) - 1u, below_a = a == 32 ? 0xffffffffu : (1u << a) - 1u;
+    return below_b & ~below_a;
+}
+
 // Columns c .. c + 3 of a row as float32, zeros past the dimension.
 template <typename T>
 __device__ __forceinline__ float4 four_columns(const T *row, int c, int dim, bool vec) {
@@ -72,6 +79,56 @@ __device__ __forceinline__ float4 four_columns(const T *row, int c, int dim, boo
     }
     return make_float4(c < dim ? to_float<T>(row[c]) : 0.f, c + 1 < dim ? to_float<T>(row[c + 1]) : 0.f,
                        c + 2 < dim ? to_float<T>(row[c + 2]) : 0.f, c + 3 < dim ? to_float<T>(row[c + 3]) : 0.f);
+}
+
+constexpr int kNotFinite = 1, kSumZero = 2;   // what a row came out with
+
+// The rows of a block that need another look, out of the way of the others' code. A row that is not finite is computed again over its
+// visible keys alone. A row with a sum of 0 sees no key, and is zeros, or nothing but scores of minus infinity, and is NaN (0 / 0):
+// which, the mask says, 4096 candidates at a time as bits in the list's place, a word a lane.
+template <typename T>
+__device__ __noinline__ void window_plain_again(const T *q, const T *k, const T *v, const int8_t *mask, T *context, const WindowShape *s, float *s_q,
+                                                int *s_list, int *s_bad, int b, int h, int row0) {
+    constexpr int WARPS = kPlainThreads / 32, WORDS = 128;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int last_row = min(row0 + kPlainRows, s->seq) - 1;
+    const int lo = row0 > s->before ? row0 - s->before : 0;
+    const int hi = s->after < s->seq - 1 - last_row ? last_row + s->after + 1 : s->seq;
+    const int sinks_end = min(s->sinks, lo), listed = sinks_end + hi - lo;
+    const int8_t *kept = mask != nullptr ? mask + (int64_t) b * s->seq : nullptr;
+    if (__syncthreads_or(threadIdx.x < kPlainRows && s_bad[threadIdx.x] == kSumZero)) {
+        for (int base = 0; base < listed; base += 32 * WORDS) {
+            const int words = min(WORDS, (listed - base + 31) / 32);
+#pragma unroll 4
+            for (int w = warp; w < words; w += WARPS) {
+                const int u = base + 32 * w + lane, j = u < sinks_end ? u : lo + u - sinks_end;
+                const unsigned on = __ballot_sync(0xffffffffu, u < listed && (kept == nullptr || kept[j] != 0));
+                if (lane == 0) {
+                    s_list[w] = (int) on;
+                }
+            }
+            __syncthreads();
+            if (threadIdx.x < kPlainRows && s_bad[threadIdx.x] == kSumZero) {
+                const int i = row0 + (int) threadIdx.x;
+                const int i_lo = i > s->before ? i - s->before : 0, i_hi = s->after < s->seq - 1 - i ? i + s->after + 1 : s->seq;
+                const int sinks = min(s->sinks, i_hi), from = i_lo - lo + sinks_end, to = i_hi - lo + sinks_end;   // candidates that the row may see
+                unsigned seen = 0;
+                for (int w = 0; w < words; ++w) {
+                    const int bit = base + 32 * w;
+                    seen |= (unsigned) s_list[w] & (range_bits(0, sinks, bit) | range_bits(from, to, bit));
+                }
+                if (seen != 0) {
+                    s_bad[threadIdx.x] = kNotFinite;
+                }
+            }
+            __syncthreads();
+        }
+    }
+    for (int r = warp; r < kPlainRows; r += WARPS) {
+        if (s_bad[r] == kNotFinite) {
+            window_prompt_row<T>(q, k, v, mask, context, *s, s_q + warp * kWindowMaxDim, b, row0 + r, h);
+        }
+    }
 }
 
 template <typename T, int DP>
@@ -128,6 +185,7 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
         }
     }
     int cursor = 0, have = 0;   // candidates looked at, keys in the list
+    bool met = false;           // any key at all
     for (;;) {
         while (have < kPlainKeys && cursor < listed) {
             const int u = cursor + threadIdx.x, j = u < sinks_end ? u : lo + u - sinks_end;
@@ -153,6 +211,7 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
         if (keys == 0) {
             break;
         }
+        met = true;
         __syncthreads();   // the list, also where it needed nothing
         // eight loads of a thread in flight at a time
 #pragma unroll
@@ -273,6 +332,7 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
         have = left;
     }
     const float most = sizeof(T) == 4 ? 3.402823466e38f : 65504.f;
+    bool rest = false;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const float all = group_sum<16>(total[r]);
@@ -293,14 +353,12 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
         }
         const unsigned bad = __ballot_sync(0xffffffffu, !finite);
         if (cg == 0) {
-            s_bad[8 * rg + r] = (bad >> (lane & 16) & 0xffffu) != 0 && i < s.seq;
+            s_bad[8 * rg + r] = i >= s.seq ? 0 : (bad >> (lane & 16) & 0xffffu) != 0 ? kNotFinite : all == 0.f ? kSumZero : 0;
+            rest = rest || s_bad[8 * rg + r] != 0;
         }
     }
-    __syncthreads();   // Q is no longer read: its place serves the rows that are computed again
-    for (int r = warp; r < kPlainRows; r += kPlainThreads / 32) {
-        if (s_bad[r] != 0) {
-            window_prompt_row<T>(q, k, v, mask, context, s, s_q + warp * kWindowMaxDim, b, row0 + r, h);
-        }
+    if (__syncthreads_or(rest && met)) {   // Q is no longer read: its place serves the rows that are computed again
+        window_plain_again<T>(q, k, v, mask, context, &s, s_q, s_list, s_bad, b, h, row0);
     }
 }
 
@@ -536,13 +594,6 @@ __device__ __forceinline__ void tma_rows(const CUtensorMap *map, const void *src
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(smem_addr(src)), "r"(column),
                  "r"(row), "r"(head), "r"(batch)
                  : "memory");
-}
-
-// Bits lo .. hi - 1 of a word that stands for positions base .. base + 31.
-__device__ __forceinline__ uint32_t range_bits(int lo, int hi, int base) {
-    const int a = min(max(lo - base, 0), 32), b = min(max(hi - base, 0), 32);
-    const uint32_t below_b = b == 32 ? 0xffffffffu : (1u << b) - 1u, below_a = a == 32 ? 0xffffffffu : (1u << a) - 1u;
-    return below_b & ~below_a;
 }
 
 // Zeros into the rows of a swizzled tile of V whose bits are not set (whole rows, so that the swizzle does not matter), for the MMAs
@@ -980,7 +1031,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             const int hi = s.after < s.seq - 1 - i ? i + s.after + 1 : s.seq;
             const int sinks_hi = min(s.sinks, hi);
             float top = -INFINITY, total = 0.f;   // top: of q.k, unscaled
-            bool first = true;
+            bool first = true, any = false;       // any: the row has met a key that it sees
             // One step of this row. The number of its 16-column chunks is fixed, so that its loops have no branches and the exponentials of
             // one chunk overlap the arithmetic of the next (a branch per chunk costs a third of the rate).
             auto softmax_step = [&](auto chunks, const WindowStep *d, uint32_t flags) {
@@ -1005,11 +1056,14 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
 #pragma unroll
                     for (int w = 0; w < CHUNKS; w += 2) {   // 32 columns
                         const uint32_t see = d->kept[w / 2] & (range_bits(lo, hi, j0 + 16 * w) | range_bits(0, sinks_hi, j0 + 16 * w));
+                        any = any || see != 0;
 #pragma unroll
                         for (int e = 0; e < (w + 1 < CHUNKS ? 32 : 16); ++e) {
                             r[w + e / 16][e % 16] = (see >> e & 1u) != 0 ? r[w + e / 16][e % 16] : 0xff800000u;
                         }
                     }
+                } else {
+                    any = true;
                 }
                 float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -1021,7 +1075,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 }
                 const float here = max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
                 if (!(here < INFINITY)) {
-                    total = NAN;   // an infinite score or a NaN: the row is computed again
+                    total = NAN;   // an infinite score or a NaN: the row is NaN as it is
                 }
                 const bool raise = (here - top) * c > kRaiseBy;   // the first visible key: infinity > 8
                 float shrink = 1.f;
@@ -1103,6 +1157,9 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             if (!ok) {
                 atomicMin(&s_first_bad, turn);
                 break;
+            }
+            if (any && total == 0.f) {
+                total = NAN;   // nothing but scores of minus infinity: 0 / 0
             }
             const float inv = total == 0.f ? 0.f : 1.f / total;
             float most = 0.f;

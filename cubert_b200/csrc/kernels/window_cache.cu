@@ -68,7 +68,8 @@ struct StepPartial {
 
 constexpr int kStepBlocks = 8;   // of a cluster at most
 
-// Parts (maximum, sum, weighted sum of values) joined into one; a part without keys has the sum 0 and counts for nothing.
+// Parts (maximum, sum, weighted sum of values) joined into one; a part without keys has sums of 0 and counts for nothing. At least
+// one key is visible, so a sum of 0 in the end means that all scores are minus infinity, and 0 / 0 is what the row holds then.
 template <int N>
 __device__ __forceinline__ float3 join_parts(const float2 (&stat)[N], const float (&o)[N]) {
     float top = -INFINITY;
@@ -80,10 +81,8 @@ __device__ __forceinline__ float3 join_parts(const float2 (&stat)[N], const floa
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float weight = stat[i].x == -INFINITY ? 0.f : fast_exp2(stat[i].x - top);
-        if (stat[i].y != 0.f) {
-            total = fmaf(weight, stat[i].y, total);
-            sum = fmaf(weight, o[i], sum);
-        }
+        total = fmaf(weight, stat[i].y, total);
+        sum = fmaf(weight, o[i], sum);
     }
     return make_float3(top, total, sum);
 }
@@ -116,7 +115,7 @@ __device__ __forceinline__ void step_join(StepPartial<WARPS, HEADS, DP> *part, i
         for (int u = 0; u < PER_THREAD; ++u) {
             const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
             if (h < heads_here && x < dim) {
-                out[h * dim + x] = from_float<T>(joined[u].y == 0.f ? 0.f : joined[u].z / joined[u].y);
+                out[h * dim + x] = from_float<T>(joined[u].z / joined[u].y);
             }
         }
         return;
@@ -148,7 +147,7 @@ __device__ __forceinline__ void step_join(StepPartial<WARPS, HEADS, DP> *part, i
             }
         }
         const float3 all = join_parts<kStepBlocks>(stat, o);
-        out[e] = from_float<T>(all.y == 0.f ? 0.f : all.z / all.y);
+        out[e] = from_float<T>(all.z / all.y);
     }
     cluster.sync();   // nobody leaves while its sums are read
 }

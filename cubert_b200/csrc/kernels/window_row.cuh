@@ -28,6 +28,7 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
         o[i] = 0.f;
     }
     float top = -INFINITY, total = 0.f;
+    bool any = false;
     for (int part = 0; part < 2; ++part) {
         const int begin = part == 0 ? 0 : lo, end = part == 0 ? sinks_end : hi;
         for (int j0 = begin; j0 < end; j0 += 32) {
@@ -61,14 +62,13 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
                 s = scale * kLog2e * (a0 + a1);
             }
             unsigned visible = __ballot_sync(0xffffffffu, use);
-            const float next = fmaxf(top, group_max<32>(s));
-            if (visible == 0 || next == -INFINITY) {
-                if (!__any_sync(0xffffffffu, use && !(s == -INFINITY))) {   // a NaN score goes on below
-                    continue;
-                }
+            if (visible == 0) {
+                continue;
             }
+            any = true;
+            const float next = fmaxf(top, group_max<32>(s));
             const float shrink = top == -INFINITY ? 0.f : fast_exp2(top - next);
-            const float p = use ? fast_exp2(s - next) : 0.f;
+            const float p = use ? fast_exp2(s - (next == -INFINITY ? 0.f : next)) : 0.f;   // scores of minus infinity: 0
             top = next;
             total = total * shrink + group_sum<32>(p);
 #pragma unroll
@@ -100,7 +100,7 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
             }
         }
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
+    const float inv = any ? 1.f / total : 0.f;   // nothing but scores of minus infinity: 0 times infinity, NaN as 0 / 0 is
 #pragma unroll
     for (int i = 0; i < kWindowMaxDim / 32; ++i) {
         if (lane + 32 * i < dim) {

@@ -334,7 +334,8 @@ int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int cod
 /* ---- K8: attention with a sliding window and sinks ----------------------------------------------------
  * Query i of a sequence sees key j when mask[b, j] != 0 (or mask is NULL), j <= i + after, and j >= i - before or
  * j < sinks: a window around the query plus the sequence's first tokens, which stay visible from any distance.
- *   context[i] = sum_j softmax_j(scale * q_i . k_j) v_j over the keys i sees; zeros when it sees none
+ *   context[i] = sum_j softmax_j(scale * q_i . k_j) v_j over the keys i sees; zeros when it sees none, NaN (0 / 0) when all
+ *   their scores are minus infinity
  * after = 0 is the causal form of decoders; before = after = w the local attention of encoders for long documents
  * (sinks = 1: every token also sees [CLS]); before >= seq lifts the window. Unlike K4, a masked key is left out rather
  * than lowered by 10000, whatever its rows hold (infinities and NaN included). The reference attends to every key of
