@@ -64,6 +64,7 @@ template <int WARPS, int HEADS, int DP>
 struct StepPartial {
     float o[WARPS][HEADS][DP + 2];   // two columns of padding spread the rows over the banks
     float2 stat[WARPS][HEADS];       // maximum (log2 domain) and sum
+    static_assert(HEADS <= 32, "a bit a head in step_join");
 };
 
 constexpr int kStepBlocks = 8;   // of a cluster at most
@@ -87,14 +88,26 @@ __device__ __forceinline__ float3 join_parts(const float2 (&stat)[N], const floa
     return make_float3(top, total, sum);
 }
 
-// First the warps of a block, in its own shared memory, then the blocks: each output element's parts are loaded together.
+// First the warps of a block, in its own shared memory, then the blocks: each output element's parts are loaded together. What comes back
+// in the first block are the heads to compute again: not finite although their scores are, in binary16, whose products see a weight
+// of 0 where float32 has a small one, and 0 times an infinite value is NaN.
 template <typename T, int WARPS, int HEADS, int DP>
-__device__ __forceinline__ void step_join(StepPartial<WARPS, HEADS, DP> *part, int heads_here, int dim, T *out) {
+__device__ __forceinline__ unsigned step_join(StepPartial<WARPS, HEADS, DP> *part, unsigned *s_again, int heads_here, int dim, T *out) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int) cluster.num_blocks(), rank = (int) cluster.block_rank();
     constexpr int PER_THREAD = (HEADS * DP + 32 * WARPS - 1) / (32 * WARPS);
     float3 joined[PER_THREAD];
+    auto store = [&](unsigned *again, int h, int at, float total, float sum) {
+        const float x = sum / total;
+        out[at] = from_float<T>(x);
+        if (sizeof(T) == 2 && !(fabsf(x) <= 65504.f) && total > 0.f) {
+            atomicOr(again, 1u << h);
+        }
+    };
+    if (threadIdx.x == 0) {
+        *s_again = 0;
+    }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < PER_THREAD; ++u) {
@@ -115,10 +128,11 @@ __device__ __forceinline__ void step_join(StepPartial<WARPS, HEADS, DP> *part, i
         for (int u = 0; u < PER_THREAD; ++u) {
             const int e = threadIdx.x + u * 32 * WARPS, h = e / DP, x = e % DP;
             if (h < heads_here && x < dim) {
-                out[h * dim + x] = from_float<T>(joined[u].z / joined[u].y);
+                store(s_again, h, h * dim + x, joined[u].y, joined[u].z);
             }
         }
-        return;
+        __syncthreads();
+        return *s_again;
     }
     __syncthreads();   // every warp's part has been read: the first one's place takes the block's
 #pragma unroll
@@ -147,9 +161,17 @@ __device__ __forceinline__ void step_join(StepPartial<WARPS, HEADS, DP> *part, i
             }
         }
         const float3 all = join_parts<kStepBlocks>(stat, o);
-        out[e] = from_float<T>(all.z / all.y);
+        store(cluster.map_shared_rank(s_again, 0), h, e, all.y, all.z);
     }
     cluster.sync();   // nobody leaves while its sums are read
+    return rank == 0 ? *s_again : 0;
+}
+
+// One head again, by a warp of its own over every visible slot.
+__device__ __forceinline__ void step_row_again(const __half *q, const __half *kn, const __half *vn, const __half *kc, const __half *vc, __half *out, float *s_q,
+                                            int dim, float scale, int slot, int n) {
+    window_row<__half>(q, s_q, dim, scale, 0, 0, n, [&](int j) { return j == slot ? kn : kc + (int64_t) j * dim; },
+                       [&](int j) { return j == slot ? vn : vc + (int64_t) j * dim; }, [&](int) { return true; }, out);
 }
 
 struct StepPlace {
@@ -210,13 +232,15 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
 // (g, t) = (lane / 4, lane % 4) reads 16 bytes (chunk t, t + 4, ..) of the K rows g and g + 8: eight columns that are two steps
 // of the reduction, in an order that Q shares. Of V it reads chunk g (g + 8) of the rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and pairs
 // the halves of two rows: word i of a chunk is rows g and g + 8 of the i-th 16 output columns. So K and V go from memory to
-// operands with no stop in shared memory; P^T turns around in registers.
+// operands with no stop in shared memory; P^T turns around in registers. Registers are bounded so that five blocks of four warps share an SM
+// for heads of 64 (16 streams of 12 heads, 1024 slots: 11.0 us, with four 15.3).
 template <int WARPS, int DP, int NT>
-__global__ void __launch_bounds__(32 * WARPS, (DP == 64 ? 16 : (NT == 1 ? 12 : 8)) / WARPS)
+__global__ void __launch_bounds__(32 * WARPS, (DP == 64 ? (NT == 1 ? 20 : 16) : (NT == 1 ? 12 : 8)) / WARPS)
 window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const int32_t *positions, __half *k_cache, __half *v_cache,
                        __half *context, const __grid_constant__ RingShape s, int chunks) {
     constexpr int HEADS = 8 * NT, KC = DP / 32, VC = DP / 64;
     __shared__ StepPartial<WARPS, HEADS, DP> part;
+    __shared__ unsigned s_again;
     StepPlace at;
     if (!step_place<WARPS, HEADS>(positions, s, chunks, at)) {
         return;
@@ -386,7 +410,16 @@ window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const 
             }
         }
     }
-    step_join<__half, WARPS, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
+    __half *out = context + at.b * s.context_stride + (int64_t) at.first_head * s.dim;
+    const unsigned again = step_join<__half, WARPS, HEADS, DP>(&part, &s_again, at.heads_here, s.dim, out);
+    if (again != 0) {   // the parts have been read: their place holds the queries
+        for (int h = warp; h < at.heads_here; h += WARPS) {
+            if ((again >> h & 1u) != 0) {
+                step_row_again(q + at.b * s.q_stride + (int64_t) (at.first_head + h) * s.dim, kn, vn, kc, vc, out + h * s.dim,
+                               part.o[warp][0], s.dim, s.scale, at.slot, at.n);
+            }
+        }
+    }
 }
 
 // float32: LPK lanes share a key, four columns each, so that a warp reads 32 / LPK whole rows per instruction; every group of
@@ -398,6 +431,7 @@ window_step_f32_kernel(const float *q, const float *k, const float *v, const int
                        const __grid_constant__ RingShape s, int chunks) {
     constexpr int DP = 4 * LPK, GROUPS = 32 / LPK, U = HEADS == 1 ? 8 : 4;   // U: rows per lane group in flight
     __shared__ StepPartial<WARPS, HEADS, DP> part;
+    __shared__ unsigned s_again;
     StepPlace at;
     if (!step_place<WARPS, HEADS>(positions, s, chunks, at)) {
         return;
@@ -484,7 +518,7 @@ window_step_f32_kernel(const float *q, const float *k, const float *v, const int
             *reinterpret_cast<float2 *>(&part.o[warp][h][col + 2]) = make_float2(r[3], r[4]);
         }
     }
-    step_join<float, WARPS, HEADS, DP>(&part, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
+    step_join<float, WARPS, HEADS, DP>(&part, &s_again, at.heads_here, s.dim, context + at.b * s.context_stride + (int64_t) at.first_head * s.dim);
 }
 
 // Blocks of a cluster: doubled until the grid has two blocks per SM, and on to about five while every warp keeps 6 KB of keys (below

@@ -363,7 +363,9 @@ int cubk_window_attention_f16(const void *q, const void *k, const void *v, int64
  * attention of row b of q over the stream's first min(position + 1, sinks + window) slots to row b of context: the
  * causal form above with before = window - 1. A stream with a negative position is idle: its cache and its row of
  * context are left as they are. Slots that no position has reached may hold anything. Positions are read on the
- * device, so a captured call can be replayed as they advance; calls that share a cache must be ordered. */
+ * device, so a captured call can be replayed as they advance; calls that share a cache must be ordered.
+ * Binary16 heads that come out not finite from finite scores (an infinity or a NaN in a visible value) are computed again with float32
+ * weights by a warp each, which is slow; weights below 2^-126 of a row's largest count as 0 in every form. */
 int cubk_window_attention_step_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride,
                                    const int32_t *positions, int batch, int heads, int kv_heads, int head_dim, int window, int sinks,
                                    float scale, float *k_cache, float *v_cache, float *context, int64_t context_stride, void *stream);

@@ -1,4 +1,4 @@
-"""Corners of K8: visible scores of minus infinity. Bars as in test_norm_w4_window_gpu."""
+"""Corners of K8: visible scores of minus infinity, infinite values of little weight. Bars as in test_norm_w4_window_gpu."""
 import pytest
 import torch
 
@@ -71,3 +71,43 @@ def test_steps_that_see_only_scores_of_minus_infinity_are_nan(heads, kv_heads, d
     ref = attention64(q.reshape(batch, heads, 1, dim).double(), kc.double().repeat_interleave(share, 1), vc.double().repeat_interleave(share, 1),
                       seen[:, None, None, :], dim ** -0.5, dim)
     check_window(ctx[1:], tuple(a[1:] for a in ref), t)
+
+
+# ============================================================================ K8: infinite values of little weight
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,window,batch", [(2, 2, 64, 40, 2), (8, 2, 128, 300, 2), (16, 1, 64, 1000, 2), (32, 2, 128, 500, 2),
+                                                             (2, 2, 64, 3000, 2), (4, 4, 64, 200, 120), (3, 1, 32, 17, 2), (2, 1, 5, 33, 2)])
+def test_step_infinite_value_whose_weight_binary16_cannot_hold(heads, kv_heads, dim, window, batch, t):
+    """A weight of 2^-40 times infinity is infinity, in its own column alone; a NaN value is NaN there."""
+    sinks = 1
+    slots, g = window + sinks, gen(window + heads)
+    q, k, v = normal(g, batch, heads * dim, t=t), normal(g, batch, kv_heads * dim, t=t), normal(g, batch, kv_heads * dim, t=t)
+    kc, vc = normal(g, batch, kv_heads, slots, dim, t=t), normal(g, batch, kv_heads, slots, dim, t=t)
+    scale = 1.0 / dim
+    q.view(batch, heads, dim)[:, :, 0] = 4.0
+    kc[:, :, :, 0], k.view(batch, kv_heads, dim)[:, :, 0] = 2.0, 2.0
+    far = [3, slots - 2]                                         # their scores lie 28 below the others': a weight of 2^-40
+    for j in far:
+        kc[:, :, j] = 0
+        kc[:, :, j, 0] = 2.0 - 7.0 * dim
+    pos = torch.full((batch,), 10 * slots, dtype=torch.int32, device="cuda")
+    at = sinks + (10 * slots - sinks) % window
+    assert at not in far
+    args = (batch, heads, kv_heads, dim, window, sinks, scale)
+    kc[:, :, at], vc[:, :, at] = k.view(batch, kv_heads, dim), v.view(batch, kv_heads, dim)
+    share = heads // kv_heads
+    vc[:, :, far, 1], vc[0, :, far[1], 2] = 0, 0
+    ref = attention64(q.reshape(batch, heads, 1, dim).double(), kc.double().repeat_interleave(share, 1), vc.double().repeat_interleave(share, 1),
+                      torch.ones((batch, 1, 1, slots), dtype=torch.bool, device="cuda"), scale, dim)
+    vc[:, :, far[0], 1] = INF
+    vc[0, :, far[1], 2] = float("nan")
+    ctx = torch.zeros((batch, heads * dim), dtype=q.dtype, device="cuda")
+    step(q, k, v, pos, *args, kc, vc, ctx, t)
+    got, odd = ctx.view(batch, heads, dim), torch.zeros((batch, heads, dim), dtype=torch.bool, device="cuda")
+    assert bool((got[:, :, 1] == INF).all()) and torch.isnan(got[0, :, 2]).all()
+    odd[:, :, 1] = True
+    odd[0, :, 2] = True
+    odd = odd.view(batch, -1)
+    assert torch.isfinite(ctx[~odd]).all()
+    check_window(ctx.masked_fill(odd, 0), tuple(a.masked_fill(odd, 0) for a in ref), t)
