@@ -408,8 +408,8 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 //     fits beside the contexts: 128 for heads of up to 64 (two blocks of one tile share an SM), 80 for 128 (one of two tiles).
 //   * Steps of an item: first the sinks below the window, then the window, then one without keys that ends it. A step whose keys are
 //     all masked is left out; one that every row of a tile sees whole skips the masking.
-//   * The running maximum of a row is raised only when a step's maximum exceeds it by 2^8 (a weight is then at most 256, far
-//     inside binary16, and the sums are float32), so that O is read back and scaled in few steps.
+//   * The running maximum of a row is raised only when a step's maximum exceeds it by 2^8, so that O is read back and scaled in few steps;
+//     weights are 2^7 times as large as they need be (at most 2^15, inside binary16), so that small ones last; the sums are float32.
 //   * Weights of unseen keys are exactly 0, but 0 times an infinity or NaN in an unseen V row is NaN. V rows of masked keys, and of
 //     those outside the item's keys, are cleared in shared memory while the weights are awaited. That leaves keys that some rows of a
 //     tile see and others do not: a row that comes out not finite from finite scores is computed again by one warp over its visible
@@ -1083,7 +1083,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     shrink = fast_exp2((top - here) * c);
                     top = here;
                 }
-                const float2 c2 = splat2(c), nt2 = splat2(top == -INFINITY ? 0.f : -top * c);
+                const float2 c2 = splat2(c), nt2 = splat2(top == -INFINITY ? 0.f : fmaf(-top, c, kWeightScale));
                 float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < CHUNKS; ++w) {

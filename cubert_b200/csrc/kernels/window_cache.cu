@@ -341,7 +341,7 @@ window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {   // e: head 2 t + e % 2, key g + 8 (e / 2)
                 sc[m][e] = j0 + g + 8 * (e >> 1) < at.n ? sc[m][e] * c2 : -INFINITY;
-                raise = raise || sc[m][e] - top[m][e & 1] > kRaiseBy;
+                raise = raise || sc[m][e] - top[m][e & 1] > kRaiseBy + kWeightScale;
             }
         }
         if (__any_sync(0xffffffffu, raise)) {
@@ -349,7 +349,7 @@ window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const 
             for (int m = 0; m < NT; ++m) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float here = fmaxf(fmaxf(sc[m][e], sc[m][e + 2]), top[m][e]);
+                    float here = fmaxf(fmaxf(sc[m][e], sc[m][e + 2]) - kWeightScale, top[m][e]);   // 2^7 below the largest
                     here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 4));
                     here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 8));
                     here = fmaxf(here, __shfl_xor_sync(0xffffffffu, here, 16));

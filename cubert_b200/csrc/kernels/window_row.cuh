@@ -7,7 +7,10 @@
 namespace cubk {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaiseBy = 8.f;   // log2 of the largest weight before a running maximum is raised
+// Weights of binary16 products are 2^kWeightScale times what they are relative to the running maximum, and that is raised when a
+// weight passes 2^kRaiseBy of it: at most 2^15, and what is smaller than 2^-32 of the largest is lost instead of 2^-25 (40000 keys of
+// 2^-25.5 beside one key make 2^-10 of a row). The scale cancels in the division by the sum.
+constexpr float kWeightScale = 7.f, kRaiseBy = 8.f;
 constexpr int kWindowMaxDim = 256;
 constexpr int kWindowRowWarps = 4;
 

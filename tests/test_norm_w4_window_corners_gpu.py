@@ -1,8 +1,12 @@
-"""Corners of K8: visible scores of minus infinity, infinite values of little weight. Bars as in test_norm_w4_window_gpu."""
+"""Corners of K8: visible scores of minus infinity, infinite values of little weight, many
+small weights. Bars as in test_norm_w4_window_gpu."""
+import math
+
 import pytest
 import torch
 
-from test_norm_w4_window_gpu import TYPES, attention64, check_window, gen, normal, step, window64, window_attention, window_inputs
+import gpu_harness as G
+from test_norm_w4_window_gpu import TYPES, attention64, check_window, gen, normal, step, window64, window_attention, window_inputs, within
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -111,3 +115,44 @@ def test_step_infinite_value_whose_weight_binary16_cannot_hold(heads, kv_heads, 
     odd = odd.view(batch, -1)
     assert torch.isfinite(ctx[~odd]).all()
     check_window(ctx.masked_fill(odd, 0), tuple(a.masked_fill(odd, 0) for a in ref), t)
+
+
+# ============================================================================ K8: many small weights
+
+def small_weight_bar(want, count):
+    # Weights of binary16 products are held 2^7 below the largest at the least, so one of them is off by 2^-32 of the largest or by
+    # 2^-11 of itself; then the result, the sums (2^-23 for each 16 products) and the exponentials (arguments of up to 30: 2^-17).
+    return count * 2.0 ** -32 + want * (2 * 2.0 ** -11 + (count / 16 + 64) * 2.0 ** -23 + 2.0 ** -16) + 2.0 ** -25
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_small_weights_are_not_lost(dim, t):
+    """One key far above all others, whose value is 0; the others weigh 2^-25.5 each and together 2^-10 of a row."""
+    seq = 40000
+    q, k, v = (torch.zeros((seq, dim), dtype=G.TORCH_DTYPE[t], device="cuda") for _ in range(3))
+    q[:, 0], k[0, 0], v[1:] = 4.0, 25.5 * math.log(2) / 4, 1.0
+    got = window_attention(q, k, v, None, 1, seq, 1, 1, dim, seq, 0, 0, 1.0, t).double()
+    w = math.exp(-4.0 * float(k[0, 0]))
+    others = torch.arange(seq, dtype=torch.float64, device="cuda")
+    want = (others * w / (1 + others * w))[:, None].expand_as(got)
+    within(got, want, small_weight_bar(want, others[:, None]))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 64), (4, 2, 128)])
+def test_many_small_weights_of_a_step_are_not_lost(heads, kv_heads, dim, t):
+    batch, slots = 440 // kv_heads, 20000
+    dt = G.TORCH_DTYPE[t]
+    kc, vc = torch.zeros((batch, kv_heads, slots, dim), dtype=dt, device="cuda"), torch.ones((batch, kv_heads, slots, dim), dtype=dt, device="cuda")
+    q, k, v = torch.zeros((batch, heads * dim), dtype=dt, device="cuda"), torch.zeros((batch, kv_heads * dim), dtype=dt, device="cuda"), None
+    v = torch.ones_like(k)
+    q[:, 0::dim] = 4.0
+    kc[:, :, 100, 0] = 25.5 * math.log(2) / 4
+    vc[:, :, 100] = 0
+    pos = torch.full((batch,), 3 * slots, dtype=torch.int32, device="cuda")
+    ctx = torch.zeros((batch, heads * dim), dtype=dt, device="cuda")
+    step(q, k, v, pos, batch, heads, kv_heads, dim, slots, 0, 1.0, kc, vc, ctx, t)
+    w = (slots - 1) * math.exp(-4.0 * float(kc[0, 0, 100, 0]))
+    want = torch.full_like(ctx, w / (1 + w), dtype=torch.float64)
+    within(ctx, want, small_weight_bar(want, slots))
