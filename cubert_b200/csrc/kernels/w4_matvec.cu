@@ -141,17 +141,25 @@ struct XLoad<X_F32> {
         }
         return r;
     }
-    // the top 16 bits of a float32 are a bfloat16; what is left of 24 bits of mantissa after two of them fits a third
+    // the top 16 bits of a float32 are a bfloat16 (of a NaN, only with its quiet bit set; without it they may be an infinity); what is left
+    // of 24 bits of mantissa after two of them fits a third
     static __device__ __forceinline__ void operands(Raw r, uint32_t (&b)[3][4]) {
 #pragma unroll
         for (int s = 0; s < 3; ++s) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                if (s == 0) {
+                    r.v[2 * i] = quiet(r.v[2 * i]);
+                    r.v[2 * i + 1] = quiet(r.v[2 * i + 1]);
+                }
                 b[s][i] = __byte_perm(__float_as_uint(r.v[2 * i]), __float_as_uint(r.v[2 * i + 1]), 0x7632);
                 r.v[2 * i] = rest(r.v[2 * i]);
                 r.v[2 * i + 1] = rest(r.v[2 * i + 1]);
             }
         }
+    }
+    static __device__ __forceinline__ float quiet(float v) {
+        return v != v ? __uint_as_float(0x7fffffffu) : v;
     }
     static __device__ __forceinline__ float rest(float v) {
         const uint32_t top = __float_as_uint(v) & 0xffff0000u;

@@ -1,12 +1,13 @@
-"""Corners of K8: visible scores of minus infinity, infinite values of little weight, many
-small weights. Bars as in test_norm_w4_window_gpu."""
+"""Corners of K8 (visible scores of minus infinity, infinite values of little weight, many small weights) and of K7 (NaN bit
+patterns). Bars as in test_norm_w4_window_gpu."""
 import math
 
 import pytest
 import torch
 
 import gpu_harness as G
-from test_norm_w4_window_gpu import TYPES, attention64, check_window, gen, normal, step, window64, window_attention, window_inputs, within
+from test_norm_w4_window_gpu import (TYPES, attention64, check_window, gen, matvec, normal, pack, step, window64, window_attention, window_inputs,
+                                     within)
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -156,3 +157,20 @@ def test_many_small_weights_of_a_step_are_not_lost(heads, kv_heads, dim, t):
     w = (slots - 1) * math.exp(-4.0 * float(kc[0, 0, 100, 0]))
     want = torch.full_like(ctx, w / (1 + w), dtype=torch.float64)
     within(ctx, want, small_weight_bar(want, slots))
+
+
+# ============================================================================ K7
+
+@pytest.mark.parametrize("rows,k,n", [(1, 128, 16), (3, 1000, 77), (20, 300, 40)])
+def test_w4_matvec_every_nan_stays_nan(rows, k, n):
+    """A float32 is a NaN by any of its 23 bits, the low 16 among them."""
+    g = gen(k)
+    codes = torch.randint(-8, 8, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    scales = torch.rand((-(-k // 64), n), generator=g, device="cuda") + 0.5
+    packed, x = pack(codes), normal(g, rows, k)
+    clean = matvec(x, packed, scales, 64, n, None, "f32")
+    for bits in (0x7f800001, 0xff800001 - 2 ** 32, 0x7f80ffff, 0x7fc00000, 0x7fffffff, -1):
+        y = x.clone()
+        y.view(torch.int32)[0, k // 2] = bits
+        got = matvec(y, packed, scales, 64, n, None, "f32")
+        assert torch.isnan(got[0]).all() and torch.equal(got[1:], clean[1:]), hex(bits)
