@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "bounded_wait.h"
 #include "cubert_kernels.h"
 
 namespace cubk {
@@ -352,29 +353,23 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
     return t;
 }
 
-// Waits for the phase with the given parity to complete. The wait is bounded twice over: by a
-// deadline on the GPU's nanosecond timer (kBarrierWaitNs; read every 64 polls, so a wait that
-// completes at once never reads it) and by a poll count (which alone bounds the short waits of the
-// self-test). Returns false on give-up.
+// Waits for the phase with the given parity to complete. The wait is bounded twice over: by the time
+// it takes on the GPU's nanosecond timer (WaitClock; read every 64 polls, so a wait that completes at
+// once never reads it) and by a poll count (which alone bounds the short waits of the self-test).
+// Returns false on give-up, after a last look.
 constexpr uint32_t kMaxBarrierPolls = 1u << 22;
-constexpr uint64_t kBarrierWaitNs = 200ull * 1000 * 1000;  // 0.2 s: five orders above a copy's latency
 
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t *bar, uint32_t parity, uint32_t polls = kMaxBarrierPolls) {
-    uint64_t deadline = 0;
+    WaitClock clock;
     for (uint32_t i = 0; i < polls; ++i) {
         if (mbar_try_wait(bar, parity)) {
             return true;
         }
-        if ((i & 63u) == 63u) {
-            const uint64_t now = global_timer_ns();
-            if (deadline == 0) {
-                deadline = now + kBarrierWaitNs;
-            } else if (now > deadline) {
-                return false;
-            }
+        if ((i & 63u) == 63u && clock.over((uint32_t) global_timer_ns())) {
+            break;
         }
     }
-    return false;
+    return mbar_try_wait(bar, parity);
 }
 
 __device__ __forceinline__ uint4 ld_shared_vec(const void *p) {
