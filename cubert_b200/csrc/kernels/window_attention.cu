@@ -5,12 +5,11 @@
 // key gets zeros.
 #include <cuda.h>
 
-#include <limits.h>
-
 #include <atomic>
 #include <type_traits>
 
 #include "window_row.cuh"
+#include "window_turns.h"
 
 namespace cubk {
 
@@ -421,8 +420,10 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 // lengths 81 us (3 steps an item that ran; half of it goes into the ends of items). Rows computed
 // again are far slower: one causal sequence of 40000 tokens, 2 heads of 64, all of it from token 100 on: 542 ms (1.2 ms without). Tried
 // and slower: two threads a row, part of the exponentials by polynomial, scores of 96 keys twice, masks gathered by a warp of their own.
-// Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, frees its tensor memory and
-// returns.
+// Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, counts in g_window_give_ups,
+// frees its tensor memory and returns.
+__device__ unsigned int g_window_give_ups = 0;     // blocks, on this device
+
 constexpr int kTileRows = 128;
 constexpr int kHalfTileBytes = kTileRows * 128;    // 128 rows x 64 binary16
 constexpr int kStepSlots = 8;                      // descriptors of steps in flight; more than the stages + 2
@@ -655,7 +656,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     __shared__ uint64_t s_sfull[NQ], s_sfree[NQ], s_pfull[NQ], s_ofull[NQ];   // scores written, scores read, weights written, O added to
     __shared__ __align__(16) uint4 s_taken[2];
     __shared__ uint64_t s_takes;
-    __shared__ int s_items[4], s_turns, s_first_bad;   // items begun, the latest four; the first that a give-up left without rows
+    __shared__ WindowTurns s_turns;
     __shared__ uint32_t s_tmem;
     __shared__ WindowStep s_steps[kStepSlots];
     __shared__ float s_row[C::SOFTMAX_WARPS][kWindowMaxDim];
@@ -678,8 +679,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (threadIdx.x == 32) {
-        s_turns = 0;
-        s_first_bad = INT_MAX;
+        s_turns.reset();
         s_stop = 0;
         for (int w = 0; w < C::SOFTMAX_WARPS; ++w) {
             s_agains[w] = 0;
@@ -720,8 +720,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             for (int item = blockIdx.x; item >= 0 && ok; ++turn) {
                 const WindowItem<NQ> w(item, s, row_blocks, pair_heads);
                 if (lane == 0) {
-                    s_items[turn & 3] = item;
-                    s_turns = turn + 1;
+                    s_turns.add(turn, item);
                 }
                 const int lo = w.row0 > s.before ? (w.row0 - s.before) & ~15 : 0;   // whole vectors of the mask
                 const int hi = s.after < s.seq - 1 - w.last_row ? w.last_row + s.after + 1 : s.seq;
@@ -910,8 +909,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             }
             if (!ok) {   // the copies in flight land before the block's shared memory goes
                 if (turn > 0 && wait_together(&s_takes, (turn - 1) & 1) && lane == 0 && taken_block(&s_taken[(turn - 1) & 1]) >= 0) {
-                    s_items[turn & 3] = taken_block(&s_taken[(turn - 1) & 1]);   // taken over and not begun
-                    s_turns = turn + 1;
+                    s_turns.add(turn, taken_block(&s_taken[(turn - 1) & 1]));   // taken over and not begun
                 }
                 for (int i = max(turn - C::QUERIES, 0); i <= turn; ++i) {
                     (void) wait_together(&s_qfull[i % C::QUERIES], (i / C::QUERIES) & 1);
@@ -1018,7 +1016,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         for (int turn = 0;; ++step, ++turn) {
             ok = wait_together(&s_sfull[t], step & 1);   // an item's first step says which it is
             if (!ok) {
-                atomicMin(&s_first_bad, turn);
+                atomicMin(&s_turns.first_bad, turn);
                 break;
             }
             if (s_steps[step % kStepSlots].columns < 0) {
@@ -1155,7 +1153,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             }
             // ---- context rows (the last completion waited for covers every product into O)
             if (!ok) {
-                atomicMin(&s_first_bad, turn);
+                atomicMin(&s_turns.first_bad, turn);
                 break;
             }
             if (any && total == 0.f) {
@@ -1251,8 +1249,11 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     }
     tmem_fence_before();
     __syncthreads();
-    for (int turn = s_first_bad; turn < s_turns; ++turn) {   // after a give-up only
-        const WindowItem<NQ> w(s_items[turn & 3], s, row_blocks, pair_heads);
+    if (threadIdx.x == 0 && s_turns.first_bad != kNoTurn) {
+        atomicAdd(&g_window_give_ups, 1u);
+    }
+    for (int turn = s_turns.first_bad; turn < s_turns.known; ++turn) {   // after a give-up only
+        const WindowItem<NQ> w(s_turns.item(turn), s, row_blocks, pair_heads);
         for (int e = threadIdx.x; e < NQ * kTileRows * s.dim; e += C::THREADS) {
             const int t = e / (kTileRows * s.dim), r = e / s.dim % kTileRows, i = w.tile_row[t] + r;
             if (i < s.seq) {
@@ -1392,6 +1393,18 @@ int window_attention(const T *q, const T *k, const T *v, int64_t q_stride, int64
 }  // namespace cubk
 
 extern "C" {
+
+int cubk_window_give_ups(unsigned int *count) {
+    if (count == nullptr) {
+        return CUBK_ERR_INVALID_ARG;
+    }
+    const cudaError_t err = cudaMemcpyFromSymbol(count, cubk::g_window_give_ups, sizeof(unsigned int));
+    if (err != cudaSuccess) {
+        cubk::set_last_error(err);
+        return CUBK_ERR_LAUNCH;
+    }
+    return CUBK_OK;
+}
 
 int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
                               int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,

@@ -65,6 +65,7 @@ _SIGNATURES = {
     "cubk_w4_matvec_{t}": (_I, [_P, _I, _I, _P, _P, _I, _I, _P, _P, _P]),
     "cubk_w4_matvec_e4m3_{t}": (_I, [_P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P]),
     "cubk_window_attention_{t}": (_I, [_P, _P, _P, _L, _L, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _L, _P]),
+    "cubk_window_give_ups": (_I, [_P]),
     "cubk_window_attention_step_{t}": (_I, [_P, _P, _P, _L, _L, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _L, _P]),
     "cubk_window_cache_fill_{t}": (_I, [_P, _P, _L, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
     "cubk_not_{t}": (_I, [_P, _P, _L, _P]),
@@ -132,4 +133,11 @@ def copy_timeouts():
     """Warps on the current device that gave up waiting for a shared-memory copy (expected: 0)."""
     n = C.c_uint(0)
     check(load().cubk_copy_timeouts(C.byref(n)))
+    return n.value
+
+
+def window_give_ups():
+    """Blocks of the binary16 window attention on the current device that gave up a bounded wait (expected: 0)."""
+    n = C.c_uint(0)
+    check(load().cubk_window_give_ups(C.byref(n)))
     return n.value

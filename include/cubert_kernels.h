@@ -346,7 +346,7 @@ int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int cod
  * to 256 (CUBK_ERR_UNSUPPORTED beyond). mask int8 [batch, seq]. context must not overlap the inputs.
  *   _f16, head_dim a multiple of 8 up to 128, q, k, v on 16-byte boundaries, strides multiples of 8, scale > 0: tcgen05 with
  *     scores, weights and contexts in tensor memory; weights are rounded to binary16. Every wait is bounded (0.2 s): a
- *     block that gives up writes NaN into the rows it has not finished.
+ *     block that gives up writes NaN into the rows it has not finished and counts in cubk_window_give_ups.
  *   otherwise, head_dim up to 128: the float32 pipes, 64 x 64 tiles.
  *   head_dim above 128, and up to 6 (binary16) or 12 (float32) tokens a sequence: one row per warp. */
 int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
@@ -355,6 +355,10 @@ int cubk_window_attention_f32(const float *q, const float *k, const float *v, in
 int cubk_window_attention_f16(const void *q, const void *k, const void *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
                               int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,
                               void *context, int64_t context_stride, void *stream);
+
+/* Blocks of cubk_window_attention_f16, on the current device and since the library was loaded, that gave up a bounded wait and left NaN
+ * rows. Expected to stay 0; NaN rows come from the inputs then. Synchronises with the device. */
+int cubk_window_give_ups(unsigned int *count);
 
 /* K8 for one new token of each of `batch` streams. The keys and values a stream can still see live in a ring of
  * sinks + window slots, k_cache and v_cache [batch, kv_heads, sinks + window, head_dim]: position p sits in slot p

@@ -13,3 +13,7 @@ def test_rms_norm_refuses_rows_whose_columns_pass_32_bit_arithmetic(channels, t)
     assert getattr(lib, "cubk_residual_rms_norm_" + t)(A, None, A, 1, channels, 1e-6, None, A, None) == kernels.CUBK_ERR_UNSUPPORTED
     for group in (0, 128):
         assert getattr(lib, "cubk_residual_rms_norm_e4m3_" + t)(A, None, A, 1, channels, 1e-6, group, None, A, A, None) == kernels.CUBK_ERR_UNSUPPORTED
+
+
+def test_window_give_ups_needs_a_place_for_the_count():
+    assert kernels.load().cubk_window_give_ups(None) == kernels.CUBK_ERR_INVALID_ARG

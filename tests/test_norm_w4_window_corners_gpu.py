@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import gpu_harness as G
+from cubert_b200 import kernels
 from test_norm_w4_window_gpu import (TYPES, attention64, check_window, gen, matvec, normal, pack, step, window64, window_attention, window_inputs,
                                      within)
 
@@ -174,3 +175,18 @@ def test_w4_matvec_every_nan_stays_nan(rows, k, n):
         y.view(torch.int32)[0, k // 2] = bits
         got = matvec(y, packed, scales, 64, n, None, "f32")
         assert torch.isnan(got[0]).all() and torch.equal(got[1:], clean[1:]), hex(bits)
+
+
+# ============================================================================ K8: give-ups
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_attention_gives_up_no_wait(dim):
+    """NaN rows from the inputs are not give-ups, and nothing else should be there to count."""
+    before = kernels.window_give_ups()
+    q, k, v, m = window_inputs(dim, 4, 2000, 6, 3, dim, "holes", "f16")
+    args = (4, 2000, 6, 3, dim, 300, 20, 2, dim ** -0.5)
+    check_window(window_attention(q, k, v, m, *args, "f16"), window64(q, k, v, m, *args), "f16")
+    k[100] = float("nan")
+    m[0, 100] = 1
+    assert torch.isnan(window_attention(q, k, v, m, *args, "f16")).any()
+    assert kernels.window_give_ups() == before == 0

@@ -1,5 +1,6 @@
 // The host-side build of the kernels' plain arithmetic, for tests through ctypes.
 #include "bounded_wait.h"
+#include "window_turns.h"
 
 extern "C" {
 
@@ -12,6 +13,34 @@ int wait_over_at(const uint64_t *readings, int n) {
         }
     }
     return n + 1;
+}
+
+int turns_size() {
+    return (int) sizeof(cubk::WindowTurns);
+}
+
+void turns_reset(cubk::WindowTurns *t) {
+    t->reset();
+}
+
+void turns_add(cubk::WindowTurns *t, int turn, int item) {
+    t->add(turn, item);
+}
+
+void turns_gave_up(cubk::WindowTurns *t, int turn) {   // atomicMin on the device
+    t->first_bad = turn < t->first_bad ? turn : t->first_bad;
+}
+
+int turns_first_bad(const cubk::WindowTurns *t) {
+    return t->first_bad;
+}
+
+int turns_known(const cubk::WindowTurns *t) {
+    return t->known;
+}
+
+int turns_item(const cubk::WindowTurns *t, int turn) {
+    return t->item(turn);
 }
 
 }
