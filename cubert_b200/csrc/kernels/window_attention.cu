@@ -1308,7 +1308,7 @@ int window_tc_launch(const CUtensorMap &qm, const CUtensorMap &km, const CUtenso
         cudaFuncAttributes attr;
         err = cudaFuncGetAttributes(&attr, window_tc_kernel<DP, NQ>);
         if (err == cudaSuccess && attr.numRegs < C::LAUNCH_REGS) {
-            return CUBK_ERR_UNSUPPORTED;   // compiled to fewer registers than its groups of warps share out among themselves
+            err = cudaErrorInvalidKernelImage;   // compiled to fewer registers than its groups of warps share out among themselves: a broken build
         }
         if (err == cudaSuccess) {
             err = cudaFuncSetAttribute(window_tc_kernel<DP, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);

@@ -190,3 +190,27 @@ def test_window_attention_gives_up_no_wait(dim):
     m[0, 100] = 1
     assert torch.isnan(window_attention(q, k, v, m, *args, "f16")).any()
     assert kernels.window_give_ups() == before == 0
+
+
+# ============================================================================ K8: which kernel runs
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (40, 2, 1), (128, 4, 2), (72, 3, 3)])
+def test_binary16_sequences_on_16_byte_boundaries_run_on_the_tensor_cores(dim, heads, kv_heads):
+    """Only there are weights rounded to binary16. Rows that start 2 bytes later go by the float32 pipes: the same up to what is rounded,
+    but not bit by bit, which it would be if both took that way."""
+    batch, seq = 2, 300
+    q, k, v, m = window_inputs(dim, batch, seq, heads, kv_heads, dim, "holes", "f16")
+    parts = [a.contiguous() for a in (q, k, v)]
+    shifted = []
+    for a in parts:
+        room = torch.zeros(a.numel() + 8, dtype=a.dtype, device="cuda")
+        shifted.append(room[1:1 + a.numel()].view(a.shape).copy_(a))
+    assert all(a.data_ptr() % 16 == 0 for a in parts) and all(a.data_ptr() % 16 == 2 for a in shifted)
+    args = (batch, seq, heads, kv_heads, dim, 70, 11, 2, dim ** -0.5)
+    ctx, bar, pv, tiny = window64(*parts, m, *args)
+    fast, slow = window_attention(*parts, m, *args, "f16"), window_attention(*shifted, m, *args, "f16")
+    check_window(slow, (ctx, bar, pv, tiny), "f16")
+    # both within the bar of the float32 steps; the weights' rounding on one side; the results' on both
+    within(fast, slow.double(), 2 * bar + 2.0 ** -11 * pv * (1 + 2.0 ** -6) + tiny + 2 * (2.0 ** -11 * ctx.abs() + 2.0 ** -25) * (1 + 2.0 ** -8))
+    assert not torch.equal(fast, slow)
+    assert torch.equal(slow, window_attention(*shifted, m, *args, "f16"))
