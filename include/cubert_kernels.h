@@ -19,7 +19,7 @@
  *     (rows * channels may exceed 2^31).
  *   - A fast path is taken when pointers are 16-byte aligned and the row length is a
  *     multiple of 16 bytes; any other shape or alignment runs a slower generic kernel
- *     with identical results.
+ *     with identical results (K6 to K8: results that agree within their roundings, as said there).
  *   - `stream` is a `cudaStream_t` passed as `void *` (as the reference does). The stream and every buffer belong to
  *     the device that is current on the calling thread.
  */
@@ -288,6 +288,9 @@ int cubk_pooler_head_f16(const void *x, const void *pooler_bias, const void *wei
  * scales [rows]) or over blocks of 128 columns (group = 128, scales [rows, ceil(channels / 128)], the last block as
  * short as the row leaves it). A group whose largest |y| is below 2^-100 is stored as zeros with scale 0. A NaN in a
  * group makes its scale and codes NaN. The e4m3 codes are what cubk_w4_matvec_e4m3_* and 8-bit library products read.
+ * Rows of other lengths or alignments add their squares in another order: t has the same bits, y and the scales differ by
+ * (channels / 32 + 24) 2^-24 of themselves at most, before they are rounded. Squares are float32: |t| from 2^64 on (a mean of
+ * infinity) gives zeros.
  * eps >= 0; a row of zeros under eps = 0 gives NaN. channels up to 2^30 (CUBK_ERR_UNSUPPORTED beyond). */
 int cubk_residual_rms_norm_f32(const float *x, const float *residual, const float *gamma, int64_t rows, int channels, float eps,
                                float *sum, float *out, void *stream);
@@ -305,7 +308,9 @@ int cubk_residual_rms_norm_e4m3_f16(const void *x, const void *residual, const v
  * (CUBK_ERR_UNSUPPORTED beyond), but with more than a few a library product of binary16 weights, where there is room for
  * them, takes no longer: from 16 rows on at 4096 by 4096, from about 28 at 4096 by 11008; a third of the time at 128 rows.
  * x [rows, k], bias [n] (or NULL), out [rows, n] and the scales [ceil(k / group), n] in the storage type. Sums are
- * float32; a code times its scale is never rounded. out must not overlap the operands.
+ * float32, of x times codes over a group before they meet its scale (float32 x beyond 2^118 can overflow there); a code
+ * times its scale is never rounded. x of any alignment gives the same bits; the order of the sums depends on rows, k and n.
+ * out must not overlap the operands.
  * The _e4m3 calls take x as the 8-bit codes and scales K6 writes: code_scales [rows] (code_group = 0) or
  * [rows, ceil(k / 128)] (code_group = 128).
  * packed: cubk_w4_packed_bytes(n, k) bytes on a 16-byte boundary and scales on a 4-byte one (CUBK_ERR_UNSUPPORTED
@@ -348,7 +353,8 @@ int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int cod
  *     scores, weights and contexts in tensor memory; weights are rounded to binary16. Every wait is bounded (0.2 s): a
  *     block that gives up writes NaN into the rows it has not finished and counts in cubk_window_give_ups.
  *   otherwise, head_dim up to 128: the float32 pipes, 64 x 64 tiles.
- *   head_dim above 128, and up to 6 (binary16) or 12 (float32) tokens a sequence: one row per warp. */
+ *   head_dim above 128, and up to 6 (binary16) or 12 (float32) tokens a sequence: one row per warp.
+ * The three agree within their roundings: float32 sums of another order, and 2^-11 of sum_j p_j |v_j| where weights are rounded. */
 int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
                               int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,
                               float *context, int64_t context_stride, void *stream);
@@ -368,6 +374,8 @@ int cubk_window_give_ups(unsigned int *count);
  * causal form above with before = window - 1. A stream with a negative position is idle: its cache and its row of
  * context are left as they are. Slots that no position has reached may hold anything. Positions are read on the
  * device, so a captured call can be replayed as they advance; calls that share a cache must be ordered.
+ * _f16, head_dim a multiple of 8 up to 128, rows and heads on 16-byte boundaries: weights are rounded to binary16 (2^-11 of each at
+ * most) for the tensor cores; in any other form they are float32.
  * Binary16 heads that come out not finite from finite scores (an infinity or a NaN in a visible value) are computed again with float32
  * weights by a warp each, which is slow; weights below 2^-126 of a row's largest count as 0 in every form. */
 int cubk_window_attention_step_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride,

@@ -7,8 +7,8 @@ import torch
 
 import gpu_harness as G
 from cubert_b200 import kernels
-from test_norm_w4_window_gpu import (TYPES, attention64, check_window, gen, matvec, normal, pack, step, window64, window_attention, window_inputs,
-                                     within)
+from test_norm_w4_window_gpu import (HALF_STEP, SMALLEST, TYPES, attention64, check_window, gen, matvec, norm_bar, normal, pack, rms_norm, step,
+                                     window64, window_attention, window_inputs, within)
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -214,3 +214,56 @@ def test_binary16_sequences_on_16_byte_boundaries_run_on_the_tensor_cores(dim, h
     within(fast, slow.double(), 2 * bar + 2.0 ** -11 * pv * (1 + 2.0 ** -6) + tiny + 2 * (2.0 ** -11 * ctx.abs() + 2.0 ** -25) * (1 + 2.0 ** -8))
     assert not torch.equal(fast, slow)
     assert torch.equal(slow, window_attention(*shifted, m, *args, "f16"))
+
+
+# ============================================================================ the same data by every path
+
+def by_every_start(a):
+    """`a` on a 16-byte boundary, and one element further."""
+    out = []
+    for shift in (0, 1):
+        room = torch.zeros(a.numel() + 16, dtype=a.dtype, device="cuda")
+        out.append(room[shift:shift + a.numel()].view(a.shape).copy_(a))
+    return out
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,ch", [(5, 64), (9, 1024), (3, 8192), (2, 16384)])
+def test_rms_norm_by_every_path_agrees(rows, ch, t):
+    """The sums of squares are added in another order: their error (as norm_bar has it) on both sides, and a rounding on both."""
+    g = gen(rows + ch)
+    x, gamma = normal(g, rows, ch, t=t), 1 + normal(g, ch, std=0.3, t=t)
+    (xa, xb), (ga, gb) = by_every_start(x), by_every_start(gamma)
+    (sum_a, a), (sum_b, b) = rms_norm(xa, None, ga, 1e-6, t), rms_norm(xb, None, gb, 1e-6, t)
+    assert torch.equal(sum_a, sum_b)
+    within(b, a, 2 * (HALF_STEP[t] + norm_bar(ch)) * a.double().abs() * (1 + 2.0 ** -8) + 2 * SMALLEST[t])
+    for group in (0, 128):
+        (_, ca, sa), (_, cb, sb) = rms_norm(xa, None, ga, 1e-6, t, e4m3=group), rms_norm(xb, None, gb, 1e-6, t, e4m3=group)
+        within(sb, sa, 2 * (norm_bar(ch) + 2.0 ** -22) * sa.double().abs())
+        # half a step of a code (2^-4, 2^-10 near 0) on both sides, and the values' own difference
+        within(cb.float(), ca.float(), ca.double().abs() * (2 * 2.0 ** -4 * (1 + 2.0 ** -3) + 4 * norm_bar(ch)) + 2 * 2.0 ** -10 * (1 + 2.0 ** -8))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,window", [(2, 2, 64, 40), (8, 2, 128, 700), (3, 1, 32, 17)])
+def test_steps_by_every_path_agree(heads, kv_heads, dim, window, t):
+    batch, sinks = 3, 2
+    slots, g = window + sinks, gen(window)
+    q, k, v = normal(g, batch, heads * dim, t=t), normal(g, batch, kv_heads * dim, t=t), normal(g, batch, kv_heads * dim, t=t)
+    caches = normal(g, batch, kv_heads, slots, dim, t=t), normal(g, batch, kv_heads, slots, dim, t=t)
+    pos = torch.tensor([slots // 2, 3 * slots, -1], dtype=torch.int32, device="cuda")
+    got = []
+    for kc, vc in zip(*(by_every_start(c) for c in caches)):
+        ctx = torch.zeros((batch, heads * dim), dtype=q.dtype, device="cuda")
+        step(q, k, v, pos, batch, heads, kv_heads, dim, window, sinks, dim ** -0.5, kc, vc, ctx, t)
+        got.append((ctx, kc, vc))
+    assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][2], got[1][2])
+    seen = torch.ones((batch, slots), dtype=torch.bool, device="cuda")
+    seen[0, slots // 2 + 1:] = False
+    share = heads // kv_heads
+    ctx, bar, pv, tiny = attention64(q.reshape(batch, heads, 1, dim).double(), got[0][1].double().repeat_interleave(share, 1),
+                                     got[0][2].double().repeat_interleave(share, 1), seen[:, None, None, :], dim ** -0.5, dim)
+    bar = 2 * bar + 2 * (HALF_STEP[t] * ctx.abs() + SMALLEST[t]) * (1 + 2.0 ** -8)
+    if t == "f16":                                               # weights rounded on one side
+        bar = bar + 2.0 ** -11 * pv * (1 + 2.0 ** -6) + tiny
+    within(got[1][0][:2], got[0][0][:2].double(), bar[:2])
