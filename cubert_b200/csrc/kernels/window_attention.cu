@@ -21,7 +21,7 @@ struct WindowShape {
 };
 
 // Row (b, i) of head h of a whole sequence.
-template <typename T>
+template <typename T, int COLS>
 __device__ __forceinline__ void window_prompt_row(const T *q, const T *k, const T *v, const int8_t *mask, T *context, const WindowShape &s,
                                                   float *s_q, int b, int i, int h) {
     const int64_t first = (int64_t) b * s.seq;
@@ -30,12 +30,12 @@ __device__ __forceinline__ void window_prompt_row(const T *q, const T *k, const 
     const T *kb = k + first * s.kv_stride + (int64_t) kh * s.dim, *vb = v + first * s.kv_stride + (int64_t) kh * s.dim;
     const int lo = i > s.before ? i - s.before : 0;
     const int hi = s.after < s.seq - 1 - i ? i + s.after + 1 : s.seq;
-    window_row<T>(q + (first + i) * s.q_stride + (int64_t) h * s.dim, s_q, s.dim, s.scale, min(min(s.sinks, lo), hi), lo, hi,
+    window_row<T, COLS>(q + (first + i) * s.q_stride + (int64_t) h * s.dim, s_q, s.dim, s.scale, min(min(s.sinks, lo), hi), lo, hi,
                   [&](int j) { return kb + j * s.kv_stride; }, [&](int j) { return vb + j * s.kv_stride; },
                   [&](int j) { return kept == nullptr || kept[j] != 0; }, context + (first + i) * s.context_stride + (int64_t) h * s.dim);
 }
 
-template <typename T>
+template <typename T, int COLS>
 __global__ void __launch_bounds__(32 * kWindowRowWarps)
 window_rows_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *context, WindowShape s) {
     __shared__ float s_q[kWindowRowWarps][kWindowMaxDim];
@@ -43,7 +43,7 @@ window_rows_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *co
     const int64_t total = (int64_t) s.batch * s.seq * s.heads;
     for (int64_t r = (int64_t) blockIdx.x * kWindowRowWarps + warp; r < total; r += (int64_t) gridDim.x * kWindowRowWarps) {
         const int64_t bh = r / s.seq;
-        window_prompt_row<T>(q, k, v, mask, context, s, s_q[warp], (int) (bh / s.heads), (int) (r - bh * s.seq), (int) (bh % s.heads));
+        window_prompt_row<T, COLS>(q, k, v, mask, context, s, s_q[warp], (int) (bh / s.heads), (int) (r - bh * s.seq), (int) (bh % s.heads));
     }
 }
 
@@ -85,7 +85,7 @@ constexpr int kNotFinite = 1, kSumZero = 2;   // what a row came out with
 // The rows of a block that need another look, out of the way of the others' code. A row that is not finite is computed again over its
 // visible keys alone. A row with a sum of 0 sees no key, and is zeros, or nothing but scores of minus infinity, and is NaN (0 / 0):
 // which, the mask says, 4096 candidates at a time as bits in the list's place, a word a lane.
-template <typename T>
+template <typename T, int DP>
 __device__ __noinline__ void window_plain_again(const T *q, const T *k, const T *v, const int8_t *mask, T *context, const WindowShape *s, float *s_q,
                                                 int *s_list, int *s_bad, int b, int h, int row0) {
     constexpr int WARPS = kPlainThreads / 32, WORDS = 128;
@@ -125,7 +125,7 @@ __device__ __noinline__ void window_plain_again(const T *q, const T *k, const T 
     }
     for (int r = warp; r < kPlainRows; r += WARPS) {
         if (s_bad[r] == kNotFinite) {
-            window_prompt_row<T>(q, k, v, mask, context, *s, s_q + warp * kWindowMaxDim, b, row0 + r, h);
+            window_prompt_row<T, DP / 32>(q, k, v, mask, context, *s, s_q + warp * kWindowMaxDim, b, row0 + r, h);
         }
     }
 }
@@ -357,7 +357,7 @@ window_plain_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *c
         }
     }
     if (__syncthreads_or(rest && met)) {   // Q is no longer read: its place serves the rows that are computed again
-        window_plain_again<T>(q, k, v, mask, context, &s, s_q, s_list, s_bad, b, h, row0);
+        window_plain_again<T, DP>(q, k, v, mask, context, &s, s_q, s_list, s_bad, b, h, row0);
     }
 }
 
@@ -618,9 +618,10 @@ __device__ __forceinline__ void clear_rows(unsigned char *tile, const uint32_t (
 }
 
 // One row again over its visible keys alone (rows whose tile held an infinity or NaN).
+template <int DP>
 __device__ __noinline__ void window_row_again(const __half *q, const __half *k, const __half *v, const int8_t *mask, __half *context,
                                               const WindowShape *s, float *s_q, int b, int i, int h) {
-    window_prompt_row<__half>(q, k, v, mask, context, *s, s_q, b, i, h);
+    window_prompt_row<__half, DP / 32>(q, k, v, mask, context, *s, s_q, b, i, h);
 }
 
 // The rows and heads of a work item.
@@ -1242,7 +1243,7 @@ window_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             for (int n = 0; n < s_agains[warp]; ++n) {
                 const int4 rows = s_again[warp][n % kAgainItems];
                 for (unsigned bad = (unsigned) rows.w; bad != 0; bad &= bad - 1) {
-                    window_row_again(q, k, v, mask, context, &s, s_row[warp], rows.x, rows.y + __ffs(bad) - 1, rows.z);
+                    window_row_again<DP>(q, k, v, mask, context, &s, s_row[warp], rows.x, rows.y + __ffs(bad) - 1, rows.z);
                 }
             }
         }
@@ -1370,9 +1371,9 @@ int window_attention(const T *q, const T *k, const T *v, int64_t q_stride, int64
     }
     const WindowShape s = {batch, seq, heads, kv_heads, dim, before, after, sinks, scale, q_stride, kv_stride, context_stride};
     // A tile of rows takes as long for one token as for 64 or 128; a warp per row is faster for a few. 12 heads of 64, float32: 1 x 8
-    // tokens 5.4 us against 10.7 in tiles, 1024 x 8 154 against 358, but 1024 x 16 381 against 378. Binary16: 1 x 4 4.1 against 6.2,
-    // 1024 x 6 99 against 121, but 1024 x 8 138 against 121.
-    if (seq > (sizeof(T) == 2 ? 6 : 12)) {
+    // tokens 4.8 us against 10.3 in tiles, 1024 x 16 328 against 363, but 1024 x 24 628 against 382. Binary16: 1 x 4 4.2 against 6.4,
+    // 1024 x 8 96 against 124, but 1024 x 12 162 against 124.
+    if (seq > (sizeof(T) == 2 ? 8 : 16)) {
         if constexpr (sizeof(T) == 2) {
             const int rc = window_tc(q, k, v, mask, context, s, stream);
             if (rc != CUBK_ERR_UNSUPPORTED) {
@@ -1386,7 +1387,8 @@ int window_attention(const T *q, const T *k, const T *v, int64_t q_stride, int64
     }
     const int64_t groups = ((int64_t) batch * seq * heads + kWindowRowWarps - 1) / kWindowRowWarps;
     const unsigned blocks = (unsigned) (groups < 148 * 64 ? groups : 148 * 64);
-    window_rows_kernel<T><<<blocks, 32 * kWindowRowWarps, 0, stream>>>(q, k, v, mask, context, s);
+    const auto kernel = dim <= 64 ? window_rows_kernel<T, 2> : dim <= 128 ? window_rows_kernel<T, 4> : window_rows_kernel<T, 8>;
+    kernel<<<blocks, 32 * kWindowRowWarps, 0, stream>>>(q, k, v, mask, context, s);
     return check_launch();
 }
 

@@ -22,7 +22,7 @@ __device__ __forceinline__ int ring_slot(int p, int window, int sinks) {
 
 // One (stream, head) per warp. The new token's key and value are read where they came from, never from the slot that the
 // warp of the group's first head writes.
-template <typename T>
+template <typename T, int COLS>
 __global__ void __launch_bounds__(32 * kWindowRowWarps)
 window_step_rows_kernel(const T *q, const T *k, const T *v, const int32_t *positions, T *k_cache, T *v_cache, T *context, RingShape s) {
     __shared__ float s_q[kWindowRowWarps][kWindowMaxDim];
@@ -46,7 +46,7 @@ window_step_rows_kernel(const T *q, const T *k, const T *v, const int32_t *posit
                 vc[(int64_t) slot * s.dim + c] = vn[c];
             }
         }
-        window_row<T>(q + b * s.q_stride + (int64_t) h * s.dim, s_q[warp], s.dim, s.scale, 0, 0, n,
+        window_row<T, COLS>(q + b * s.q_stride + (int64_t) h * s.dim, s_q[warp], s.dim, s.scale, 0, 0, n,
                       [&](int j) { return j == slot ? kn : kc + (int64_t) j * s.dim; },
                       [&](int j) { return j == slot ? vn : vc + (int64_t) j * s.dim; }, [&](int) { return true; },
                       context + b * s.context_stride + (int64_t) h * s.dim);
@@ -168,9 +168,10 @@ __device__ __forceinline__ unsigned step_join(StepPartial<WARPS, HEADS, DP> *par
 }
 
 // One head again, by a warp of its own over every visible slot.
+template <int DP>
 __device__ __forceinline__ void step_row_again(const __half *q, const __half *kn, const __half *vn, const __half *kc, const __half *vc, __half *out, float *s_q,
                                             int dim, float scale, int slot, int n) {
-    window_row<__half>(q, s_q, dim, scale, 0, 0, n, [&](int j) { return j == slot ? kn : kc + (int64_t) j * dim; },
+    window_row<__half, DP / 32>(q, s_q, dim, scale, 0, 0, n, [&](int j) { return j == slot ? kn : kc + (int64_t) j * dim; },
                        [&](int j) { return j == slot ? vn : vc + (int64_t) j * dim; }, [&](int) { return true; }, out);
 }
 
@@ -415,7 +416,7 @@ window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const 
     if (again != 0) {   // the parts have been read: their place holds the queries
         for (int h = warp; h < at.heads_here; h += WARPS) {
             if ((again >> h & 1u) != 0) {
-                step_row_again(q + at.b * s.q_stride + (int64_t) (at.first_head + h) * s.dim, kn, vn, kc, vc, out + h * s.dim,
+                step_row_again<DP>(q + at.b * s.q_stride + (int64_t) (at.first_head + h) * s.dim, kn, vn, kc, vc, out + h * s.dim,
                                part.o[warp][0], s.dim, s.scale, at.slot, at.n);
             }
         }
@@ -622,7 +623,8 @@ int window_attention_step(const T *q, const T *k, const T *v, int64_t q_stride, 
     }
     const int64_t groups = ((int64_t) batch * heads + kWindowRowWarps - 1) / kWindowRowWarps;
     const unsigned blocks = (unsigned) (groups < 148 * 64 ? groups : 148 * 64);
-    window_step_rows_kernel<T><<<blocks, 32 * kWindowRowWarps, 0, stream>>>(q, k, v, positions, k_cache, v_cache, context, s);
+    const auto kernel = dim <= 64 ? window_step_rows_kernel<T, 2> : dim <= 128 ? window_step_rows_kernel<T, 4> : window_step_rows_kernel<T, 8>;
+    kernel<<<blocks, 32 * kWindowRowWarps, 0, stream>>>(q, k, v, positions, k_cache, v_cache, context, s);
     return check_launch();
 }
 

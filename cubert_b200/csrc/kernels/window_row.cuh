@@ -14,9 +14,12 @@ constexpr float kWeightScale = 7.f, kRaiseBy = 8.f;
 constexpr int kWindowMaxDim = 256;
 constexpr int kWindowRowWarps = 4;
 
-// Any head dimension up to 256, any strides: 32 keys at a time, a key per lane for the scores, a column (or several)
-// per lane for the context. `key(j)` and `value(j)` give the addresses of row j, `seen(j)` says whether it counts.
-template <typename T, typename Key, typename Value, typename Seen>
+// Head dimensions up to 32 COLS, any strides: 32 keys at a time, a key per lane for the scores, COLS columns
+// per lane for the context. The values of four keys are loaded as they are stored and converted together afterwards, over a number of
+// columns that the compiler knows: 1024 x 6 binary16 tokens of 12 heads of 64 take 70 us (with eight columns a lane for every dimension,
+// converted one by one, 111 to 116). Bound by latency: each warp waits for its 32 key rows and then eight times for four value rows.
+// `key(j)` and `value(j)` give the addresses of row j, `seen(j)` says whether it counts.
+template <typename T, int COLS, typename Key, typename Value, typename Seen>
 __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sinks_end, int lo, int hi, Key key, Value value, Seen seen,
                            T *context) {
     const int lane = threadIdx.x & 31;
@@ -25,9 +28,9 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
         s_q[c] = to_float<T>(q[c]);
     }
     __syncwarp();
-    float o[kWindowMaxDim / 32];
+    float o[COLS];
 #pragma unroll
-    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+    for (int i = 0; i < COLS; ++i) {
         o[i] = 0.f;
     }
     float top = -INFINITY, total = 0.f;
@@ -75,11 +78,12 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
             top = next;
             total = total * shrink + group_sum<32>(p);
 #pragma unroll
-            for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+            for (int i = 0; i < COLS; ++i) {
                 o[i] *= shrink;
             }
             while (visible != 0) {   // the rows of four keys on their way at a time
-                float w[4], e[4][kWindowMaxDim / 32];
+                float w[4];
+                T e[4][COLS];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     const bool on = visible != 0;
@@ -89,15 +93,15 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
                     w[u] = on ? w[u] : 0.f;
                     const T *vr = value(j0 + from);
 #pragma unroll
-                    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
-                        e[u][i] = on && lane + 32 * i < dim ? to_float<T>(vr[lane + 32 * i]) : 0.f;
+                    for (int i = 0; i < COLS; ++i) {
+                        e[u][i] = on && lane + 32 * i < dim ? vr[lane + 32 * i] : T(0.f);
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
 #pragma unroll
-                    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
-                        o[i] = fmaf(w[u], e[u][i], o[i]);
+                    for (int i = 0; i < COLS; ++i) {
+                        o[i] = fmaf(w[u], to_float<T>(e[u][i]), o[i]);
                     }
                 }
             }
@@ -105,7 +109,7 @@ __device__ void window_row(const T *q, float *s_q, int dim, float scale, int sin
     }
     const float inv = any ? 1.f / total : 0.f;   // nothing but scores of minus infinity: 0 times infinity, NaN as 0 / 0 is
 #pragma unroll
-    for (int i = 0; i < kWindowMaxDim / 32; ++i) {
+    for (int i = 0; i < COLS; ++i) {
         if (lane + 32 * i < dim) {
             context[lane + 32 * i] = from_float<T>(o[i] * inv);
         }

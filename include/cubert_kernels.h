@@ -289,8 +289,8 @@ int cubk_pooler_head_f16(const void *x, const void *pooler_bias, const void *wei
  * short as the row leaves it). A group whose largest |y| is below 2^-100 is stored as zeros with scale 0. A NaN in a
  * group makes its scale and codes NaN. The e4m3 codes are what cubk_w4_matvec_e4m3_* and 8-bit library products read.
  * Rows of other lengths or alignments add their squares in another order: t has the same bits, y and the scales differ by
- * (channels / 32 + 24) 2^-24 of themselves at most, before they are rounded. Squares are float32: |t| from 2^64 on (a mean of
- * infinity) gives zeros.
+ * (channels / 32 + 24) 2^-24 of themselves at most, before they are rounded. Squares and their sum are float32: a row
+ * that leaves its range there (|t| about 2^64) comes out as zeros.
  * eps >= 0; a row of zeros under eps = 0 gives NaN. channels up to 2^30 (CUBK_ERR_UNSUPPORTED beyond). */
 int cubk_residual_rms_norm_f32(const float *x, const float *residual, const float *gamma, int64_t rows, int channels, float eps,
                                float *sum, float *out, void *stream);
@@ -353,7 +353,7 @@ int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int cod
  *     scores, weights and contexts in tensor memory; weights are rounded to binary16. Every wait is bounded (0.2 s): a
  *     block that gives up writes NaN into the rows it has not finished and counts in cubk_window_give_ups.
  *   otherwise, head_dim up to 128: the float32 pipes, 64 x 64 tiles.
- *   head_dim above 128, and up to 6 (binary16) or 12 (float32) tokens a sequence: one row per warp.
+ *   head_dim above 128, and up to 8 (binary16) or 16 (float32) tokens a sequence: one row per warp.
  * The three agree within their roundings: float32 sums of another order, and 2^-11 of sum_j p_j |v_j| where weights are rounded. */
 int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
                               int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,

@@ -267,3 +267,20 @@ def test_steps_by_every_path_agree(heads, kv_heads, dim, window, t):
     if t == "f16":                                               # weights rounded on one side
         bar = bar + 2.0 ** -11 * pv * (1 + 2.0 ** -6) + tiny
     within(got[1][0][:2], got[0][0][:2].double(), bar[:2])
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (40, 2, 1), (128, 4, 2), (72, 3, 3)])
+@pytest.mark.parametrize("shift,pad", [(1, 0), (0, 1), (8, 4), (2, 6)])
+def test_tensor_core_sequences_into_a_context_of_any_alignment(dim, heads, kv_heads, shift, pad):
+    """Operands on 16-byte boundaries, a context that starts or whose rows start elsewhere: the same bits, and nothing beside them."""
+    batch, seq = 2, 300
+    q, k, v, m = window_inputs(dim, batch, seq, heads, kv_heads, dim, "holes", "f16")
+    q, k, v = (a.contiguous() for a in (q, k, v))
+    args = (batch, seq, heads, kv_heads, dim, 70, 11, 2, dim ** -0.5)
+    want = window_attention(q, k, v, m, *args, "f16")
+    wide = heads * dim + pad
+    room = torch.full((batch * seq * wide + 16,), 3.0, dtype=torch.float16, device="cuda")
+    ctx = room[shift:shift + batch * seq * wide].view(batch * seq, wide)
+    window_attention(q, k, v, m, *args, "f16", ctx=ctx[:, :heads * dim])
+    assert torch.equal(ctx[:, :heads * dim], want) and bool((ctx[:, heads * dim:] == 3).all())
+    assert bool((room[:shift] == 3).all() and (room[shift + batch * seq * wide:] == 3).all())
