@@ -58,7 +58,7 @@ window_step_rows_kernel(const T *q, const T *k, const T *v, const int32_t *posit
 // what it took; at the end the blocks read one another's partial sums through distributed shared memory and every block
 // writes its share of the context. Nothing is staged in device memory, so calls need no workspace and no order among them,
 // and the sums are added in the same order every time. The kernels are bound by the cache's bytes: 32 streams of 32 / 8 heads of 128
-// over 2048 slots, binary16, take 39.9 us (5.3 TB/s, 0.82 of what a copy reaches). Small grids are bound by the loads an SM has in
+// over 2048 slots, binary16, take 40.5 us (5.2 TB/s, 0.81 of what a copy reaches). Small grids are bound by the loads an SM has in
 // flight and by two cluster barriers: one such stream with 4096 slots 10.7 us, one float32 stream of 12 heads of 64 with 512 slots 4.5.
 template <int WARPS, int HEADS, int DP>
 struct StepPartial {
@@ -376,16 +376,26 @@ window_step_f16_kernel(const __half *q, const __half *k, const __half *v, const 
                 p[e] = sc[m][e] == -INFINITY ? 0.f : fast_exp2(sc[m][e] - top[m][e & 1]);
                 total[m][e & 1] += p[e];
             }
-            const __half2 lo = __floats2half2_rn(p[0], p[1]), hi = __floats2half2_rn(p[2], p[3]);
-            const uint32_t b0 = transpose_8x8(*reinterpret_cast<const uint32_t *>(&lo)), b1 = transpose_8x8(*reinterpret_cast<const uint32_t *>(&hi));
+            // each weight as two binary16 numbers: 22 bits of it, where one has 11 (32 streams of 32 / 8 heads of 128: 40.5 us, with one 40.15)
+            uint32_t b[2][2];   // high and low parts, keys 0 to 7 and 8 to 15
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const __half2 high = __floats2half2_rn(p[2 * i], p[2 * i + 1]);
+                const float2 back = __half22float2(high);
+                const __half2 low = __floats2half2_rn(p[2 * i] - back.x, p[2 * i + 1] - back.y);
+                b[0][i] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&high));
+                b[1][i] = transpose_8x8(*reinterpret_cast<const uint32_t *>(&low));
+            }
 #pragma unroll
             for (int x = 0; x < VC; ++x) {
                 const uint32_t w0[4] = {vr[0][x].x, vr[0][x].y, vr[0][x].z, vr[0][x].w}, w1[4] = {vr[1][x].x, vr[1][x].y, vr[1][x].z, vr[1][x].w};
                 const uint32_t w2[4] = {vr[2][x].x, vr[2][x].y, vr[2][x].z, vr[2][x].w}, w3[4] = {vr[3][x].x, vr[3][x].y, vr[3][x].z, vr[3][x].w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    mma_f16(o[m][x][i], __byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x5410),
-                            __byte_perm(w2[i], w3[i], 0x7632), b0, b1);
+                    const uint32_t a[4] = {__byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x5410),
+                                           __byte_perm(w2[i], w3[i], 0x7632)};
+                    mma_f16(o[m][x][i], a[0], a[1], a[2], a[3], b[1][0], b[1][1]);
+                    mma_f16(o[m][x][i], a[0], a[1], a[2], a[3], b[0][0], b[0][1]);
                 }
             }
         }

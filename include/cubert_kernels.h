@@ -374,8 +374,8 @@ int cubk_window_give_ups(unsigned int *count);
  * causal form above with before = window - 1. A stream with a negative position is idle: its cache and its row of
  * context are left as they are. Slots that no position has reached may hold anything. Positions are read on the
  * device, so a captured call can be replayed as they advance; calls that share a cache must be ordered.
- * _f16, head_dim a multiple of 8 up to 128, rows and heads on 16-byte boundaries: weights are rounded to binary16 (2^-11 of each at
- * most) for the tensor cores; in any other form they are float32.
+ * _f16, head_dim a multiple of 8 up to 128, rows and heads on 16-byte boundaries: weights meet the tensor cores as two binary16
+ * parts (2^-22 of each at most, and 2^-32 of a row's largest where they are small); in any other form they are float32.
  * Binary16 heads that come out not finite from finite scores (an infinity or a NaN in a visible value) are computed again with float32
  * weights by a warp each, which is slow; weights below 2^-126 of a row's largest count as 0 in every form. */
 int cubk_window_attention_step_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride,

@@ -284,3 +284,25 @@ def test_tensor_core_sequences_into_a_context_of_any_alignment(dim, heads, kv_he
     window_attention(q, k, v, m, *args, "f16", ctx=ctx[:, :heads * dim])
     assert torch.equal(ctx[:, :heads * dim], want) and bool((ctx[:, heads * dim:] == 3).all())
     assert bool((room[:shift] == 3).all() and (room[shift + batch * seq * wide:] == 3).all())
+
+
+# ============================================================================ K8: bits of a weight
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 64), (8, 2, 128), (16, 1, 64), (32, 2, 128)])
+def test_step_weights_keep_22_bits(heads, kv_heads, dim):
+    """Few keys whose values nearly cancel: the context is small beside its terms, and so is its own rounding beside that of a weight
+    held in 11 bits. Scores are one product each."""
+    batch, slots, g = 64, 6, gen(dim + heads)
+    q = torch.zeros((batch, heads * dim), dtype=torch.float16, device="cuda")
+    q[:, 0::dim] = 1.0
+    k, v = torch.zeros((batch, kv_heads * dim), dtype=torch.float16, device="cuda"), normal(g, batch, kv_heads * dim, t="f16")
+    kc, vc = torch.zeros((batch, kv_heads, slots, dim), dtype=torch.float16, device="cuda"), normal(g, batch, kv_heads, slots, dim, t="f16")
+    kc[..., 0] = torch.rand((batch, kv_heads, slots), generator=g, device="cuda").half()
+    pos = torch.full((batch,), 4 * slots + 1, dtype=torch.int32, device="cuda")
+    ctx = torch.zeros((batch, heads * dim), dtype=torch.float16, device="cuda")
+    step(q, k, v, pos, batch, heads, kv_heads, dim, slots, 0, 1.0, kc, vc, ctx, "f16")
+    share = heads // kv_heads
+    want, bar, pv, _ = attention64(q.reshape(batch, heads, 1, dim).double(), kc.double().repeat_interleave(share, 1),
+                                   vc.double().repeat_interleave(share, 1), torch.ones((batch, 1, 1, slots), dtype=torch.bool, device="cuda"), 1.0, dim)
+    # two binary16 parts of a weight: half a step of the second is 2^-22 of it at most; then the result's rounding
+    within(ctx, want, bar + 2.0 ** -22 * pv + 2.0 ** -11 * want.abs() * (1 + 2.0 ** -8) + 2.0 ** -25)
