@@ -37,7 +37,8 @@ __device__ __forceinline__ float group_max_nan(float v) {
     return v;
 }
 
-// Rows of any length and alignment up to 128 * GROUPS * WARPS elements: in registers too, an element at a time. A warp takes groups of
+// Rows of any length and alignment up to 128 * GROUPS * WARPS elements: in registers too, an element at a time, and so bound by issue
+// (8000 x 1001 binary16: 17 us, 73 % of the issue slots). A warp takes groups of
 // 128 columns, four elements a lane, so that a group's largest magnitude stays within it. One warp a row (four rows a block) or a block.
 template <typename T, int WARPS, int GROUPS, NormOut OUT>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : 32 * WARPS)
@@ -143,7 +144,8 @@ rms_norm_elements_kernel(const T *x, const T *residual, const T *gamma, int64_t 
 constexpr int kRmsGenericBlock = 256;
 
 // Any row length and alignment: a block per row, three passes over it (sum of squares, largest magnitude of
-// each group, output); x and residual are read again from L2 in each.
+// each group, output); x and residual are read again from L2 in each. 2000 x 20000 binary16: 100 us, with residual and scales per 128
+// columns, whose groups are two barriers each, 452.
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(kRmsGenericBlock)
 rms_norm_generic_kernel(const T *x, const T *residual, const T *gamma, int64_t rows, int channels, float eps, int group,
@@ -416,7 +418,7 @@ int residual_rms_norm(const T *x, const T *residual, const T *gamma, int64_t row
             return rc;
         }
     }
-    if (channels <= 128 * 4 * 16) {   // 8000 x 1001 binary16: 24 us, with the three passes below 37
+    if (channels <= 128 * 4 * 16) {   // 8000 x 1001 binary16: 17 us, with the three passes below 23
 #define ELEMENTS(WARPS, GROUPS, OUT)                                                                                                        \
     do {                                                                                                                                    \
         const int64_t want = WARPS == 1 ? (rows + 3) / 4 : rows, most = 148 * (WARPS == 16 ? 4 : 16);                                       \

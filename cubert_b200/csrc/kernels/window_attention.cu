@@ -53,7 +53,7 @@ window_rows_kernel(const T *q, const T *k, const T *v, const int8_t *mask, T *co
 // x 4 keys of the scores and 8 rows x DP / 16 columns of the context; Q and K are transposed on their way into shared memory, so that
 // each step of a reduction is two or three 16-byte reads for 32 or 64 multiply-adds, issued in pairs of rows. The 16 threads of a row
 // are half a warp: maxima and sums need shuffles only. Bound by the multiply-adds, and for short windows by the latency of a block's
-// two or three steps: 3 x 777 tokens, 12 heads of 64, window 131, half of the keys masked: 40 to 46 us, 468 blocks in 1.05 waves.
+// two or three steps: 3 x 777 tokens, 12 heads of 64, window 131, half of the keys masked: 37 us, 468 blocks in 1.05 waves.
 constexpr int kPlainRows = 64, kPlainKeys = 64, kPlainThreads = 128;
 
 template <int DP>
@@ -418,7 +418,7 @@ int window_plain(const T *q, const T *k, const T *v, const int8_t *mask, T *cont
 // its tensor cores (heads of 64; 1024 for heads of 128), a step 1500. Measured: 8192 tokens, 32 / 8 heads of 128, window 2048: 265 to
 // 290 us by the clock under the power cap (840 to 910 TFLOP/s); 4 x 4096 tokens, 16 heads of 64, no window 400 us, window 513 and ragged
 // lengths 81 us (3 steps an item that ran; half of it goes into the ends of items). Rows computed
-// again are far slower: one causal sequence of 40000 tokens, 2 heads of 64, all of it from token 100 on: 542 ms (1.2 ms without). Tried
+// again are far slower: one causal sequence of 40000 tokens, 2 heads of 64, all of it from token 100 on: 180 ms (0.64 ms without). Tried
 // and slower: two threads a row, part of the exponentials by polynomial, scores of 96 keys twice, masks gathered by a warp of their own.
 // Every wait is bounded; a block that gives up writes NaN into the rows of the items it has not finished, counts in g_window_give_ups,
 // frees its tensor memory and returns.

@@ -306,7 +306,7 @@ int cubk_residual_rms_norm_e4m3_f16(const void *x, const void *residual, const v
  * For requests of a few tokens, whose dense products do nothing but read weights. No counterpart in the reference,
  * whose products are float32 or binary16 library calls (src/cuBERT/op/Dense.cpp:41-52). Up to 1048560 rows are computed
  * (CUBK_ERR_UNSUPPORTED beyond), but with more than a few a library product of binary16 weights, where there is room for
- * them, takes no longer: from 16 rows on at 4096 by 4096, from about 28 at 4096 by 11008; a third of the time at 128 rows.
+ * them, takes no longer: from 16 rows on at 4096 by 4096, from about 28 at 4096 by 11008; 0.43 and 0.34 of the time at 128.
  * x [rows, k], bias [n] (or NULL), out [rows, n] and the scales [ceil(k / group), n] in the storage type. Sums are
  * float32, of x times codes over a group before they meet its scale (float32 x beyond 2^118 can overflow there); a code
  * times its scale is never rounded. x of any alignment gives the same bits; the order of the sums depends on rows, k and n.
@@ -353,7 +353,8 @@ int cubk_w4_matvec_e4m3_f16(const void *codes, const float *code_scales, int cod
  *     scores, weights and contexts in tensor memory; weights are rounded to binary16. Every wait is bounded (0.2 s): a
  *     block that gives up writes NaN into the rows it has not finished and counts in cubk_window_give_ups.
  *   otherwise, head_dim up to 128: the float32 pipes, 64 x 64 tiles.
- *   head_dim above 128, and up to 8 (binary16) or 16 (float32) tokens a sequence: one row per warp.
+ *   head_dim above 128, and up to 8 (binary16) or 16 (float32) tokens a sequence: one row per warp. Long sequences take far longer so:
+ *     8 heads of 256, 2048 causal tokens, 3.4 ms in binary16 (of 128, 42 us) and 5.2 ms in float32.
  * The three agree within their roundings: float32 sums of another order, and 2^-11 of sum_j p_j |v_j| where weights are rounded. */
 int cubk_window_attention_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride, const int8_t *mask,
                               int batch, int seq, int heads, int kv_heads, int head_dim, int before, int after, int sinks, float scale,
@@ -376,6 +377,8 @@ int cubk_window_give_ups(unsigned int *count);
  * device, so a captured call can be replayed as they advance; calls that share a cache must be ordered.
  * _f16, head_dim a multiple of 8 up to 128, rows and heads on 16-byte boundaries: weights meet the tensor cores as two binary16
  * parts (2^-22 of each at most, and 2^-32 of a row's largest where they are small); in any other form they are float32.
+ * head_dim above 128, and rows or heads off 16-byte boundaries: one head per warp, which takes far longer (one stream, 8 heads of 256,
+ * 2048 slots: 1.3 ms; of 128 on 16-byte boundaries 7 us).
  * Binary16 heads that come out not finite from finite scores (an infinity or a NaN in a visible value) are computed again with float32
  * weights by a warp each, which is slow; weights below 2^-126 of a row's largest count as 0 in every form. */
 int cubk_window_attention_step_f32(const float *q, const float *k, const float *v, int64_t q_stride, int64_t kv_stride,
