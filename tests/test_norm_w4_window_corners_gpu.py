@@ -306,3 +306,23 @@ def test_step_weights_keep_22_bits(heads, kv_heads, dim):
                                    vc.double().repeat_interleave(share, 1), torch.ones((batch, 1, 1, slots), dtype=torch.bool, device="cuda"), 1.0, dim)
     # two binary16 parts of a weight: half a step of the second is 2^-22 of it at most; then the result's rounding
     within(ctx, want, bar + 2.0 ** -22 * pv + 2.0 ** -11 * want.abs() * (1 + 2.0 ** -8) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("pad", [0, 1])
+def test_long_rows_of_minus_infinity_and_of_nothing(pad, t):
+    """Three keys of 9000: one whose score is minus infinity, then one that is not."""
+    seq, dim = 9000, 64
+    q, k, v, _ = window_inputs(17, 1, seq, 1, 1, dim, None, t, pad)
+    q.abs_().add_(0.125)
+    k[5, 0] = -INF
+    m = torch.zeros((1, seq), dtype=torch.int8, device="cuda")
+    m[0, [5, 4600, 8901]] = 1
+    got = window_attention(q, k, v, m, 1, seq, 1, 1, dim, seq, 0, 0, dim ** -0.5, t)
+    assert bool((got[:5] == 0).all()) and torch.isnan(got[5:4600]).all()
+    assert torch.equal(got[4600:8901], v[4600:4601].expand(4301, dim))
+    s = q[8901:].double() @ k[[4600, 8901]].double().t() * dim ** -0.5
+    want, pv = torch.softmax(s, 1) @ v[[4600, 8901]].double(), torch.softmax(s, 1) @ v[[4600, 8901]].double().abs()
+    # scores of up to 64 (72 steps of float32), the exponential, then weights and result in binary16 at the most
+    half = 2.0 ** -11 if t == "f16" else 2.0 ** -24
+    within(got[8901:], want, pv * (2 * 64 * 72 * 2.0 ** -23 + 2.0 ** -18 + half * (1 + 2.0 ** -6)) + half * want.abs() + 2.0 ** -25)
